@@ -42,6 +42,7 @@
 #include <stdlib.h>
 
 #include "kmb_common.cuh"
+#include "tc_ptx.cuh"
 
 namespace kmb {
 
@@ -107,46 +108,6 @@ struct TcParams {
 };
 
 // ---------------------------------------------------------------------------- PTX
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ void mbar_init(void* bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(void* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(void* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
-               "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(void* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// The same test, but the hardware may keep the thread asleep for up to `hint_ns` nanoseconds
-// while the phase is incomplete: a waiting warp then costs no issue slots (a spinning one
-// competes with the epilogue warps for the integer pipe).
-__device__ __forceinline__ bool mbar_try_wait_sleep(void* bar, uint32_t parity, uint32_t hint_ns) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(hint_ns)
-      : "memory");
-  return ok != 0;
-}
-
 // Bounded wait: false when the CTA is aborting or the time limit ran out.
 __device__ __forceinline__ bool mbar_wait(void* bar, uint32_t parity, TcSmem* sm, int* error_flag,
                                           uint32_t sleep_ns = 0u) {
@@ -168,75 +129,6 @@ __device__ __forceinline__ bool mbar_wait(void* bar, uint32_t parity, TcSmem* sm
   }
 }
 
-// Leaving an aborting CTA: wait, for about a millisecond at most, until phase `parity` of a
-// barrier has completed.
-__device__ __forceinline__ void drain_wait(void* bar, uint32_t parity) {
-  for (int i = 0; i < 4096; ++i) {
-    if (mbar_try_wait(bar, parity)) return;
-    __nanosleep(256);
-  }
-}
-// A producer that armed the `full` barriers of a ring of n_slots slots for items 0 .. issued - 1
-// (item i -> slot i mod n_slots, phase (i / n_slots) & 1) waits for the last copy into every slot,
-// so that no bulk copy is still writing this CTA's shared memory when the CTA exits.
-__device__ __forceinline__ void drain_ring(unsigned long long* bars, uint32_t n_slots, uint32_t issued) {
-  for (uint32_t s = 0; s < n_slots && s < issued; ++s) {
-    const uint32_t last = s + ((issued - 1u - s) / n_slots) * n_slots;
-    drain_wait(&bars[s], (last / n_slots) & 1u);
-  }
-}
-__device__ __forceinline__ void fence_barrier_init() {
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-}
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y,
-                                            void* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
-      "%4}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_alloc(void* smem_dst, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                   smem_u32(smem_dst)),
-               "r"(ncols)
-               : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
-               : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void umma_commit(void* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
-        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
-        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -248,9 +140,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
       "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
       "r"(v[30]), "r"(v[31])
       : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 // A operand read from tensor memory (lane = row, one 32-bit column per tf32 element).
 __device__ __forceinline__ void umma_tf32_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
@@ -266,38 +155,6 @@ __device__ __forceinline__ void umma_tf32_ts(uint32_t d_tmem, uint32_t a_tmem, u
 // of a whole sample tile then runs on the ALU instead of the conversion unit.
 __device__ __forceinline__ float tf32_round_alu(float x) {
   return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
-}
-
-// One lane of a converged warp (warp-uniform predicate).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t pred;
-  asm volatile(
-      "{\n\t.reg .pred P;\n\t"
-      "elect.sync _|P, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, P;\n\t}"
-      : "=r"(pred));
-  return pred != 0;
-}
-// Aborting CTA: the elected lane of an MMA warp commits once more, to a barrier nobody else uses,
-// and waits (bounded) for it: all MMAs it issued have then completed.
-__device__ __forceinline__ void mma_drain(void* bar) {
-  if (elect_one()) {
-    umma_commit(bar);
-    drain_wait(bar, 0u);
-  }
-  __syncwarp();
-}
-
-// Shared-memory matrix descriptor of a K-major, 128B-swizzled tile whose rows are 128 bytes
-// apart and whose 8-row groups are 1024 bytes apart.
-__device__ __forceinline__ uint64_t make_sdesc(uint32_t saddr) {
-  uint64_t desc = 0;
-  desc |= (uint64_t)((saddr & 0x3FFFF) >> 4);   // start address, 16-byte units
-  desc |= (uint64_t)1 << 16;                    // leading byte offset (unused with swizzle)
-  desc |= (uint64_t)(1024 >> 4) << 32;          // stride byte offset between 8-row groups
-  desc |= (uint64_t)1 << 46;                    // descriptor version of sm_100
-  desc |= (uint64_t)2 << 61;                    // SWIZZLE_128B
-  return desc;
 }
 
 // kind::tf32, fp32 accumulate, both operands K-major, M = 128, N = 128.
@@ -1322,24 +1179,6 @@ __global__ void tc_split_centroids_kernel(const float* __restrict__ C, const flo
 }
 
 // ------------------------------------------------------------------------------ host
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn get_encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (fn == nullptr) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) ==
-            cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      fn = (EncodeTiledFn)ptr;
-  }
-  return fn;
-}
-
 // (rows, cols) fp32 row-major tensor with row stride ld (elements); box = 32 cols x 128 rows.
 static int make_map(CUtensorMap* map, const float* base, int64_t rows, int cols, int64_t ld) {
   EncodeTiledFn fn = get_encode_fn();
