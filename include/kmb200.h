@@ -30,7 +30,8 @@
 extern "C" {
 #endif
 
-typedef enum { KMB_F32 = 0, KMB_F64 = 1 } kmb_dtype;
+/* KMB_F16 and KMB_BF16 are types of the expert and 8-bit calls at the end of this file only. */
+typedef enum { KMB_F32 = 0, KMB_F64 = 1, KMB_F16 = 2, KMB_BF16 = 3 } kmb_dtype;
 
 typedef enum {
   KMB_OK = 0,
@@ -386,6 +387,73 @@ int kmb_matmul_nt(int dtype, int algo, const void* X, const void* Y, void* out, 
  * least 8 * 256 * (SM count) elements of `dtype` (never written in practice).  Waits for the
  * stream.  No counterpart in the reference. */
 int kmb_measure_fma_peak(int dtype, int repeats, double* tflops, void* scratch, void* stream);
+
+/* ---- mixture of experts -------------------------------------------------------------
+ * `dtype` is KMB_F32, KMB_F16 or KMB_BF16 in these calls; arithmetic is in 32 bits or more.
+ * None of them has a counterpart in the reference. */
+enum {
+  KMB_ROUTE_SIGMOID = 1,     /* scores by sigmoid, not by softmax over the experts          */
+  KMB_ROUTE_RENORMALIZE = 2  /* a token's weights are divided by their sum                   */
+};
+
+/* Routing.  logits (n, n_experts); s = softmax or sigmoid of them; key = s + bias (n_experts floats, or
+ * NULL).  With groups > 1 the experts fall into consecutive groups of equal size, a group's score is the
+ * sum of its group_best (1 or 2) greatest keys, and only the topk_groups best groups are looked at.  The k
+ * greatest keys are chosen: descending, lowest index among equals, NaN greatest, as kmb_topk orders
+ * them; the order is that of the keys in 64 bits.  Without a bias experts are ordered by their logits, and
+ * so are groups with group_best = 1.
+ * experts (n, k) int32; weights (n, k) float: scale * s of the chosen, over their sum with
+ * KMB_ROUTE_RENORMALIZE.  An expert whose logit (or key) is -inf is never chosen: places left over hold
+ * expert -1 and weight 0.  n_experts <= 1024, k <= 32, groups <= 32. */
+int kmb_route_topk(int dtype, const void* logits, const float* bias, int64_t n, int n_experts, int k,
+                   int flags, int groups, int topk_groups, int group_best, float scale, float* weights,
+                   int32_t* experts, void* stream);
+/* grad_logits (n, n_experts) from grad_weights (n, k), the choice being held fixed.  An `experts` entry
+ * outside [0, n_experts) is no choice; the entries of a row must differ otherwise. */
+int kmb_route_topk_grad(int dtype, const void* logits, const int32_t* experts, const float* grad_weights,
+                        int64_t n, int n_experts, int k, int flags, float scale, void* grad_logits,
+                        void* stream);
+
+/* Expert order of the n * k choices: sorted by expert, token order kept within one.  slots (n, k): place of
+ * each choice; rows (n * k): token in each place; offsets (n_experts + 1): first place of each expert.
+ * A choice outside [0, n_experts) has slot -1, and rows behind offsets[n_experts] are -1.
+ * n_experts <= 1024. */
+int kmb_expert_slots(const int32_t* experts, int64_t n, int k, int n_experts, int32_t* slots, int32_t* rows,
+                     int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream);
+size_t kmb_expert_slots_workspace_bytes(int64_t n, int k, int n_experts);
+
+/* out (n, d): out[t] = sum_j weights[t, j] * values[slots[t, j]], values (n_values, d); a slot outside
+ * [0, n_values) adds nothing, whatever its weight. */
+int kmb_combine_experts(int dtype, const void* values, int64_t n_values, const int32_t* slots,
+                        const float* weights, int64_t n, int k, int d, void* out, void* stream);
+/* grad_values (n_values, d) and grad_weights (n, k) from grad_out (n, d).  Rows that several choices share
+ * get the sum of their gradients in ascending order of the choices, rows that nobody chose get zeros. */
+int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, const int32_t* slots,
+                             const float* weights, const void* grad_out, int64_t n, int k, int d,
+                             void* grad_values, float* grad_weights, void* workspace, size_t workspace_bytes,
+                             void* stream);
+size_t kmb_combine_experts_grad_workspace_bytes(int64_t n_values);
+
+/* ---- products in 8-bit integers ------------------------------------------------------- */
+/* q[i, f] = round_half_even(127 x[r, f] / max_f |x[r, f]|) and scales[i] = max_f |x[r, f]| / 127 with
+ * r = rows[i], or i when rows is NULL (then m = n).  x (n, d) of `dtype`; q (m, d) at a pitch of q_pitch
+ * bytes (a multiple of 16; bytes between d and the pitch may be overwritten).  The rounding is that of the
+ * exact quotient.  A row outside [0, n) or of zeros gives zeros and scale 0; a row that holds an
+ * infinity or NaN gives zeros and scale NaN. */
+int kmb_quantize_rows(int dtype, const void* x, int64_t n, int d, const int32_t* rows, int64_t m,
+                      int8_t* q, int64_t q_pitch, float* scales, void* stream);
+/* out[i, j] = a_scales[i] * b_scales[g, j] * sum_f a[i, f] * b[g, j, f] + bias[g, j], for the rows
+ * offsets[g] <= i < offsets[g + 1] of every group g; offsets (groups + 1 int32 on the device, ascending) may
+ * be NULL with groups = 1: all m rows.  Rows behind offsets[groups] become zeros.  a (m, d) and
+ * b (groups * n, d) are row-major at pitches lda and ldb (bytes, multiples of 16) and 16-byte aligned;
+ * bias (groups * n) may be NULL.  out (m, n) of out_dtype.  d <= 131071, groups <= 1024. */
+int kmb_int8_matmul(int out_dtype, const int8_t* a, int64_t lda, const float* a_scales, const int8_t* b,
+                    int64_t ldb, const float* b_scales, const float* bias, const int32_t* offsets,
+                    int groups, void* out, int64_t m, int n, int d, void* stream);
+/* Whether a bounded wait of kmb_int8_matmul ran out on the current device since the last call of this
+ * function: KMB_ERR_CUDA and *flag = 1 then (the tiles concerned hold NaN), and the flag is cleared.
+ * Waits for the stream. */
+int kmb_int8_wait_error(int* flag, void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,11 +14,12 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libkmb200.so")
 
-KMB_F32, KMB_F64 = 0, 1
+KMB_F32, KMB_F64, KMB_F16, KMB_BF16 = 0, 1, 2, 3
 KMB_OK, KMB_ERR_INVALID, KMB_ERR_CUDA, KMB_ERR_UNSUPPORTED, KMB_ERR_WORKSPACE = 0, -1, -2, -3, -4
 ALGO_AUTO, ALGO_CUDA_CORE, ALGO_TF32X3 = 0, 1, 2
 ALGO_NAMES = {"auto": ALGO_AUTO, "cuda_core": ALGO_CUDA_CORE, "tf32x3": ALGO_TF32X3}
 STEP_ACC_CLEARED, STEP_OPERANDS_READY = 1, 2
+ROUTE_SIGMOID, ROUTE_RENORMALIZE = 1, 2
 FIN_MERGE, FIN_CLEAR_ACC, FIN_PREPARE_TF32X3 = 1, 2, 4
 
 
@@ -87,6 +88,19 @@ _SIGNATURES = {
     "kmb_u64_to_unit_f64": (c_double, [c_uint64]),
     "kmb_measure_fma_peak": (c_int, [c_int, c_int, POINTER(c_double), _P, _P]),
     "kmb_matmul_nt": (c_int, [c_int, c_int, _P, _P, _P, c_int64, c_int, c_int, _P, c_size_t, _P]),
+    "kmb_route_topk": (c_int, [c_int, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,
+                               c_float, _P, _P, _P]),
+    "kmb_route_topk_grad": (c_int, [c_int, _P, _P, _P, c_int64, c_int, c_int, c_int, c_float, _P, _P]),
+    "kmb_expert_slots": (c_int, [_P, c_int64, c_int, c_int, _P, _P, _P, _P, c_size_t, _P]),
+    "kmb_expert_slots_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "kmb_combine_experts": (c_int, [c_int, _P, c_int64, _P, _P, c_int64, c_int, c_int, _P, _P]),
+    "kmb_combine_experts_grad": (c_int, [c_int, _P, c_int64, _P, _P, _P, c_int64, c_int, c_int, _P, _P,
+                                         _P, c_size_t, _P]),
+    "kmb_combine_experts_grad_workspace_bytes": (c_size_t, [c_int64]),
+    "kmb_quantize_rows": (c_int, [c_int, _P, c_int64, c_int, _P, c_int64, _P, c_int64, _P, _P]),
+    "kmb_int8_matmul": (c_int, [c_int, _P, c_int64, _P, _P, c_int64, _P, _P, _P, c_int, _P, c_int64,
+                                c_int, c_int, _P]),
+    "kmb_int8_wait_error": (c_int, [POINTER(c_int), _P]),
 }
 
 class LloydPlan(ctypes.Structure):
@@ -144,6 +158,17 @@ def dtype_code(torch_dtype):
     raise ValueError(f"Expected float32 or float64 data but got {torch_dtype}")
 
 
+_ROW_TYPES = {torch.float32: KMB_F32, torch.float16: KMB_F16, torch.bfloat16: KMB_BF16}
+
+
+def row_dtype_code(torch_dtype, name):
+    """Type code of the expert and 8-bit calls, which take rows in 16 or 32 bits."""
+    code = _ROW_TYPES.get(torch_dtype)
+    if code is None:
+        raise ValueError(f"{name} must have dtype float32, float16 or bfloat16, got {torch_dtype}")
+    return code
+
+
 def ptr(t):
     """Device (or host) address of a tensor's first element; None -> NULL."""
     if t is None:
@@ -153,6 +178,25 @@ def ptr(t):
 
 def stream_ptr(device=None):
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+class on_device_of:
+    """Makes a tensor's device the current one for a call: the library asks the current device for
+    its size, and launches go to a stream of that device."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, t):
+        self.index = t.device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
 
 
 def require_cuda_tensor(t, name, dtype=None, contiguous=True):

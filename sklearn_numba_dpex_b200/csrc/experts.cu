@@ -1,0 +1,940 @@
+// Mixture of experts around the experts' products: routing of tokens to experts (with its gradient),
+// the expert order of the chosen rows, and the weighted sum that brings the experts' rows back to
+// their tokens (with its gradients).  No counterpart in the reference; routing stands beside the
+// top-k of topk.cu and keeps its order (greatest first, lowest index among equals, NaN greatest).
+#include <limits.h>
+
+#include "kmb_common.cuh"
+#include "row_types.cuh"
+
+namespace kmb {
+
+constexpr unsigned FULL = 0xffffffffu;
+
+// ================================================================================== routing
+// One warp per token.  Lane l holds the V consecutive experts l * V .. l * V + V - 1 in registers, so
+// that the lowest lane among equals is the lowest index.
+constexpr int RT_WARPS = 4;
+constexpr int RT_MAX_EXPERTS = 1024;
+constexpr int RT_MAX_K = 32;       // the choices of a token live one to a lane
+constexpr int RT_MAX_GROUPS = 32;  // and so do its groups
+
+struct RouteParams {
+  const void* logits;
+  const float* bias;        // or NULL
+  float* weights;
+  int32_t* experts;
+  int64_t n;
+  int n_experts, k, groups, topk_groups, group_best, group_size;
+  int sigmoid, renormalize, vec;
+  float scale;
+};
+
+// Whole numbers in the order of the values, NaN on top; 0 is below everything, -inf among it.
+__device__ __forceinline__ uint32_t order_bits(float v) {
+  if (v != v) return 0xffffffffu;
+  uint32_t b = __float_as_uint(v + 0.f);      // -0 and 0 are one value
+  b ^= (b >> 31) ? 0xffffffffu : 0x80000000u;
+  return b == 0x007fffffu ? 0u : b;           // -inf: never chosen
+}
+__device__ __forceinline__ unsigned long long order_bits(double v) {
+  if (v != v) return 0xffffffffffffffffull;
+  unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
+  b ^= (b >> 63) ? 0xffffffffffffffffull : 0x8000000000000000ull;
+  return b == 0x000fffffffffffffull ? 0ull : b;
+}
+__device__ __forceinline__ uint32_t warp_max_bits(uint32_t v) { return __reduce_max_sync(FULL, v); }
+__device__ __forceinline__ unsigned long long warp_max_bits(unsigned long long v) {
+  const uint32_t hi = (uint32_t)(v >> 32), top = __reduce_max_sync(FULL, hi);
+  const uint32_t lo = __reduce_max_sync(FULL, hi == top ? (uint32_t)v : 0u);
+  return ((unsigned long long)top << 32) | lo;
+}
+__device__ __forceinline__ float from_order_bits(uint32_t b) {
+  if (b == 0u) return __int_as_float(0xff800000);
+  return __uint_as_float((b >> 31) ? b ^ 0x80000000u : ~b);
+}
+template <typename K>
+struct OrderBits;
+template <>
+struct OrderBits<float> { typedef uint32_t type; };
+template <>
+struct OrderBits<double> { typedef unsigned long long type; };
+
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+
+template <typename K>
+__device__ __forceinline__ K warp_sum_of(K v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  return v;
+}
+
+// What a pass over one token finds: lane j < k holds choice j.
+struct Chosen {
+  int expert;      // or -1
+  float logit;
+  bool unsure;     // (32 bits) two values that the choice hangs on lie closer than they are exact
+};
+
+// Scores, keys, groups and choice of one token in arithmetic of type K.
+//
+// In 32 bits the keys carry rounding errors, and two keys closer than `margin` may be in the wrong
+// order.  The errors: the exponential 2 ulp, its argument's rounding |x - top| 2^-24 against a factor
+// exp(x - top) (at most 0.37 ulp of the largest score), the sum of the scores V + 5 additions of 2^-24
+// each, the quotient, the bias's addition.  (V + 16) 2^-24 of the largest score and key covers both
+// keys of a pair.  A token with such a pair (about one in a hundred) is done again in 64 bits, which
+// is what the definition says.  Equal logits with equal biases have equal keys and need no second look.
+template <typename K, int V>
+__device__ __noinline__ Chosen route_token(const RouteParams& p, const float (&x)[V], int lane, bool by_logit,
+                                           float* s_keys) {
+  typedef typename OrderBits<K>::type B;
+  constexpr bool narrow = sizeof(K) == 4;
+  const int e0 = lane * V;
+  const K ninf = -(K)INFINITY;
+  K key[V];
+  K margin = 0;
+  if (by_logit) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = (K)x[i];
+  } else {
+    K top_score = 1;
+    if (p.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) key[i] = (K)1 / ((K)1 + exp_of(-(K)x[i]));
+    } else {
+      uint32_t t = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) t = max(t, order_bits(x[i]));
+      t = warp_max_bits(t);
+      const K top = t == 0xffffffffu ? (K)NAN : t == 0u ? (K)0 : (K)from_order_bits(t);
+      K sum = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        key[i] = exp_of((K)x[i] - top);
+        sum += key[i];
+      }
+      sum = warp_sum_of(sum);
+      sum = sum == (K)0 ? (K)1 : sum;
+#pragma unroll
+      for (int i = 0; i < V; ++i) key[i] = key[i] / sum;
+      top_score = (K)1 / sum;
+    }
+    K most = 0;
+    if (p.bias) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int e = e0 + i;
+        if (e < p.n_experts) key[i] += (K)p.bias[e];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (x[i] == -INFINITY) key[i] = ninf;
+      if (narrow && key[i] > ninf) most = fmaxf((float)most, fabsf((float)key[i]));
+    }
+    if (narrow) {
+      uint32_t m = __float_as_uint((float)most);
+      m = __reduce_max_sync(FULL, m);
+      margin = (K)((float)(V + 16) * 0x1p-24f) * (top_score + (K)__uint_as_float(m));
+    }
+  }
+  bool unsure = false;
+
+  if (p.groups > 1) {
+    // lane g works out the score of group g from the keys in shared memory
+    K* keys = reinterpret_cast<K*>(s_keys);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (e0 + i < p.n_experts) keys[e0 + i] = key[i];
+    __syncwarp();
+    K score = ninf;
+    B bits = 0;
+    if (lane < p.groups) {
+      const K* mine = keys + lane * p.group_size;
+      B b1 = 0, b2 = 0;      // the two greatest of the group
+      K v1 = ninf, v2 = ninf;
+      for (int i = 0; i < p.group_size; ++i) {
+        const K v = mine[i];
+        const B b = order_bits(v);
+        if (b > b1) {
+          b2 = b1; v2 = v1;
+          b1 = b; v1 = v;
+        } else if (b > b2) {
+          b2 = b; v2 = v;
+        }
+      }
+      score = p.group_best == 2 ? v1 + v2 : v1;
+      bits = order_bits(score);
+    }
+    int rank = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const B other = __shfl_sync(FULL, bits, g);
+      if (other > bits || (other == bits && g < lane)) ++rank;
+    }
+    const bool kept = lane < p.groups && rank < p.topk_groups;
+    if (narrow && !by_logit) {
+      const unsigned last_m = __ballot_sync(FULL, lane < p.groups && rank == p.topk_groups - 1);
+      const unsigned next_m = __ballot_sync(FULL, lane < p.groups && rank == p.topk_groups);
+      if (next_m) {
+        const K a = __shfl_sync(FULL, score, __ffs(last_m) - 1), b = __shfl_sync(FULL, score, __ffs(next_m) - 1);
+        if (a > ninf && !(a - b > 3 * margin)) unsure = true;
+      }
+    }
+    const unsigned mask = __ballot_sync(FULL, kept);
+    int g = e0 / p.group_size, left = (g + 1) * p.group_size - e0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      // without a bias the order of the scores is the logits' own, and that is exact
+      if (!((mask >> (g & 31)) & 1u)) key[i] = ninf;
+      else if (!p.bias) key[i] = (K)x[i];
+      if (--left == 0) {
+        ++g;
+        left = p.group_size;
+      }
+    }
+  }
+
+  B bits[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) bits[i] = e0 + i < p.n_experts ? order_bits(key[i]) : (B)0;
+  B best = 0;
+  int best_i = 0;
+  float best_x = 0.f;
+  K best_key = ninf;
+  auto rescan = [&]() {
+    best = 0;
+#pragma unroll
+    for (int i = V - 1; i >= 0; --i)
+      if (bits[i] >= best) {
+        best = bits[i];
+        best_i = i;
+        best_x = x[i];
+        best_key = key[i];
+      }
+  };
+  rescan();
+  Chosen c = {-1, 0.f, false};
+  K mine = ninf, next = ninf;
+  float next_x = 0.f;
+  int next_e = -1;
+  const bool check = narrow && p.bias != nullptr;
+  const int rounds = check ? p.k + 1 : p.k;      // the first that is left out counts too
+  for (int j = 0; j < rounds; ++j) {
+    const B top = warp_max_bits(best);
+    if (top == 0) break;
+    const int w = __ffs(__ballot_sync(FULL, best == top)) - 1;
+    const int e = __shfl_sync(FULL, e0 + best_i, w);
+    const float ex = __shfl_sync(FULL, best_x, w);
+    const K ek = check ? __shfl_sync(FULL, best_key, w) : (K)0;
+    if (lane == j && j < p.k) {
+      c.expert = e;
+      c.logit = ex;
+      mine = ek;
+    }
+    if (lane == j - 1) {
+      next = ek;
+      next_x = ex;
+      next_e = e;
+    }
+    if (lane == w) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i == best_i) bits[i] = 0;
+      rescan();
+    }
+  }
+  if (check) {
+    bool close = lane < p.k && next_e >= 0 && !(mine - next > margin);
+    if (close && c.logit == next_x && p.bias[c.expert] == p.bias[next_e]) close = false;
+    unsure = unsure || __any_sync(FULL, close);
+  }
+  c.unsure = unsure;
+  return c;
+}
+
+// exp(-|x|) never leaves the range, and keeps the small scores of negative logits.
+__device__ __forceinline__ float sigmoid_of(float x) {
+  const float t = expf(-fabsf(x));
+  return (x < 0.f ? t : 1.f) / (1.f + t);
+}
+
+// Share of each lane's choice among the choices of its token (sum 1), 0 where there is none.
+// Softmax: exp(x - top of the chosen) over its sum.  Sigmoid: s over its sum, with exp(x) for s
+// where all chosen logits lie below -60 (there s = exp(x) to 2^-80, and s itself runs out of range).
+__device__ __forceinline__ float share_of(bool there, float x, bool sigmoid) {
+  uint32_t t = warp_max_bits(there ? order_bits(x) : 0u);
+  const float top = from_order_bits(t);
+  float s;
+  if (sigmoid && !(top < -60.f)) s = sigmoid_of(x);
+  else s = expf(x - top);
+  if (t == 0xffffffffu) s = __uint_as_float(0x7fffffffu);
+  if (!there) s = 0.f;
+  float sum = warp_sum_of(s);
+  return there ? s / sum : 0.f;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void route_load(const T* row, int lane, int n_experts, int vec, float (&x)[V]) {
+  const int e0 = lane * V;
+  constexpr int BYTES = V * (int)sizeof(T);
+  if (vec && e0 + V <= n_experts) {
+    if constexpr (BYTES >= 16) {
+      union { uint4 u[BYTES / 16]; T t[V]; } r;
+#pragma unroll
+      for (int j = 0; j < BYTES / 16; ++j) r.u[j] = reinterpret_cast<const uint4*>(row + e0)[j];
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = to_float(r.t[i]);
+      return;
+    } else if constexpr (BYTES == 8) {
+      union { uint2 u; T t[V]; } r;
+      r.u = *reinterpret_cast<const uint2*>(row + e0);
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = to_float(r.t[i]);
+      return;
+    } else if constexpr (BYTES == 4) {
+      union { uint32_t u; T t[V]; } r;
+      r.u = *reinterpret_cast<const uint32_t*>(row + e0);
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = to_float(r.t[i]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = e0 + i < n_experts ? to_float(row[e0 + i]) : -INFINITY;
+}
+
+// (top, sum of exp(x - top)) of a token's logits; top 0 where nothing but -inf is there.
+template <int V>
+__device__ __forceinline__ void softmax_stats(const float (&x)[V], float& top, float& sum) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) t = max(t, order_bits(x[i]));
+  t = warp_max_bits(t);
+  top = t == 0u ? 0.f : t == 0xffffffffu ? __uint_as_float(0x7fffffffu) : from_order_bits(t);
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum += expf(x[i] - top);
+  sum = warp_sum_of(sum);
+  if (sum == 0.f) sum = 1.f;
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(RT_WARPS * 32)
+route_topk_kernel(const RouteParams p) {
+  // groups: one row of keys per warp, wide enough for 64-bit keys
+  extern __shared__ __align__(16) float s_route[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* s_keys = s_route + (size_t)warp * 2 * p.n_experts;
+  const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_best == 1);
+  for (int64_t i = (int64_t)blockIdx.x * RT_WARPS + warp; i < p.n; i += (int64_t)gridDim.x * RT_WARPS) {
+    float x[V];
+    route_load<T, V>((const T*)p.logits + i * p.n_experts, lane, p.n_experts, p.vec, x);
+    Chosen c = route_token<float, V>(p, x, lane, by_logit, s_keys);
+    if (c.unsure) c = route_token<double, V>(p, x, lane, by_logit, s_keys);
+    const bool there = c.expert >= 0;
+    float w;
+    float top = 0.f, sum = 1.f;
+    const bool stats = !p.sigmoid && (!p.renormalize || !by_logit);
+    if (stats) softmax_stats<V>(x, top, sum);
+    if (p.renormalize) {
+      w = share_of(there, c.logit, p.sigmoid != 0);
+      if (stats && sum != sum) w = sum;            // a NaN that was not chosen still is in every score
+    } else {
+      w = p.sigmoid ? sigmoid_of(c.logit) : expf(c.logit - top) / sum;
+    }
+    if (lane < p.k) {
+      p.weights[i * p.k + lane] = there ? w * p.scale : 0.f;
+      p.experts[i * p.k + lane] = c.expert;
+    }
+  }
+}
+
+struct RouteGradParams {
+  const void* logits;
+  const int32_t* experts;
+  const float* grad_weights;
+  void* grad_logits;
+  int64_t n;
+  int n_experts, k;
+  int sigmoid, renormalize, vec;
+  float scale;
+};
+
+// Gradient of the weights to the logits.  With p the shares and g = scale * grad of the chosen:
+//   softmax, renormalised   p_j (g_j - sum p g)                 on the chosen, 0 elsewhere
+//   sigmoid, renormalised   p_j (g_j - sum p g) (1 - s_j)       on the chosen
+//   sigmoid                 g_j s_j (1 - s_j)                   on the chosen
+//   softmax                 s_e ([e chosen] g_e - sum s g)      everywhere
+// The warp writes the row's dense part and then, ordered by __syncwarp, the chosen places.
+template <typename T, int V>
+__global__ void __launch_bounds__(RT_WARPS * 32)
+route_topk_grad_kernel(const RouteGradParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = lane * V;
+  const bool dense = !p.sigmoid && !p.renormalize;
+  for (int64_t i = (int64_t)blockIdx.x * RT_WARPS + warp; i < p.n; i += (int64_t)gridDim.x * RT_WARPS) {
+    const T* row = (const T*)p.logits + i * p.n_experts;
+    T* out = (T*)p.grad_logits + i * p.n_experts;
+    int e = -1;
+    float g = 0.f, xe = -INFINITY;
+    if (lane < p.k) {
+      e = p.experts[i * p.k + lane];
+      if (e >= p.n_experts) e = -1;
+      if (e >= 0) {
+        g = p.grad_weights[i * p.k + lane] * p.scale;
+        xe = to_float(row[e]);
+      }
+    }
+    const bool there = e >= 0;
+    float d = 0.f;
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = 0.f;
+    if (dense) {
+      float x[V], top, sum;
+      route_load<T, V>(row, lane, p.n_experts, p.vec, x);
+      softmax_stats<V>(x, top, sum);
+      const float s = there ? expf(xe - top) / sum : 0.f;
+      const float dot = warp_sum_of(s * g);
+      const float inv = 1.f / sum;
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = -(expf(x[j] - top) * inv) * dot;
+      d = s * (g - dot);
+    } else if (p.renormalize) {
+      const float share = share_of(there, xe, p.sigmoid != 0);
+      const float dot = warp_sum_of(share * g);
+      d = share * (g - dot);
+      if (p.sigmoid) d *= 1.f - sigmoid_of(xe);
+    } else {
+      const float s = sigmoid_of(xe);
+      d = g * s * (1.f - s);
+    }
+    constexpr int BYTES = V * (int)sizeof(T);
+    if (p.vec && e0 + V <= p.n_experts) {
+      union { uint4 u4[(BYTES + 15) / 16]; uint2 u2; uint32_t u1; T t[V]; } r;
+#pragma unroll
+      for (int j = 0; j < V; ++j) r.t[j] = from_float<T>(v[j]);
+      if constexpr (BYTES >= 16) {
+#pragma unroll
+        for (int j = 0; j < BYTES / 16; ++j) reinterpret_cast<uint4*>(out + e0)[j] = r.u4[j];
+      } else if constexpr (BYTES == 8) {
+        *reinterpret_cast<uint2*>(out + e0) = r.u2;
+      } else if constexpr (BYTES == 4) {
+        *reinterpret_cast<uint32_t*>(out + e0) = r.u1;
+      } else {
+        out[e0] = r.t[0];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (e0 + j < p.n_experts) out[e0 + j] = from_float<T>(v[j]);
+    }
+    __syncwarp();
+    if (there) out[e] = from_float<T>(d);
+    __syncwarp();
+  }
+}
+
+template <typename T>
+bool route_rows_are_vec(const void* a, const void* b, int n_experts, int v) {
+  const int64_t bytes = (int64_t)v * sizeof(T) < 16 ? (int64_t)v * sizeof(T) : 16;
+  return (((uintptr_t)a | (uintptr_t)b) % bytes) == 0 && (n_experts * (int64_t)sizeof(T)) % bytes == 0;
+}
+
+#define KMB_ROUTE_WIDTHS(RUN)                                                                   \
+  do {                                                                                          \
+    if (p.n_experts <= 32) { RUN(1); }                                                          \
+    else if (p.n_experts <= 64) { RUN(2); }                                                     \
+    else if (p.n_experts <= 128) { RUN(4); }                                                    \
+    else if (p.n_experts <= 256) { RUN(8); }                                                    \
+    else if (p.n_experts <= 512) { RUN(16); }                                                   \
+    else { RUN(32); }                                                                           \
+  } while (0)
+
+static unsigned route_grid(int64_t n) {
+  const int64_t blocks = ceil_div(n, RT_WARPS), cap = (int64_t)sm_count() * 16;
+  return (unsigned)(blocks < cap ? blocks : cap);
+}
+
+template <typename T>
+int route_run(RouteParams p, cudaStream_t s) {
+  const size_t smem = p.groups > 1 ? (size_t)RT_WARPS * 2 * p.n_experts * sizeof(float) : 0;
+#define KMB_RUN(V)                                                                              \
+  p.vec = route_rows_are_vec<T>(p.logits, nullptr, p.n_experts, V);                             \
+  route_topk_kernel<T, V><<<route_grid(p.n), RT_WARPS * 32, smem, s>>>(p)
+  KMB_ROUTE_WIDTHS(KMB_RUN);
+#undef KMB_RUN
+  KMB_CHECK_LAUNCH();
+  return KMB_OK;
+}
+
+template <typename T>
+int route_grad_run(RouteGradParams p, cudaStream_t s) {
+#define KMB_RUN(V)                                                                              \
+  p.vec = route_rows_are_vec<T>(p.logits, p.grad_logits, p.n_experts, V);                       \
+  route_topk_grad_kernel<T, V><<<route_grid(p.n), RT_WARPS * 32, 0, s>>>(p)
+  KMB_ROUTE_WIDTHS(KMB_RUN);
+#undef KMB_RUN
+  KMB_CHECK_LAUNCH();
+  return KMB_OK;
+}
+
+// ============================================================================= expert order
+// A stable counting sort of the choices by expert.  A block takes SL_CHUNK consecutive choices, a warp
+// of it SL_ROUNDS * 32 of them; match_any ranks the equal experts of 32 choices, the warp's own
+// counters carry the rank from round to round, and the counters of the warps before it, the chunks
+// before it and the experts before it make the place.
+constexpr int SL_WARPS = 16, SL_ROUNDS = 8;
+constexpr int SL_THREADS = SL_WARPS * 32;
+constexpr int SL_CHUNK = SL_THREADS * SL_ROUNDS;
+constexpr int SL_MAX_EXPERTS = 1024;
+
+// counts[chunk][e] for every chunk
+__global__ void __launch_bounds__(SL_THREADS)
+slots_count_kernel(const int32_t* __restrict__ experts, int64_t total, int n_experts,
+                   int32_t* __restrict__ counts) {
+  __shared__ int32_t s_cnt[SL_MAX_EXPERTS];
+  for (int e = threadIdx.x; e < n_experts; e += SL_THREADS) s_cnt[e] = 0;
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * SL_CHUNK;
+#pragma unroll
+  for (int r = 0; r < SL_ROUNDS; ++r) {
+    const int64_t c = first + r * SL_THREADS + threadIdx.x;
+    const int e = c < total ? experts[c] : -1;
+    if (e >= 0 && e < n_experts) atomicAdd(&s_cnt[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < n_experts; e += SL_THREADS)
+    counts[(int64_t)blockIdx.x * n_experts + e] = s_cnt[e];
+}
+
+// counts[chunk][e] -> choices of expert e in the chunks before; totals[e].  One warp per expert.
+__global__ void __launch_bounds__(256)
+slots_scan_kernel(int32_t* __restrict__ counts, int chunks, int n_experts, int32_t* __restrict__ totals) {
+  const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (e >= n_experts) return;
+  int base = 0;
+  for (int c0 = 0; c0 < chunks; c0 += 32) {
+    const int c = c0 + lane;
+    const int v = c < chunks ? counts[(int64_t)c * n_experts + e] : 0;
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(FULL, inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (c < chunks) counts[(int64_t)c * n_experts + e] = base + inc - v;
+    base += __shfl_sync(FULL, inc, 31);
+  }
+  if (lane == 0) totals[e] = base;
+}
+
+// ONE: a single chunk, whose counts are the totals.
+template <bool ONE>
+__global__ void __launch_bounds__(SL_THREADS)
+slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, int n_experts,
+                   const int32_t* __restrict__ counts, const int32_t* __restrict__ totals,
+                   int32_t* __restrict__ slots, int32_t* __restrict__ rows, int32_t* __restrict__ offsets) {
+  extern __shared__ int32_t s_dyn[];
+  int32_t* s_base = s_dyn;                            // first place of each expert in this chunk
+  uint16_t* s_warp = (uint16_t*)(s_dyn + n_experts);  // [SL_WARPS][n_experts] choices in the warp
+  __shared__ int32_t s_scan[SL_WARPS];
+  __shared__ int32_t s_end;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t first = (int64_t)blockIdx.x * SL_CHUNK + warp * (SL_ROUNDS * 32);
+
+  int32_t e_r[SL_ROUNDS];
+#pragma unroll
+  for (int r = 0; r < SL_ROUNDS; ++r) {
+    const int64_t c = first + r * 32 + lane;
+    const int e = c < total ? experts[c] : -1;
+    e_r[r] = e >= 0 && e < n_experts ? e : -1;
+  }
+  uint16_t* mine = s_warp + warp * n_experts;
+  for (int e = lane; e < n_experts; e += 32) mine[e] = 0;
+  __syncwarp();
+  uint32_t rank[SL_ROUNDS];
+#pragma unroll
+  for (int r = 0; r < SL_ROUNDS; ++r) {
+    const unsigned same = __match_any_sync(FULL, e_r[r]);
+    const int before = __popc(same & ((1u << lane) - 1u));
+    const bool valid = e_r[r] >= 0;
+    const uint32_t seen = valid ? mine[e_r[r]] : 0u;
+    rank[r] = seen + before;
+    __syncwarp();
+    if (valid && before == 0) mine[e_r[r]] = (uint16_t)(seen + __popc(same));
+    __syncwarp();
+  }
+  __syncthreads();
+  // warps' counts -> choices in the warps before; then the experts' first places
+  int carry = 0;
+  for (int e0 = 0; e0 < n_experts; e0 += SL_THREADS) {
+    const int e = e0 + threadIdx.x;
+    int in_chunk = 0;
+    if (e < n_experts) {
+#pragma unroll
+      for (int w = 0; w < SL_WARPS; ++w) {
+        const int v = s_warp[w * n_experts + e];
+        s_warp[w * n_experts + e] = (uint16_t)in_chunk;
+        in_chunk += v;
+      }
+    }
+    const int tot = e < n_experts ? (ONE ? in_chunk : totals[e]) : 0;
+    int inc = tot;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(FULL, inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (lane == 31) s_scan[warp] = inc;
+    __syncthreads();
+    int base = carry, all = carry;
+    for (int w = 0; w < SL_WARPS; ++w) {
+      if (w < warp) base += s_scan[w];
+      all += s_scan[w];
+    }
+    if (e < n_experts) {
+      const int start = base + inc - tot;
+      s_base[e] = start + (ONE ? 0 : counts[(int64_t)blockIdx.x * n_experts + e]);
+      if (blockIdx.x == 0) offsets[e] = start;
+    }
+    carry = all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    s_end = carry;
+    if (blockIdx.x == 0) offsets[n_experts] = carry;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < SL_ROUNDS; ++r) {
+    const int64_t c = first + r * 32 + lane;
+    if (c >= total) continue;
+    const int e = e_r[r];
+    int place = -1;
+    if (e >= 0) {
+      place = s_base[e] + mine[e] + (int)rank[r];
+      rows[place] = (int32_t)(c / k);
+    }
+    slots[c] = place;
+    if (c >= s_end) rows[c] = -1;      // places behind the last chosen row
+  }
+}
+
+// ============================================================================= weighted sums
+// out[t] = sum_j w[t, j] values[slots[t, j]]; a slot outside [0, n_values) counts as none.
+constexpr int CB_THREADS = 128;
+constexpr int CB_K = 8;        // rows in flight per thread
+
+template <typename T>
+__global__ void __launch_bounds__(CB_THREADS)
+combine_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __restrict__ slots,
+               const float* __restrict__ weights, int k, int d, T* __restrict__ out, int vec) {
+  const int64_t t = blockIdx.x;
+  for (int f = (blockIdx.y * CB_THREADS + threadIdx.x) * 8; f < d; f += gridDim.y * CB_THREADS * 8) {
+    float acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    for (int j = 0; j < k; ++j) {
+      const int slot = slots[t * k + j];
+      if (slot < 0 || slot >= n_values) continue;
+      const float w = weights[t * k + j];
+      float v[8];
+      load_vec8(values + (int64_t)slot * d, f, d, vec != 0, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+    }
+    store_vec8(out + t * d, f, d, vec != 0, acc);
+  }
+}
+
+// Gradients.  A row of values that several choices share needs the sum of their gradients, in a fixed
+// order: `users` counts the choices of each row and `first` names the lowest of them, which alone
+// writes the row.  Rows that nobody chose get zeros.
+__global__ void combine_users_kernel(const int32_t* __restrict__ slots, int64_t total, int64_t n_values,
+                                     int32_t* __restrict__ users, int32_t* __restrict__ first) {
+  const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (c >= total) return;
+  const int slot = slots[c];
+  if (slot < 0 || slot >= n_values) return;
+  atomicAdd(&users[slot], 1);
+  atomicMin(&first[slot], (int32_t)c);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(CB_THREADS)
+combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __restrict__ slots,
+                    const float* __restrict__ weights, const T* __restrict__ grad_out, int64_t n, int k, int d,
+                    const int32_t* __restrict__ users, const int32_t* __restrict__ first,
+                    T* __restrict__ grad_values, float* __restrict__ grad_weights, int vec) {
+  __shared__ float red[CB_THREADS / 32][CB_K];
+  __shared__ int32_t list[CB_THREADS];
+  __shared__ int list_n[CB_THREADS / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if ((int64_t)blockIdx.x >= n) {
+    // the blocks behind the tokens': zeros for the rows that nobody chose
+    const int64_t step = (int64_t)gridDim.x - n;
+    for (int64_t r = (int64_t)blockIdx.x - n; r < n_values; r += step) {
+      if (users[r] != 0) continue;
+      float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int f = threadIdx.x * 8; f < d; f += CB_THREADS * 8) store_vec8(grad_values + r * d, f, d, vec != 0, z);
+    }
+    return;
+  }
+  const int64_t t = blockIdx.x;
+  const T* g_row = grad_out + t * d;
+  for (int j0 = 0; j0 < k; j0 += CB_K) {
+    float dot[CB_K];
+#pragma unroll
+    for (int j = 0; j < CB_K; ++j) dot[j] = 0.f;
+    for (int f = threadIdx.x * 8; f < d; f += CB_THREADS * 8) {
+      float g[8];
+      load_vec8(g_row, f, d, vec != 0, g);
+#pragma unroll
+      for (int j = 0; j < CB_K; ++j) {
+        if (j0 + j >= k) continue;
+        const int64_t c = t * k + j0 + j;
+        const int slot = slots[c];
+        if (slot < 0 || slot >= n_values) continue;
+        float v[8];
+        load_vec8(values + (int64_t)slot * d, f, d, vec != 0, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dot[j] = fmaf(v[i], g[i], dot[j]);
+        if (users[slot] == 1) {
+          const float w = weights[c];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = w * g[i];
+          store_vec8(grad_values + (int64_t)slot * d, f, d, vec != 0, v);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < CB_K; ++j) {
+      dot[j] = warp_sum_of(dot[j]);
+      if (lane == 0) red[warp][j] = dot[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < CB_K && j0 + threadIdx.x < k) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < CB_THREADS / 32; ++w) sum += red[w][threadIdx.x];
+      grad_weights[t * k + j0 + threadIdx.x] = sum;     // 0 where there is no row
+    }
+    __syncthreads();
+  }
+  // rows with several users: the block of the lowest of them finds the others by walking the choices
+  // behind it, CB_THREADS at a time, and adds them up in ascending order
+  for (int j = 0; j < k; ++j) {
+    const int64_t c0 = t * k + j;
+    const int slot = slots[c0];
+    if (slot < 0 || slot >= n_values || users[slot] == 1 || first[slot] != c0) continue;
+    for (int fb = 0; fb < d; fb += CB_THREADS * 8) {
+      const int f = fb + threadIdx.x * 8;
+      float acc[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+      int left = users[slot];
+      for (int64_t cb = c0; left > 0 && cb < n * k; cb += CB_THREADS) {
+        const int64_t c = cb + threadIdx.x;
+        const bool hit = c < n * k && slots[c] == slot;
+        const unsigned m = __ballot_sync(FULL, hit);
+        if (lane == 0) list_n[warp] = __popc(m);
+        __syncthreads();
+        int at = 0, found = 0;
+        for (int w = 0; w < CB_THREADS / 32; ++w) {
+          if (w < warp) at += list_n[w];
+          found += list_n[w];
+        }
+        if (hit) list[at + __popc(m & ((1u << lane) - 1u))] = (int32_t)(c - cb);
+        __syncthreads();
+        if (f < d)
+          for (int q = 0; q < found; ++q) {
+            const int64_t cc = cb + list[q];
+            const float w = weights[cc];
+            float g[8];
+            load_vec8(grad_out + (cc / k) * d, f, d, vec != 0, g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, g[i], acc[i]);
+          }
+        left -= found;
+        __syncthreads();
+      }
+      if (f < d) store_vec8(grad_values + (int64_t)slot * d, f, d, vec != 0, acc);
+    }
+  }
+}
+
+static int check_route(const char* who, int n_experts, int k) {
+  KMB_REQUIRE(n_experts >= 1 && n_experts <= RT_MAX_EXPERTS, "%s: the number of experts must be in [1, %d], got %d",
+              who, RT_MAX_EXPERTS, n_experts);
+  KMB_REQUIRE(k >= 1 && k <= RT_MAX_K && k <= n_experts,
+              "%s: k must be in [1, %d] and at most the number of experts, got %d", who, RT_MAX_K, k);
+  return KMB_OK;
+}
+
+}  // namespace kmb
+
+using namespace kmb;
+
+extern "C" {
+
+int kmb_route_topk(int dtype, const void* logits, const float* bias, int64_t n, int n_experts, int k,
+                   int flags, int groups, int topk_groups, int group_best, float scale, float* weights,
+                   int32_t* experts, void* stream) {
+  int rc = check_route("kmb_route_topk", n_experts, k);
+  if (rc != KMB_OK) return rc;
+  KMB_REQUIRE(n >= 0, "kmb_route_topk: bad sizes");
+  KMB_REQUIRE((flags & ~(KMB_ROUTE_SIGMOID | KMB_ROUTE_RENORMALIZE)) == 0, "kmb_route_topk: unknown flag bits");
+  KMB_REQUIRE(groups >= 1 && groups <= RT_MAX_GROUPS && n_experts % groups == 0,
+              "kmb_route_topk: the number of groups must be in [1, %d] and divide the number of experts, got %d",
+              RT_MAX_GROUPS, groups);
+  KMB_REQUIRE(topk_groups >= 1 && topk_groups <= groups,
+              "kmb_route_topk: topk_groups must be in [1, groups], got %d", topk_groups);
+  KMB_REQUIRE((int64_t)topk_groups * (n_experts / groups) >= k,
+              "Expected k to be greater than or equal to the number of items in the search space, but got "
+              "k=%d and %d items in the search space.", k, topk_groups * (n_experts / groups));
+  KMB_REQUIRE((group_best == 1 || group_best == 2) && group_best <= n_experts / groups,
+              "kmb_route_topk: group_best must be 1 or 2 and at most the size of a group, got %d", group_best);
+  if (n == 0) return KMB_OK;
+  KMB_REQUIRE(logits && weights && experts, "kmb_route_topk: NULL argument");
+  RouteParams p;
+  p.logits = logits;
+  p.bias = bias;
+  p.weights = weights;
+  p.experts = experts;
+  p.n = n;
+  p.n_experts = n_experts;
+  p.k = k;
+  p.groups = topk_groups == groups ? 1 : groups;     // every group stays: no groups
+  p.topk_groups = topk_groups;
+  p.group_best = group_best;
+  p.group_size = n_experts / groups;
+  p.sigmoid = (flags & KMB_ROUTE_SIGMOID) != 0;
+  p.renormalize = (flags & KMB_ROUTE_RENORMALIZE) != 0;
+  p.scale = scale;
+  KMB_DISPATCH_ROWS(dtype, { return route_run<T>(p, (cudaStream_t)stream); });
+}
+
+int kmb_route_topk_grad(int dtype, const void* logits, const int32_t* experts, const float* grad_weights,
+                        int64_t n, int n_experts, int k, int flags, float scale, void* grad_logits,
+                        void* stream) {
+  int rc = check_route("kmb_route_topk_grad", n_experts, k);
+  if (rc != KMB_OK) return rc;
+  KMB_REQUIRE(n >= 0, "kmb_route_topk_grad: bad sizes");
+  KMB_REQUIRE((flags & ~(KMB_ROUTE_SIGMOID | KMB_ROUTE_RENORMALIZE)) == 0,
+              "kmb_route_topk_grad: unknown flag bits");
+  if (n == 0) return KMB_OK;
+  KMB_REQUIRE(logits && experts && grad_weights && grad_logits, "kmb_route_topk_grad: NULL argument");
+  RouteGradParams p;
+  p.logits = logits;
+  p.experts = experts;
+  p.grad_weights = grad_weights;
+  p.grad_logits = grad_logits;
+  p.n = n;
+  p.n_experts = n_experts;
+  p.k = k;
+  p.sigmoid = (flags & KMB_ROUTE_SIGMOID) != 0;
+  p.renormalize = (flags & KMB_ROUTE_RENORMALIZE) != 0;
+  p.scale = scale;
+  KMB_DISPATCH_ROWS(dtype, { return route_grad_run<T>(p, (cudaStream_t)stream); });
+}
+
+size_t kmb_expert_slots_workspace_bytes(int64_t n, int k, int n_experts) {
+  if (n < 0 || k < 1 || n_experts < 1) return 0;
+  const int64_t chunks = ceil_div(n * k, SL_CHUNK);
+  return chunks <= 1 ? 0 : (size_t)(chunks + 1) * n_experts * sizeof(int32_t);
+}
+
+int kmb_expert_slots(const int32_t* experts, int64_t n, int k, int n_experts, int32_t* slots, int32_t* rows,
+                     int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream) {
+  KMB_REQUIRE(n >= 0 && k >= 1, "kmb_expert_slots: bad sizes");
+  KMB_REQUIRE(n_experts >= 1 && n_experts <= SL_MAX_EXPERTS,
+              "kmb_expert_slots: the number of experts must be in [1, %d], got %d", SL_MAX_EXPERTS, n_experts);
+  KMB_REQUIRE(n < (1ll << 31) / k - SL_CHUNK, "kmb_expert_slots: n * k must be below 2^31");
+  KMB_REQUIRE(offsets && (n == 0 || (experts && slots && rows)), "kmb_expert_slots: NULL argument");
+  const size_t need = kmb_expert_slots_workspace_bytes(n, k, n_experts);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
+    set_error("kmb_expert_slots: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    return KMB_ERR_WORKSPACE;
+  }
+  cudaStream_t s = (cudaStream_t)stream;
+  const int64_t total = n * k;
+  const int chunks = (int)ceil_div(total, SL_CHUNK);
+  const size_t smem = (size_t)n_experts * (sizeof(int32_t) + SL_WARPS * sizeof(uint16_t));
+  if (chunks <= 1) {
+    slots_place_kernel<true><<<1, SL_THREADS, smem, s>>>(experts, total, k, n_experts, nullptr, nullptr, slots,
+                                                         rows, offsets);
+    KMB_CHECK_LAUNCH();
+    return KMB_OK;
+  }
+  int32_t* counts = (int32_t*)workspace;
+  int32_t* totals = counts + (int64_t)chunks * n_experts;
+  slots_count_kernel<<<chunks, SL_THREADS, 0, s>>>(experts, total, n_experts, counts);
+  KMB_CHECK_LAUNCH();
+  slots_scan_kernel<<<(unsigned)ceil_div(n_experts, 8), 256, 0, s>>>(counts, chunks, n_experts, totals);
+  KMB_CHECK_LAUNCH();
+  slots_place_kernel<false><<<chunks, SL_THREADS, smem, s>>>(experts, total, k, n_experts, counts, totals, slots,
+                                                             rows, offsets);
+  KMB_CHECK_LAUNCH();
+  return KMB_OK;
+}
+
+int kmb_combine_experts(int dtype, const void* values, int64_t n_values, const int32_t* slots,
+                        const float* weights, int64_t n, int k, int d, void* out, void* stream) {
+  KMB_REQUIRE(n >= 0 && n < (1ll << 31) - 1 && n_values >= 0 && k >= 1 && d >= 1, "kmb_combine_experts: bad sizes");
+  if (n == 0) return KMB_OK;
+  KMB_REQUIRE((values || n_values == 0) && slots && weights && out, "kmb_combine_experts: NULL argument");
+  KMB_DISPATCH_ROWS(dtype, {
+    const int vec = rows_are_vec((const T*)values, d) && rows_are_vec((const T*)out, d);
+    dim3 grid((unsigned)n, (unsigned)ceil_div(d, CB_THREADS * 8));
+    if (grid.y > 65535) grid.y = 65535;
+    combine_kernel<T><<<grid, CB_THREADS, 0, (cudaStream_t)stream>>>((const T*)values, n_values, slots, weights, k,
+                                                                     d, (T*)out, vec);
+    KMB_CHECK_LAUNCH();
+  });
+  return KMB_OK;
+}
+
+size_t kmb_combine_experts_grad_workspace_bytes(int64_t n_values) {
+  return n_values < 0 ? 0 : (size_t)n_values * 2 * sizeof(int32_t);
+}
+
+int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, const int32_t* slots,
+                             const float* weights, const void* grad_out, int64_t n, int k, int d,
+                             void* grad_values, float* grad_weights, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  KMB_REQUIRE(n >= 0 && n_values >= 0 && k >= 1 && d >= 1, "kmb_combine_experts_grad: bad sizes");
+  KMB_REQUIRE(n <= (1ll << 30) && n < 0x7f7f7f7fll / k, "kmb_combine_experts_grad: n * k must be below 2^31");
+  if (n == 0 && n_values == 0) return KMB_OK;
+  KMB_REQUIRE((n_values == 0 || (values && grad_values)) && (n == 0 || (slots && weights && grad_out && grad_weights)),
+              "kmb_combine_experts_grad: NULL argument");
+  const size_t need = kmb_combine_experts_grad_workspace_bytes(n_values);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
+    set_error("kmb_combine_experts_grad: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    return KMB_ERR_WORKSPACE;
+  }
+  cudaStream_t s = (cudaStream_t)stream;
+  int32_t* users = (int32_t*)workspace;
+  int32_t* first = users + n_values;
+  if (n_values > 0) {
+    KMB_CHECK_CUDA(cudaMemsetAsync(users, 0, (size_t)n_values * sizeof(int32_t), s));
+    KMB_CHECK_CUDA(cudaMemsetAsync(first, 0x7f, (size_t)n_values * sizeof(int32_t), s));
+  }
+  if (n > 0) {
+    combine_users_kernel<<<(unsigned)ceil_div(n * k, 256), 256, 0, s>>>(slots, n * k, n_values, users, first);
+    KMB_CHECK_LAUNCH();
+  }
+  KMB_DISPATCH_ROWS(dtype, {
+    const int vec = rows_are_vec((const T*)values, d) && rows_are_vec((const T*)grad_out, d) &&
+                    rows_are_vec((const T*)grad_values, d);
+    const int64_t fill = n_values == 0 ? 0 : (ceil_div(n_values, 64) < sm_count() ? ceil_div(n_values, 64) : sm_count());
+    combine_grad_kernel<T><<<(unsigned)(n + fill), CB_THREADS, 0, s>>>(
+        (const T*)values, n_values, slots, weights, (const T*)grad_out, n, k, d, users, first, (T*)grad_values,
+        grad_weights, vec);
+    KMB_CHECK_LAUNCH();
+  });
+  return KMB_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,553 @@
+// Products in 8-bit integers with a scale for each row of both operands, and the quantisation of
+// rows that feeds them.
+//
+//   q[i, f] = round_half_even(127 x[i, f] / max_f |x[i, f]|),   scale[i] = max_f |x[i, f]| / 127
+//   out[i, j] = sa[i] * sb[j] * sum_f qa[i, f] qb[j, f]  (+ bias[j])
+//
+// dense, or by group: rows [offsets[g], offsets[g + 1]) of the left operand meet the g-th matrix of
+// the right one (the experts' products of a mixture of experts).  The sum is an int32 and exact for
+// d <= 131 071 (127 and 128 in magnitude: 131 072 products of 2^14 reach 2^31).
+//
+// No counterpart in the reference; they stand beside the products of matmul_hook.cu.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdlib.h>
+
+#include "kmb_common.cuh"
+#include "row_types.cuh"
+#include "tc_ptx.cuh"
+
+namespace kmb {
+
+// =============================================================================== quantisation
+// One block per row.  The row stays in registers between the maximum and the rounding when it fits
+// (QR_REGS vectors of eight elements a thread), longer rows are read a second time (from L1 / L2).
+constexpr int QR_VEC = 8;
+
+// round_half_even(127 x / top) as exact arithmetic has it.  r = x * (127 / top) in 32 bits is off by
+// less than 127 * 3 * 2^-24 < 1e-4, so only values that lie closer than that to the middle between
+// two whole numbers are decided by the quotient in 64 bits: 127 x is exact there, and a quotient of
+// such short numbers is never rounded onto a middle that it does not hit.
+__device__ __forceinline__ int quantize_one(float x, float inv, float top) {
+  const float r = x * inv;
+  float n = rintf(r);
+  if (!(fabsf(r - n) < 0.4999f)) n = (float)rint((double)x * 127.0 / (double)top);
+  return (int)n;
+}
+
+template <typename T, int THREADS, int REGS>
+__global__ void __launch_bounds__(THREADS)
+quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* __restrict__ rows,
+                     int8_t* __restrict__ q, int64_t q_pitch, float* __restrict__ scales, int vec) {
+  __shared__ uint32_t red[THREADS / 32];
+  const int64_t i = blockIdx.x;
+  int64_t src = i;
+  if (rows) {
+    src = rows[i];
+    if (src >= n) src = -1;
+  }
+  int8_t* qi = q + i * q_pitch;
+  const T* xi = x + (src < 0 ? 0 : src) * d;
+  float v[REGS][QR_VEC];
+  uint32_t top = 0;   // bits of |x|: whole numbers in the order of the values, NaN above infinity
+  for (int r = 0, f = threadIdx.x * QR_VEC; f < d; ++r, f += THREADS * QR_VEC) {
+    float w[QR_VEC];
+    if (src < 0) {
+#pragma unroll
+      for (int j = 0; j < QR_VEC; ++j) w[j] = 0.f;
+    } else {
+      load_vec8(xi, f, d, vec != 0, w);
+    }
+#pragma unroll
+    for (int j = 0; j < QR_VEC; ++j) top = max(top, __float_as_uint(w[j]) & 0x7fffffffu);
+#pragma unroll
+    for (int rr = 0; rr < REGS; ++rr)
+      if (r == rr) {
+#pragma unroll
+        for (int j = 0; j < QR_VEC; ++j) v[rr][j] = w[j];
+      }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (THREADS > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = red[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 32; ++w) top = max(top, red[w]);
+  }
+  const float topf = __uint_as_float(top);
+  // a row that holds an infinity or NaN has no 8-bit image: NaN as its scale makes its products NaN
+  const bool bad = top >= 0x7f800000u;
+  if (threadIdx.x == 0) scales[i] = bad ? __uint_as_float(0x7fffffffu) : topf / 127.f;
+  const bool zero = bad || top == 0u;
+  const float inv = 127.f / topf;   // infinite below 4e-37: quantize_one then takes the 64-bit quotient
+  for (int r = 0, f = threadIdx.x * QR_VEC; f < d; ++r, f += THREADS * QR_VEC) {
+    float w[QR_VEC];
+    bool kept = false;
+#pragma unroll
+    for (int rr = 0; rr < REGS; ++rr)
+      if (r == rr) {
+        kept = true;
+#pragma unroll
+        for (int j = 0; j < QR_VEC; ++j) w[j] = v[rr][j];
+      }
+    if (!kept) {
+      if (zero) {
+#pragma unroll
+        for (int j = 0; j < QR_VEC; ++j) w[j] = 0.f;
+      } else {
+        load_vec8(xi, f, d, vec != 0, w);
+      }
+    }
+    uint32_t p[2] = {0u, 0u};
+    if (!zero) {
+#pragma unroll
+      for (int j = 0; j < QR_VEC; ++j)
+        p[j >> 2] |= ((uint32_t)quantize_one(w[j], inv, topf) & 0xffu) << (8 * (j & 3));
+    }
+    // the pitch is a multiple of 16, so the eight bytes lie inside the row's own storage
+    *reinterpret_cast<uint2*>(qi + f) = make_uint2(p[0], p[1]);
+  }
+}
+
+template <typename T>
+int quantize_run(const T* x, int64_t n, int d, const int32_t* rows, int64_t m, int8_t* q,
+                 int64_t q_pitch, float* scales, cudaStream_t s) {
+  const int vec = rows_are_vec(x, d) ? 1 : 0;
+  const unsigned grid = (unsigned)m;
+  if (d <= 32 * QR_VEC * 2)
+    quantize_rows_kernel<T, 32, 2><<<grid, 32, 0, s>>>(x, n, d, rows, q, q_pitch, scales, vec);
+  else if (d <= 128 * QR_VEC * 2)
+    quantize_rows_kernel<T, 128, 2><<<grid, 128, 0, s>>>(x, n, d, rows, q, q_pitch, scales, vec);
+  else
+    quantize_rows_kernel<T, 256, 4><<<grid, 256, 0, s>>>(x, n, d, rows, q, q_pitch, scales, vec);
+  KMB_CHECK_LAUNCH();
+  return KMB_OK;
+}
+
+// ==================================================================================== product
+// tcgen05 kind::i8, int32 accumulators in tensor memory.  The matrix instruction's M side (128 lanes)
+// takes 128 rows of the RIGHT operand (output features), its N side BN rows of the left one (tokens):
+// a few tokens then cost a narrow instruction, and the weights, which bound small batches, stream
+// through at full width.
+//
+// One persistent CTA per SM, eight warps: 0 loads (TMA, 128-byte swizzle, a ring of stages of 128
+// bytes of the contraction), 1 issues the MMAs, 2 owns tensor memory, 4..7 scale and store (one
+// feature per lane).  Two accumulators, so that the stores of a tile overlap the MMAs of the next.
+constexpr int I8_BM = 128;
+constexpr int I8_KB = 128;            // bytes (= 8-bit features) per stage
+constexpr int I8_THREADS = 256;
+constexpr int I8_MAX_GROUPS = 1024;
+constexpr long long I8_TIMEOUT_CYCLES = 4000000000LL;   // ~2 s at 2 GHz
+
+template <int BN>
+struct I8Cfg {
+  static constexpr int A_BYTES = I8_BM * I8_KB, B_BYTES = BN * I8_KB;
+  static constexpr int FIT = (212 * 1024) / (A_BYTES + B_BYTES);
+  static constexpr int STAGES = FIT > 12 ? 12 : FIT;
+  static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
+  static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) |
+                                    ((uint32_t)(I8_BM >> 4) << 24);   // int32 += s8 * s8, both K-major
+};
+
+template <int BN>
+struct I8Smem {
+  unsigned char a[I8Cfg<BN>::STAGES][I8Cfg<BN>::A_BYTES];
+  unsigned char b[I8Cfg<BN>::STAGES][I8Cfg<BN>::B_BYTES];
+  int first_tile[I8_MAX_GROUPS + 1];   // tiles before each group
+  int scan[I8_THREADS / 32];
+  float sa[BN];
+  unsigned long long full[I8Cfg<BN>::STAGES], empty[I8Cfg<BN>::STAGES];
+  unsigned long long acc_full[2], acc_empty[2], drain;
+  long long timeout_cycles;
+  unsigned int tmem_base;
+  volatile int abort_flag;
+};
+static_assert(sizeof(I8Smem<256>) + 1024 <= 232448, "I8Smem exceeds the 227 KB a CTA may use");
+static_assert(sizeof(I8Smem<128>) + 1024 <= 232448, "I8Smem exceeds the 227 KB a CTA may use");
+static_assert(sizeof(I8Smem<64>) + 1024 <= 232448, "I8Smem exceeds the 227 KB a CTA may use");
+static_assert(sizeof(I8Smem<32>) + 1024 <= 232448, "I8Smem exceeds the 227 KB a CTA may use");
+static_assert(sizeof(I8Smem<16>) + 1024 <= 232448, "I8Smem exceeds the 227 KB a CTA may use");
+
+struct I8Params {
+  const float* sa;
+  const float* sb;
+  const float* bias;          // or NULL
+  const int32_t* offsets;     // or NULL: one group of all m rows
+  void* out;
+  int64_t m;
+  int groups, n, d;
+  int feature_tiles;
+  long long timeout_cycles;
+  int test_stall;             // test hook: the loading warp stops after its first tile
+};
+
+// Raised by a wait that ran out, on the GPU that ran it; read and cleared by kmb_int8_wait_error.
+static __device__ int g_i8_wait_error;
+
+template <typename Smem>
+__device__ __forceinline__ bool i8_wait(void* bar, uint32_t parity, Smem* sm) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (true) {
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (sm->abort_flag) return false;
+    if (clock64() - t0 > sm->timeout_cycles) {
+      sm->abort_flag = 1;
+      atomicExch(&g_i8_wait_error, 1);
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ void umma_i8_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// First row of group g, clamped so that no offset, however wrong, leads outside the m rows.
+__device__ __forceinline__ int64_t i8_row_of(const I8Params& p, int g) {
+  if (p.offsets == nullptr) return g == 0 ? 0 : p.m;
+  const int64_t o = p.offsets[g];
+  return o < 0 ? 0 : (o > p.m ? p.m : o);
+}
+
+struct I8Tile {
+  int g;
+  int64_t row0;     // first token row
+  int rows;         // token rows of the tile that belong to the group
+  int feature0;
+};
+
+template <int BN>
+__device__ __forceinline__ I8Tile i8_tile(const I8Params& p, const int* first_tile, int t) {
+  int lo = 0, hi = p.groups;                 // last group with first_tile[g] <= t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first_tile[mid] <= t) lo = mid; else hi = mid;
+  }
+  const int local = t - first_tile[lo];
+  I8Tile r;
+  r.g = lo;
+  const int mt = local / p.feature_tiles;
+  r.feature0 = (local - mt * p.feature_tiles) * I8_BM;
+  const int64_t start = i8_row_of(p, lo);
+  r.row0 = start + (int64_t)mt * BN;
+  const int64_t left = i8_row_of(p, lo + 1) - r.row0;
+  r.rows = left < BN ? (int)left : BN;
+  return r;
+}
+
+template <int BN, typename T>
+__global__ void __launch_bounds__(I8_THREADS, 1)
+int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                   const I8Params p) {
+  using Cfg = I8Cfg<BN>;
+  extern __shared__ __align__(16) unsigned char i8_dyn[];
+  I8Smem<BN>* sm = reinterpret_cast<I8Smem<BN>*>(((uintptr_t)i8_dyn + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      mbar_init(&sm->full[s], 1);
+      mbar_init(&sm->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm->acc_full[b], 1);
+      mbar_init(&sm->acc_empty[b], 4);
+    }
+    mbar_init(&sm->drain, 1);
+    sm->timeout_cycles = p.timeout_cycles;
+    sm->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(&sm->tmem_base, Cfg::TMEM_COLS);
+    tmem_relinquish();
+  }
+  // tiles before each group: a block-wide exclusive sum, four consecutive groups per thread
+  {
+    int cnt[I8_MAX_GROUPS / I8_THREADS], sum = 0;
+#pragma unroll
+    for (int j = 0; j < I8_MAX_GROUPS / I8_THREADS; ++j) {
+      const int g = threadIdx.x * (I8_MAX_GROUPS / I8_THREADS) + j;
+      cnt[j] = 0;
+      if (g < p.groups) {
+        const int64_t rows = i8_row_of(p, g + 1) - i8_row_of(p, g);
+        cnt[j] = rows > 0 ? (int)((rows + BN - 1) / BN) * p.feature_tiles : 0;
+      }
+      sum += cnt[j];
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) sm->scan[warp] = inc;
+    __syncthreads();
+    int base = inc - sum;
+    for (int w = 0; w < warp; ++w) base += sm->scan[w];
+#pragma unroll
+    for (int j = 0; j < I8_MAX_GROUPS / I8_THREADS; ++j) {
+      const int g = threadIdx.x * (I8_MAX_GROUPS / I8_THREADS) + j;
+      if (g <= p.groups) sm->first_tile[g] = base;
+      base += cnt[j];
+    }
+    if (threadIdx.x == I8_THREADS - 1 && p.groups == I8_MAX_GROUPS) sm->first_tile[I8_MAX_GROUPS] = base;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = sm->tmem_base;
+  const int tiles = sm->first_tile[p.groups];
+  const int chunks = (p.d + I8_KB - 1) / I8_KB;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------------ loads
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const I8Tile tile = i8_tile<BN>(p, sm->first_tile, t);
+        const int w_row = tile.g * p.n + tile.feature0;
+        for (int c = 0; c < chunks; ++c, ++it) {
+          const uint32_t s = it % Cfg::STAGES, lap = it / Cfg::STAGES;
+          if (!i8_wait(&sm->empty[s], (lap & 1u) ^ 1u, sm)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(&sm->full[s], Cfg::A_BYTES + Cfg::B_BYTES);
+          tma_load_2d(sm->a[s], &map_w, c * I8_KB, w_row, &sm->full[s]);
+          tma_load_2d(sm->b[s], &map_x, c * I8_KB, (int)tile.row0, &sm->full[s]);
+        }
+        if (p.test_stall) break;
+      }
+      if (sm->abort_flag) drain_ring(sm->full, Cfg::STAGES, it);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------------- MMAs
+    const uint64_t a0 = make_sdesc(smem_u32(sm->a[0])), b0 = make_sdesc(smem_u32(sm->b[0]));
+    const int last_steps = ((p.d - (chunks - 1) * I8_KB) + 31) / 32;   // 32 features per instruction
+    uint32_t it = 0, nt = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++nt) {
+      const uint32_t ab = nt & 1u;
+      if (!__all_sync(0xffffffffu, i8_wait(&sm->acc_empty[ab], ((nt >> 1) & 1u) ^ 1u, sm))) break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + ab * BN;
+      for (int c = 0; c < chunks; ++c, ++it) {
+        const uint32_t s = it % Cfg::STAGES, lap = it / Cfg::STAGES;
+        if (!__all_sync(0xffffffffu, i8_wait(&sm->full[s], lap & 1u, sm))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t ad = a0 + (uint64_t)(s * (Cfg::A_BYTES >> 4));
+          const uint64_t bd = b0 + (uint64_t)(s * (Cfg::B_BYTES >> 4));
+          const int steps = c == chunks - 1 ? last_steps : 4;
+          for (int ks = 0; ks < steps; ++ks)
+            umma_i8_ss(d_tmem, ad + 2 * ks, bd + 2 * ks, Cfg::IDESC, (c | ks) != 0);
+          umma_commit(&sm->empty[s]);
+          if (c == chunks - 1) umma_commit(&sm->acc_full[ab]);
+        }
+        __syncwarp();
+      }
+    }
+    if (sm->abort_flag) mma_drain(&sm->drain);
+  } else if (warp >= 4) {
+    // --------------------------------------------------------------- scales and stores
+    const int q = warp & 3;
+    const int etid = threadIdx.x - 128;
+    T* out = reinterpret_cast<T*>(p.out);
+    if (p.offsets) {
+      // rows behind the last group belong to nobody: zeros
+      const int64_t end = i8_row_of(p, p.groups);
+      const int64_t first = end * p.n, last = p.m * p.n;
+      for (int64_t e = first + (int64_t)blockIdx.x * 128 + etid; e < last; e += (int64_t)gridDim.x * 128)
+        out[e] = from_float<T>(0.f);
+    }
+    uint32_t nt = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++nt) {
+      const I8Tile tile = i8_tile<BN>(p, sm->first_tile, t);
+      const uint32_t ab = nt & 1u;
+      asm volatile("bar.sync 1, 128;" ::: "memory");   // everybody is done with the last tile's scales
+      for (int r = etid; r < BN; r += 128) sm->sa[r] = r < tile.rows ? p.sa[tile.row0 + r] : 0.f;
+      const int feature = tile.feature0 + q * 32 + lane;
+      const bool mine = feature < p.n;
+      const int64_t wrow = (int64_t)tile.g * p.n + feature;
+      float sb = mine ? p.sb[wrow] : 0.f;
+      const float bias = (mine && p.bias) ? p.bias[wrow] : 0.f;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const bool ok = __all_sync(0xffffffffu, i8_wait(&sm->acc_full[ab], (nt >> 1) & 1u, sm));
+      if (!ok) sb = __uint_as_float(0x7fffffffu);      // a wait ran out: the tile becomes NaN
+      tc_fence_after();
+      T* o = out + tile.row0 * p.n + feature;
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN; c0 += 16) {
+        uint32_t v[16];
+        tmem_ld16(tmem_base + ab * BN + c0 + ((uint32_t)(q * 32) << 16), v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (mine && c0 + j < tile.rows)
+            o[(int64_t)(c0 + j) * p.n] = from_float<T>((float)(int)v[j] * (sm->sa[c0 + j] * sb) + bias);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm->acc_empty[ab]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+// (rows, d) 8-bit row-major matrix at a pitch of ld bytes; box = 128 bytes x box_rows rows.
+static int i8_make_map(CUtensorMap* map, const int8_t* base, int64_t rows, int d, int64_t ld, int box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from this driver");
+    return KMB_ERR_CUDA;
+  }
+  cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)I8_KB, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)base, dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with CUresult %d (rows=%lld d=%d ld=%lld)", (int)r,
+              (long long)rows, d, (long long)ld);
+    return KMB_ERR_CUDA;
+  }
+  return KMB_OK;
+}
+
+template <int BN, typename T>
+int i8_launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const I8Params& p, unsigned grid,
+              cudaStream_t s) {
+  const int smem = (int)sizeof(I8Smem<BN>) + 1024;
+  KMB_CHECK_CUDA(cudaFuncSetAttribute(int8_matmul_kernel<BN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      smem));
+  int8_matmul_kernel<BN, T><<<grid, I8_THREADS, smem, s>>>(map_w, map_x, p);
+  KMB_CHECK_LAUNCH();
+  return KMB_OK;
+}
+
+template <int BN>
+int i8_run(int out_dtype, const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, I8Params p,
+           cudaStream_t s) {
+  CUtensorMap map_w, map_x;
+  int rc = i8_make_map(&map_w, b, (int64_t)p.groups * p.n, p.d, ldb, I8_BM);
+  if (rc != KMB_OK) return rc;
+  rc = i8_make_map(&map_x, a, p.m, p.d, lda, BN);
+  if (rc != KMB_OK) return rc;
+  // an upper bound of the tiles: every group may end inside one
+  const int64_t most = (ceil_div(p.m, BN) + p.groups - 1) * p.feature_tiles;
+  KMB_REQUIRE(most < (1ll << 31), "kmb_int8_matmul: too many output tiles");
+  const unsigned grid = (unsigned)(most < sm_count() ? most : sm_count());
+  if (out_dtype == KMB_F32) return i8_launch<BN, float>(map_w, map_x, p, grid, s);
+  if (out_dtype == KMB_F16) return i8_launch<BN, __half>(map_w, map_x, p, grid, s);
+  return i8_launch<BN, __nv_bfloat16>(map_w, map_x, p, grid, s);
+}
+
+}  // namespace kmb
+
+using namespace kmb;
+
+extern "C" {
+
+int kmb_quantize_rows(int dtype, const void* x, int64_t n, int d, const int32_t* rows, int64_t m,
+                      int8_t* q, int64_t q_pitch, float* scales, void* stream) {
+  KMB_REQUIRE(n >= 0 && d > 0 && m >= 0 && m < (1ll << 31), "kmb_quantize_rows: bad sizes");
+  KMB_REQUIRE(rows != nullptr || m == n, "kmb_quantize_rows: m must be n when no rows are named");
+  if (m == 0) return KMB_OK;
+  KMB_REQUIRE((x || n == 0) && q && scales, "kmb_quantize_rows: NULL argument");
+  KMB_REQUIRE(q_pitch >= d && q_pitch % 16 == 0 && ((uintptr_t)q & 15) == 0,
+              "kmb_quantize_rows: q must be 16-byte aligned with a pitch of a multiple of 16, at least d");
+  KMB_DISPATCH_ROWS(dtype, {
+    return quantize_run<T>((const T*)x, n, d, rows, m, q, q_pitch, scales, (cudaStream_t)stream);
+  });
+}
+
+int kmb_int8_matmul(int out_dtype, const int8_t* a, int64_t lda, const float* a_scales, const int8_t* b,
+                    int64_t ldb, const float* b_scales, const float* bias, const int32_t* offsets,
+                    int groups, void* out, int64_t m, int n, int d, void* stream) {
+  KMB_REQUIRE(out_dtype == KMB_F32 || out_dtype == KMB_F16 || out_dtype == KMB_BF16,
+              "kmb_int8_matmul: out_dtype must be KMB_F32, KMB_F16 or KMB_BF16, got %d", out_dtype);
+  KMB_REQUIRE(m >= 0 && m < (1ll << 31) - 256 && n > 0 && d > 0, "kmb_int8_matmul: bad sizes");
+  KMB_REQUIRE(d <= 131071, "kmb_int8_matmul: d must be at most 131071 (int32 sums), got %d", d);
+  KMB_REQUIRE(groups >= 1 && groups <= I8_MAX_GROUPS && (offsets || groups == 1),
+              "kmb_int8_matmul: groups must be in [1, %d], and 1 without offsets", I8_MAX_GROUPS);
+  KMB_REQUIRE((int64_t)groups * n < (1ll << 31) - 256, "kmb_int8_matmul: groups * n must be below 2^31");
+  if (m == 0) return KMB_OK;
+  KMB_REQUIRE(a && a_scales && b && b_scales && out, "kmb_int8_matmul: NULL argument");
+  KMB_REQUIRE(lda >= d && lda % 16 == 0 && ldb >= d && ldb % 16 == 0 && ((uintptr_t)a & 15) == 0 &&
+                  ((uintptr_t)b & 15) == 0,
+              "kmb_int8_matmul: a and b must be 16-byte aligned with row pitches of a multiple of 16");
+  I8Params p;
+  p.sa = a_scales;
+  p.sb = b_scales;
+  p.bias = bias;
+  p.offsets = offsets;
+  p.out = out;
+  p.m = m;
+  p.groups = groups;
+  p.n = n;
+  p.d = d;
+  p.feature_tiles = (int)ceil_div(n, I8_BM);
+  const char* e = getenv("KMB_TC_TIMEOUT_MS");
+  const long ms = e ? atol(e) : 0;
+  p.timeout_cycles = ms > 0 ? ms * 2000000LL : I8_TIMEOUT_CYCLES;
+  e = getenv("KMB_TC_TEST_STALL");
+  p.test_stall = e && atoi(e) != 0;
+  cudaStream_t s = (cudaStream_t)stream;
+  // Tokens per tile: the narrowest that holds an average group.
+  const int64_t rows = ceil_div(m, groups);
+  if (rows <= 16) return i8_run<16>(out_dtype, a, lda, b, ldb, p, s);
+  if (rows <= 32) return i8_run<32>(out_dtype, a, lda, b, ldb, p, s);
+  if (rows <= 64) return i8_run<64>(out_dtype, a, lda, b, ldb, p, s);
+  if (rows <= 128) return i8_run<128>(out_dtype, a, lda, b, ldb, p, s);
+  return i8_run<256>(out_dtype, a, lda, b, ldb, p, s);
+}
+
+int kmb_int8_wait_error(int* flag, void* stream) {
+  KMB_REQUIRE(flag, "kmb_int8_wait_error: NULL argument");
+  cudaStream_t s = (cudaStream_t)stream;
+  const int zero = 0;
+  *flag = 0;
+  KMB_CHECK_CUDA(cudaMemcpyFromSymbolAsync(flag, g_i8_wait_error, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
+  KMB_CHECK_CUDA(cudaStreamSynchronize(s));
+  if (*flag) {
+    KMB_CHECK_CUDA(cudaMemcpyToSymbolAsync(g_i8_wait_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s));
+    KMB_CHECK_CUDA(cudaStreamSynchronize(s));
+    set_error("a bounded wait of the 8-bit product ran out: its tiles were filled with NaN");
+    return KMB_ERR_CUDA;
+  }
+  return KMB_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,495 @@
+"""Routing, expert order and weighted sums of a mixture of experts against plain float64 restatements,
+at the sizes, masks and orders where they can go wrong.
+
+Tolerances.  u = 2^-24 (half a step of float32).  A share is exp(x - top) / sum: the argument carries
+|x - top| u of relative error into the exponential (|x - top| <= 40 in these inputs, beyond that the share is
+below 1e-17 of the largest), the exponential 4 u, the sum at most 37 additions, the quotient and the scale
+u each: below 128 u = 2^-17, twice that with a softmax over all experts whose sum and quotient enter again.
+Results in 16 bits add half a step of their type.
+"""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _order(keys):
+    """Indices by descending key, NaN greatest, lowest index among equals."""
+    k = np.where(np.isnan(keys), np.inf, keys)
+    return sorted(range(len(k)), key=lambda e: (not np.isnan(keys[e]), -k[e], e))
+
+
+def _scores(x, scoring):
+    with np.errstate(all="ignore"):
+        if scoring == "sigmoid":
+            return 1 / (1 + np.exp(-x))
+        top = x.max()
+        e = np.exp(x - (0 if np.isneginf(top) else top))
+        total = e.sum()
+        return e / (1 if total == 0 else total)
+
+
+def _shares(x, scoring):
+    """What each of the chosen has of their sum, from the logarithms of the scores: float64 itself runs out
+    of range for sigmoids of the lowest values."""
+    with np.errstate(all="ignore"):
+        log_s = -np.logaddexp(0, -x) if scoring == "sigmoid" else x
+        log_s = np.where(x < -700, x, log_s)
+        e = np.exp(log_s - log_s.max())
+        return e / e.sum()
+
+
+def ref_route(logits, k, bias=None, scoring="softmax", n_groups=1, topk_groups=None, group_best=1,
+              renormalize=True, scale=1.0):
+    n, e = logits.shape
+    topk_groups = topk_groups or n_groups
+    weights, experts = np.zeros((n, k)), np.full((n, k), -1, np.int32)
+    for i in range(n):
+        x = logits[i]
+        s = _scores(x, scoring)
+        key = s + bias if bias is not None else s
+        choose = key if bias is not None else x.copy()
+        choose = np.where(np.isneginf(x), -np.inf, choose)
+        if n_groups > 1:
+            size = e // n_groups
+            gkey = choose if group_best == 1 else np.where(np.isneginf(x), -np.inf, key)
+            score = []
+            for g in range(n_groups):
+                part = gkey[g * size:(g + 1) * size]
+                o = _order(part)[:group_best]
+                with np.errstate(all="ignore"):
+                    score.append(part[o].sum())
+            kept = _order(np.array(score))[:topk_groups]
+            for g in range(n_groups):
+                if g not in kept:
+                    choose[g * size:(g + 1) * size] = -np.inf
+        o = [j for j in _order(choose)[:k] if not np.isneginf(choose[j])]
+        w = s[o]
+        if renormalize and len(o):
+            w = _shares(x[o], scoring) if not np.isnan(s).all() else w
+        experts[i, :len(o)] = o
+        weights[i, :len(o)] = w * scale
+    return weights, experts
+
+
+def ref_route_grad(logits, experts, grad, scoring, renormalize, scale):
+    """By the chain rule through the scores: d weights / d scores, then d scores / d logits.  Renormalised
+    weights depend on the logarithms of the chosen scores alone, whose slopes are 1 or 1 - s."""
+    out = np.zeros_like(logits)
+    for i in range(logits.shape[0]):
+        s = _scores(logits[i], scoring)
+        there = experts[i] >= 0
+        idx, g = experts[i][there], grad[i][there].astype(np.float64) * scale
+        ds = np.zeros_like(s)
+        if renormalize and len(idx):
+            p = _shares(logits[i][idx], scoring)
+            out[i][idx] = p * (g - (p * g).sum()) * (1 - s[idx] if scoring == "sigmoid" else 1)
+            continue
+        ds[idx] = g
+        out[i] = s * (1 - s) * ds if scoring == "sigmoid" else s * (ds - (s * ds).sum())
+    return out
+
+
+def _logits(n, e, dtype, seed, masked=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, e, generator=g) * 1.5
+    if masked and e > 1 and n > 4:
+        x[torch.rand(n, e, generator=g) < 0.15] = float("-inf")
+        x[1] = float("-inf")                 # a padding token
+        x[2] = 0.25                          # all equal
+        x[3] = torch.finfo(dtype).min        # masked by the type's lowest value: still numbers
+    return x.to(dtype).cuda()
+
+
+def _same_route(x, k, **kw):
+    from sklearn_numba_dpex_b200.common import route_topk
+
+    weights, experts = route_topk(x, k, **kw)
+    if kw.get("bias") is not None:
+        kw = {**kw, "bias": kw["bias"].double().cpu().numpy()}
+    want_w, want_e = ref_route(x.double().cpu().numpy(), k, **kw)
+    assert weights.dtype == torch.float32 and experts.dtype == torch.int32
+    np.testing.assert_array_equal(experts.cpu().numpy(), want_e)
+    np.testing.assert_allclose(weights.cpu().double().numpy(), want_w, rtol=256 * U, atol=0)
+    return weights, experts
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,e,k", [(1, 1, 1), (5, 2, 2), (7, 31, 3), (33, 32, 1), (9, 33, 8), (6, 64, 6), (17, 100, 9),
+                                   (13, 128, 8), (7, 257, 16), (5, 600, 32), (6, 1024, 4), (3, 1023, 32)])
+@pytest.mark.parametrize("scoring,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True),
+                                                 ("sigmoid", False)])
+def test_route_sizes(dtype, n, e, k, scoring, renormalize):
+    _same_route(_logits(n, e, TYPES[dtype], 1), k, scoring=scoring, renormalize=renormalize, scale=2.5)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e,groups,topk_groups,best,k", [(256, 8, 4, 2, 8), (256, 8, 4, 1, 8), (64, 32, 3, 2, 6),
+                                                         (96, 3, 1, 2, 5), (105, 7, 7, 1, 9), (40, 8, 8, 2, 4),
+                                                         (1024, 16, 2, 2, 32), (6, 6, 2, 1, 2)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_route_groups_and_bias(scoring, e, groups, topk_groups, best, k, with_bias):
+    g = torch.Generator().manual_seed(3)
+    bias = (torch.randn(e, generator=g) * 0.1).cuda() if with_bias else None
+    for dtype in TYPES.values():
+        _same_route(_logits(23, e, dtype, 4), k, bias=bias, scoring=scoring, n_groups=groups, topk_groups=topk_groups,
+                    group_best=best, scale=1.5)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_near_ties_are_ordered_as_64_bits_order_them(scoring):
+    """Keys that differ by less than 32 bits resolve: the bias undoes the difference of the scores up to its
+    own rounding, so that every pair of experts lies within a few 2^-25 of each other."""
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(64, generator=g)
+    s = torch.from_numpy(_scores(x.double().numpy(), scoring))
+    bias = (0.7 - s).float().cuda()
+    _same_route(x[None].repeat(5, 1).cuda(), 16, bias=bias, scoring=scoring)
+    # and a bias of zeros leaves equal logits equal: lowest index
+    xs = torch.randint(0, 3, (50, 64), generator=g).float().cuda()
+    _same_route(xs, 20, bias=torch.zeros(64, device="cuda"), scoring=scoring)
+    _same_route(xs, 20, bias=torch.zeros(64, device="cuda"), scoring=scoring, n_groups=8, topk_groups=3, group_best=2)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_nan_and_infinity(scoring, renormalize):
+    x = torch.randn(6, 40, generator=torch.Generator().manual_seed(2))
+    x[0, 7] = float("nan")
+    x[1, 3] = float("inf")
+    x[2, 3], x[2, 30] = float("nan"), float("-inf")
+    x[3, :] = float("nan")
+    _same_route(x.cuda(), 5, scoring=scoring, renormalize=renormalize)
+    b = torch.zeros(40, device="cuda")
+    b[4], b[5] = float("-inf"), float("nan")      # an expert that is switched off, and one that is broken
+    _same_route(x[4:].cuda(), 5, scoring=scoring, renormalize=renormalize, bias=b)
+
+
+def test_route_extreme_scores_stay_finite():
+    x = torch.tensor([[-200.0, -150.0, -151.0, -300.0], [90.0, 88.0, 1.0, -90.0], [-62.0, -59.0, -61.0, -1e30]])
+    for scoring in ("softmax", "sigmoid"):
+        w, e = _same_route(x.cuda(), 3, scoring=scoring)
+        assert torch.isfinite(w).all() and torch.allclose(w.sum(1), torch.ones(3, device="cuda"))
+    _same_route(x[1:2].cuda(), 4, scoring="sigmoid", renormalize=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,e,k", [(1, 1, 1), (7, 31, 3), (6, 64, 6), (13, 130, 8), (5, 600, 32), (6, 1024, 4)])
+@pytest.mark.parametrize("scoring,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True),
+                                                 ("sigmoid", False)])
+def test_route_gradient_is_the_formula(dtype, n, e, k, scoring, renormalize):
+    from sklearn_numba_dpex_b200.common import route_topk, route_topk_grad
+
+    x = _logits(n, e, TYPES[dtype], 5)
+    grad = torch.randn(n, k, generator=torch.Generator().manual_seed(6)).cuda()
+    leaf = x.clone().requires_grad_(True)
+    weights, experts = route_topk(leaf, k, scoring=scoring, renormalize=renormalize, scale=2.5)
+    assert not experts.requires_grad
+    weights.backward(grad)
+    explicit = route_topk_grad(x, experts, grad, scoring=scoring, renormalize=renormalize, scale=2.5)
+    assert leaf.grad.dtype == x.dtype and torch.equal(leaf.grad, explicit)
+    x64, e64 = x.double().cpu().numpy(), experts.cpu().numpy()
+    want = ref_route_grad(x64, e64, grad.cpu().numpy(), scoring, renormalize, 2.5)
+    # the formulas are a share or score (at most one) times a difference of terms of at most |g|
+    s = np.stack([_scores(r, scoring) for r in x64])
+    size = np.where(want != 0, 1.0, 0.0) if renormalize else s
+    bound = 256 * U * 2 * 2.5 * np.abs(grad.cpu().numpy()).max() * size
+    bound = bound + torch.finfo(x.dtype).eps / 2 * np.abs(want) + torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps
+    assert (np.abs(explicit.double().cpu().numpy() - want) <= bound).all()
+
+
+@pytest.mark.parametrize("scoring,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True),
+                                                 ("sigmoid", False)])
+def test_route_gradient_is_the_slope(scoring, renormalize):
+    """Central differences of the forward pass with step h = 2^-6.  Third derivatives of a share in one
+    logit are below 1, so the difference is off by h^2 / 6 = 4.1e-5 per unit of sum |g|; its rounding is
+    256 u / (2 h) = 4.9e-4 of the weights."""
+    from sklearn_numba_dpex_b200.common import route_topk, route_topk_grad
+
+    h, k = 2.0 ** -6, 3
+    x = torch.linspace(-1, 1, 12)[torch.randperm(12, generator=torch.Generator().manual_seed(1))][None].cuda()
+    grad = torch.tensor([[0.7, -1.1, 0.4]], device="cuda")
+    kw = dict(scoring=scoring, renormalize=renormalize, scale=1.0)
+    _, experts = route_topk(x, k, **kw)
+    got = route_topk_grad(x, experts, grad, **kw)
+    steps = torch.cat([x + h * torch.eye(12, device="cuda"), x - h * torch.eye(12, device="cuda")])
+    w, e = route_topk(steps, k, **kw)
+    assert (e == experts).all()          # gaps of the logits are 2 / 11, far above h
+    slope = ((w[:12] - w[12:]).double() * grad.double()).sum(1) / (2 * h)
+    bound = (h * h / 6 + 256 * U / (2 * h)) * float(grad.abs().sum())
+    assert float((slope - got[0].double()).abs().max()) <= bound
+
+
+def test_route_gradient_of_a_broadcast_and_of_a_view():
+    """The gradient that arrives may have strides of 0 (a sum's), the logits may be a slice."""
+    from sklearn_numba_dpex_b200.common import route_topk, route_topk_grad
+
+    base = torch.randn(20, 48, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    leaf = base.clone().requires_grad_(True)
+    w, e = route_topk(leaf[::2, 3:43], 4, scoring="sigmoid", renormalize=False)
+    w.sum().backward()
+    want = torch.zeros_like(base)
+    want[::2, 3:43] = route_topk_grad(base[::2, 3:43], e, torch.ones(10, 4, device="cuda"), "sigmoid", False)
+    assert torch.equal(leaf.grad, want)
+
+
+# --------------------------------------------------------------------------- expert order
+def ref_slots(experts, n_experts):
+    flat = experts.reshape(-1)
+    key = np.where((flat >= 0) & (flat < n_experts), flat, n_experts)
+    order = np.argsort(key, kind="stable")
+    valid = int((key < n_experts).sum())
+    slots, rows = np.full(flat.size, -1), np.full(flat.size, -1)
+    slots[order[:valid]] = np.arange(valid)
+    rows[:valid] = order[:valid] // experts.shape[1]
+    return slots.reshape(experts.shape), rows, np.concatenate([[0], np.cumsum(np.bincount(key, minlength=n_experts + 1)[:n_experts])])
+
+
+@pytest.mark.parametrize("n,k,e", [(0, 3, 4), (1, 1, 1), (1, 8, 256), (64, 8, 256), (511, 8, 7), (512, 8, 1024), (513, 8, 64),
+                                   (4097, 1, 3), (5000, 6, 1024), (30011, 9, 129)])
+@pytest.mark.parametrize("kind", ["all", "some", "none", "one", "repeated"])
+def test_expert_slots(n, k, e, kind):
+    from sklearn_numba_dpex_b200.common import expert_slots
+
+    rng = np.random.default_rng(n + k + e)
+    x = rng.integers(0, e, (n, k))
+    if kind == "some":
+        x[rng.random((n, k)) < 0.3] = -1
+        x[rng.random((n, k)) < 0.05] = e + 3        # not an expert either
+    elif kind == "none":
+        x[:] = -1
+    elif kind == "one":
+        x[:] = e - 1
+    elif kind == "repeated" and n:
+        x[:] = x[:, :1]                             # a token names the same expert k times
+    x = x.astype(np.int32)
+    got = expert_slots(torch.from_numpy(x).cuda(), e)
+    for a, b in zip(got, ref_slots(x, e)):
+        assert a.dtype == torch.int32
+        np.testing.assert_array_equal(a.cpu().numpy(), b)
+
+
+# --------------------------------------------------------------------------- weighted sums
+def _combine_inputs(n, k, d, m, dtype, seed, repeated=False):
+    g = torch.Generator().manual_seed(seed)
+    values = torch.randn(m, d, generator=g).to(dtype)
+    if repeated:
+        slots = torch.randint(-1, m + 2, (n, k), generator=g)
+    else:
+        slots = torch.randperm(max(m, n * k), generator=g)[: n * k].view(n, k)
+        slots[torch.rand(n, k, generator=g) < 0.2] = -1
+    weights = torch.randn(n, k, generator=g)
+    weights[(slots < 0) | (slots >= m)] = float("nan")       # what a missing row weighs counts nowhere
+    return values, slots.to(torch.int32), weights, torch.randn(n, d, generator=g).to(dtype)
+
+
+def ref_combine(values, slots, weights, grad):
+    v, w, g = values.double(), weights.double(), grad.double()
+    out, gv, gw = torch.zeros(grad.shape, dtype=torch.float64), torch.zeros(v.shape, dtype=torch.float64), torch.zeros(w.shape, dtype=torch.float64)
+    big_o, big_v = torch.zeros_like(out), torch.zeros_like(gv)
+    for t in range(slots.shape[0]):
+        for j in range(slots.shape[1]):
+            r = int(slots[t, j])
+            if 0 <= r < v.shape[0]:
+                out[t] += w[t, j] * v[r]
+                big_o[t] += (w[t, j] * v[r]).abs()
+                gv[r] += w[t, j] * g[t]
+                big_v[r] += (w[t, j] * g[t]).abs()
+                gw[t, j] = (v[r] * g[t]).sum()
+    return out, gv, gw, big_o, big_v
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,d,m", [(1, 1, 1, 1), (1, 8, 4096, 8), (3, 2, 7, 9), (5, 8, 1031, 40), (17, 9, 64, 153), (33, 20, 129, 700),
+                                     (9, 3, 8200, 27), (4, 2, 16, 0), (0, 2, 16, 5)])
+@pytest.mark.parametrize("repeated", [False, True])
+def test_combine(dtype, n, k, d, m, repeated):
+    """Every sum of N products is off by N u of the sum of their magnitudes at most."""
+    from sklearn_numba_dpex_b200.common import combine_experts, combine_experts_grad
+
+    t = TYPES[dtype]
+    values, slots, weights, grad = _combine_inputs(n, k, d, m, t, 7, repeated)
+    out, gv, gw, big_o, big_v = ref_combine(values, slots, weights, grad)
+    dev = [x.cuda() for x in (values, slots, weights, grad)]
+    half = torch.finfo(t).eps / 2
+    tiny = torch.finfo(t).smallest_normal * torch.finfo(t).eps
+    got = combine_experts(*dev[:3])
+    assert got.dtype == t
+    assert ((got.double().cpu() - out).abs() <= (k + 1) * U * big_o + half * out.abs() + tiny).all()
+    got_v, got_w = combine_experts_grad(*dev)
+    users = max(1, int(torch.bincount(slots[(slots >= 0) & (slots < m)].long(), minlength=1).max())) if n else 1
+    assert ((got_v.double().cpu() - gv).abs() <= (users + 1) * U * big_v + half * gv.abs() + tiny).all()
+    size = torch.zeros(n, k, dtype=torch.float64)
+    for a in range(n):
+        for b in range(k):
+            if 0 <= slots[a, b] < m:
+                size[a, b] = (values[int(slots[a, b])].double() * grad[a].double()).abs().sum()
+    assert ((got_w.double().cpu() - gw).abs() <= (d + 1) * U * size).all()
+    again = combine_experts_grad(*dev)
+    assert torch.equal(again[0], got_v) and torch.equal(again[1], got_w)       # no order left to chance
+    if n and m:
+        a, b = dev[0].clone().requires_grad_(True), dev[2].clone().requires_grad_(True)
+        combine_experts(a, dev[1], b).backward(dev[3])
+        assert torch.equal(a.grad, got_v) and torch.equal(b.grad, got_w)
+
+
+def test_combine_many_users_of_one_row():
+    from sklearn_numba_dpex_b200.common import combine_experts_grad
+
+    n, k, d = 700, 3, 40
+    values, grad = torch.randn(5, d), torch.randn(n, d)
+    slots = torch.full((n, k), 2, dtype=torch.int32)
+    slots[::3, 1] = 4
+    weights = torch.rand(n, k)
+    out, gv, gw, _, big_v = ref_combine(values, slots, weights, grad)
+    got_v, _ = combine_experts_grad(values.cuda(), slots.cuda(), weights.cuda(), grad.cuda())
+    assert ((got_v.double().cpu() - gv).abs() <= (n * k + 1) * U * big_v).all()
+
+
+# --------------------------------------------------------------------------- used together
+def _layer(x, logits, w, w_scales, k, n_experts):
+    from sklearn_numba_dpex_b200 import common
+
+    weights, experts = common.route_topk(logits, k)
+    slots, rows, offsets = common.expert_slots(experts, n_experts)
+    q, scales = common.quantize_rows(x, rows=rows)
+    y = common.int8_matmul(q, scales, w, w_scales, offsets=offsets, out_dtype=torch.float32)
+    return weights, experts, slots, y, common.combine_experts(y, slots, weights)
+
+
+def _layer_inputs(n, e, dim, out, seed):
+    g = torch.Generator().manual_seed(seed)
+    x, logits = torch.randn(n, dim, generator=g), torch.randn(n, e, generator=g)
+    logits[n // 2] = float("-inf")                # a padding token in the middle of the batch
+    w = torch.randint(-127, 128, (e, out, dim), generator=g, dtype=torch.int8)
+    return x.cuda(), logits.cuda(), w.cuda(), (torch.rand(e, out, generator=g) * 0.01).cuda()
+
+
+def _ref_layer(x, logits, w, w_scales, k):
+    """float64, each token by itself; returns the result and what its sums add up to in magnitude."""
+    x, logits, w, ws = x.cpu().double().numpy(), logits.cpu().double().numpy(), w.cpu().numpy().astype(np.float64), w_scales.cpu().double().numpy()
+    weights, experts = ref_route(logits, k)
+    out = np.zeros((x.shape[0], w.shape[1]))
+    size = np.zeros_like(out)
+    for t in range(x.shape[0]):
+        top = np.abs(x[t]).max()
+        q = np.rint(x[t] * 127 / top)
+        for j in range(k):
+            if experts[t, j] >= 0:
+                y = (w[experts[t, j]] @ q) * (top / 127) * ws[experts[t, j]]
+                out[t] += weights[t, j] * y
+                size[t] += weights[t, j] * np.abs(y)
+    return out, size
+
+
+@pytest.mark.parametrize("n,e,dim,out,k", [(1, 8, 64, 96, 2), (37, 16, 200, 130, 4), (300, 5, 129, 257, 3)])
+def test_layer_of_experts(n, e, dim, out, k):
+    x, logits, w, ws = _layer_inputs(n, e, dim, out, 11)
+    weights, experts, slots, y, got = _layer(x, logits, w, ws, k, e)
+    want, size = _ref_layer(x, logits, w, ws, k)
+    # a share is off by 256 u, a product by 4 u (scales, their product), the sum by k + 1 roundings
+    assert (np.abs(got.cpu().double().numpy() - want) <= (256 + 4 + k + 1) * U * size).all()
+    # gradients through the sum and the routing, against float64 autograd of the same choice
+    leaf, values = logits.clone().requires_grad_(True), y.clone().requires_grad_(True)
+    from sklearn_numba_dpex_b200.common import combine_experts, route_topk
+
+    wts, _ = route_topk(leaf, k)
+    g = torch.randn(n, out, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    combine_experts(values, slots, wts).backward(g)
+    l64, v64 = logits.double().requires_grad_(True), y.double().requires_grad_(True)
+    there = experts >= 0
+    picked = torch.where(there, l64.gather(1, experts.long().clamp_min(0)), torch.tensor(-1e300, dtype=torch.float64, device="cuda"))
+    share = torch.softmax(picked, 1) * there
+    rows = torch.where(there[..., None], v64[slots.long().clamp_min(0)], torch.zeros((), dtype=torch.float64, device="cuda"))
+    (rows * share[..., None]).sum(1).backward(g.double())
+    gw = (rows.detach() * g.double()[:, None]).sum(2).abs().max()
+    dots = (rows.detach() * g.double()[:, None]).abs().sum(2).max()
+    grad = torch.nan_to_num(l64.grad)
+    assert float((leaf.grad.double() - grad).abs().max()) <= 512 * U * float(gw) + 2 * (out + 1) * U * float(dots)
+    assert float((values.grad.double() - v64.grad).abs().max()) <= 257 * U * float(g.abs().max())
+
+
+def test_layer_on_another_stream_and_in_a_graph():
+    """The run of operators on a stream of its own, captured, and replayed on new inputs."""
+    n, e, dim, out, k = 65, 16, 144, 100, 3
+    first, second = _layer_inputs(n, e, dim, out, 21), _layer_inputs(n, e, dim, out, 22)
+    want = [_layer(*a, k, e) for a in (first, second)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _layer(*first, k, e)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want[0]):
+        assert torch.equal(a, b)
+    inputs = [t.clone() for t in first]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = _layer(*inputs, k, e)
+    for source, expected in ((second, want[1]), (first, want[0])):
+        for t, s in zip(inputs, source):
+            t.copy_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, expected):
+            assert torch.equal(a, b)
+
+
+def test_gradients_in_a_graph():
+    from sklearn_numba_dpex_b200.common import combine_experts_grad, route_topk_grad
+
+    x = torch.randn(50, 32, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    from sklearn_numba_dpex_b200.common import route_topk
+
+    w, e = route_topk(x, 4)
+    values, grad = torch.randn(200, 24, device="cuda"), torch.randn(50, 24, device="cuda")
+    slots = torch.randperm(200, device="cuda").to(torch.int32).view(50, 4)
+
+    def back():
+        gv, gw = combine_experts_grad(values, slots, w, grad)
+        return gv, route_topk_grad(x, e, gw)
+
+    want = back()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = back()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held[0], want[0]) and torch.equal(held[1], want[1])
+
+
+def test_refusals_on_the_gpu():
+    from sklearn_numba_dpex_b200.common import combine_experts, expert_slots, route_topk, route_topk_grad
+
+    x = torch.randn(4, 8, device="cuda")
+    for bad in (dict(k=0), dict(k=9), dict(k=2, scoring="relu"), dict(k=2, n_groups=3), dict(k=2, n_groups=0),
+                dict(k=5, n_groups=2, topk_groups=1), dict(k=2, n_groups=2, topk_groups=3), dict(k=2, n_groups=2, group_best=3),
+                dict(k=1, n_groups=8, topk_groups=2, group_best=2), dict(k=2, bias=torch.zeros(7, device="cuda")),
+                dict(k=2, bias=torch.zeros(8)), dict(k=2, bias=torch.zeros(8, device="cuda", dtype=torch.float64))):
+        with pytest.raises(ValueError):
+            route_topk(x, **bad)
+    with pytest.raises(ValueError):
+        route_topk(x.double(), 2)
+    with pytest.raises(ValueError):
+        route_topk(torch.randn(4, 1025, device="cuda"), 2)
+    with pytest.raises(ValueError):
+        route_topk(torch.randn(4, 64, device="cuda"), 33)
+    w, e = route_topk(x, 2)
+    with pytest.raises(ValueError):
+        route_topk_grad(x, e.long(), w)
+    with pytest.raises(ValueError):
+        route_topk_grad(x, e[:3], w[:3])
+    with pytest.raises(ValueError):
+        expert_slots(e, 1025)
+    with pytest.raises(ValueError):
+        expert_slots(e, 0)
+    with pytest.raises(ValueError):
+        expert_slots(e.float(), 8)
+    with pytest.raises(ValueError):
+        combine_experts(x, e, w[:, :1])
+    with pytest.raises(ValueError):
+        combine_experts(x.double(), e, w)
+    assert torch.isfinite(route_topk(x, 2)[0]).all()
