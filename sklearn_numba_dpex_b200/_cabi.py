@@ -180,23 +180,15 @@ def stream_ptr(device=None):
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-class on_device_of:
-    """Makes a tensor's device the current one for a call: the library asks the current device for
-    its size, and launches go to a stream of that device."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, t):
-        self.index = t.device.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def launch(name, device, *args):
+    """Enqueues a library call on `device`'s current stream, which it gets as its last argument, with
+    `device` the current one: the library asks the current device for its size.  Addresses may be
+    plain numbers here (a small call costs a few microseconds on the host, and wrapping them shows)."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return launch(name, device, *args)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    return check(getattr(lib, name)(*args, stream), name)
 
 
 def require_cuda_tensor(t, name, dtype=None, contiguous=True):

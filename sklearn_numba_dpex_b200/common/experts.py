@@ -14,8 +14,7 @@ All tensors live on one CUDA device; a call is enqueued on that device's current
 """
 import torch
 
-from .._cabi import (ROUTE_RENORMALIZE, ROUTE_SIGMOID, check, lib, on_device_of, ptr, require_cuda_tensor,
-                     row_dtype_code, stream_ptr)
+from .._cabi import ROUTE_RENORMALIZE, ROUTE_SIGMOID, launch, lib, require_cuda_tensor, row_dtype_code
 
 _SCORINGS = {"softmax": 0, "sigmoid": ROUTE_SIGMOID}
 
@@ -24,7 +23,7 @@ def _matrix(t, name, dtype=None):
     require_cuda_tensor(t, name, dtype, contiguous=False)
     if t.dim() != 2:
         raise ValueError(f"{name} must have two dimensions, got {t.dim()}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _same_device(t, name, other):
@@ -44,10 +43,9 @@ def _route(logits, k, bias, flags, n_groups, topk_groups, group_best, scale):
     dev = logits.device
     weights = torch.empty((n, k), dtype=torch.float32, device=dev)
     experts = torch.empty((n, k), dtype=torch.int32, device=dev)
-    with on_device_of(logits):
-        check(lib.kmb_route_topk(row_dtype_code(logits.dtype, "logits"), ptr(logits), ptr(bias), n, e, k, flags,
-                                 n_groups, topk_groups, group_best, scale, ptr(weights), ptr(experts),
-                                 stream_ptr(dev)), "kmb_route_topk")
+    launch("kmb_route_topk", dev, row_dtype_code(logits.dtype, "logits"), logits.data_ptr(),
+           None if bias is None else bias.data_ptr(), n, e, k, flags, n_groups, topk_groups, group_best, scale,
+           weights.data_ptr(), experts.data_ptr())
     return weights, experts
 
 
@@ -118,11 +116,9 @@ def route_topk_grad(logits, experts, grad_weights, scoring="softmax", renormaliz
     _same_device(experts, "experts", logits)
     _same_device(grad_weights, "grad_weights", logits)
     grad = torch.empty_like(logits)
-    with on_device_of(logits):
-        check(lib.kmb_route_topk_grad(row_dtype_code(logits.dtype, "logits"), ptr(logits), ptr(experts),
-                                      ptr(grad_weights), n, e, experts.shape[1], _flags(scoring, renormalize),
-                                      float(scale), ptr(grad), stream_ptr(logits.device)),
-              "kmb_route_topk_grad")
+    launch("kmb_route_topk_grad", logits.device, row_dtype_code(logits.dtype, "logits"), logits.data_ptr(),
+           experts.data_ptr(), grad_weights.data_ptr(), n, e, experts.shape[1], _flags(scoring, renormalize),
+           float(scale), grad.data_ptr())
     return grad
 
 
@@ -146,9 +142,8 @@ def expert_slots(experts, n_experts):
     offsets = torch.empty(max(n_experts, 0) + 1, dtype=torch.int32, device=dev)
     nbytes = lib.kmb_expert_slots_workspace_bytes(n, k, n_experts)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with on_device_of(experts):
-        check(lib.kmb_expert_slots(ptr(experts), n, k, n_experts, ptr(slots), ptr(rows), ptr(offsets), ptr(ws),
-                                   nbytes, stream_ptr(dev)), "kmb_expert_slots")
+    launch("kmb_expert_slots", dev, experts.data_ptr(), n, k, n_experts, slots.data_ptr(), rows.data_ptr(),
+           offsets.data_ptr(), ws.data_ptr() if nbytes else None, nbytes)
     return slots, rows, offsets
 
 
@@ -168,10 +163,8 @@ def _combine(values, slots, weights):
     n, k = slots.shape
     dev = values.device
     out = torch.empty((n, values.shape[1]), dtype=values.dtype, device=dev)
-    with on_device_of(values):
-        check(lib.kmb_combine_experts(row_dtype_code(values.dtype, "values"), ptr(values), values.shape[0],
-                                      ptr(slots), ptr(weights), n, k, values.shape[1], ptr(out), stream_ptr(dev)),
-              "kmb_combine_experts")
+    launch("kmb_combine_experts", dev, row_dtype_code(values.dtype, "values"), values.data_ptr(), values.shape[0],
+           slots.data_ptr(), weights.data_ptr(), n, k, values.shape[1], out.data_ptr())
     return out
 
 
@@ -216,9 +209,7 @@ def combine_experts_grad(values, slots, weights, grad_out):
     grad_values, grad_weights = torch.empty_like(values), torch.empty_like(weights)
     nbytes = lib.kmb_combine_experts_grad_workspace_bytes(values.shape[0])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with on_device_of(values):
-        check(lib.kmb_combine_experts_grad(row_dtype_code(values.dtype, "values"), ptr(values), values.shape[0],
-                                           ptr(slots), ptr(weights), ptr(grad_out), n, k, values.shape[1],
-                                           ptr(grad_values), ptr(grad_weights), ptr(ws), nbytes, stream_ptr(dev)),
-              "kmb_combine_experts_grad")
+    launch("kmb_combine_experts_grad", dev, row_dtype_code(values.dtype, "values"), values.data_ptr(),
+           values.shape[0], slots.data_ptr(), weights.data_ptr(), grad_out.data_ptr(), n, k, values.shape[1],
+           grad_values.data_ptr(), grad_weights.data_ptr(), ws.data_ptr(), nbytes)
     return grad_values, grad_weights

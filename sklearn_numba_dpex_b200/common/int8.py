@@ -5,7 +5,7 @@ import ctypes
 
 import torch
 
-from .._cabi import check, lib, on_device_of, ptr, require_cuda_tensor, row_dtype_code, stream_ptr
+from .._cabi import check, launch, lib, require_cuda_tensor, row_dtype_code, stream_ptr
 
 #: Features that a sum of products of 8-bit integers may run over before it could leave 32 bits.
 MAX_FEATURES = 131071
@@ -40,7 +40,7 @@ def quantize_rows(x, rows=None):
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x must have shape (n, d) with d >= 1, got {tuple(x.shape)}")
     code = row_dtype_code(x.dtype, "x")
-    x = x.detach().contiguous()
+    x = x if x.is_contiguous() else x.contiguous()
     n, d = x.shape
     m = n
     if rows is not None:
@@ -52,9 +52,8 @@ def quantize_rows(x, rows=None):
     dev = x.device
     q = torch.empty((m, pitch), dtype=torch.int8, device=dev)
     scales = torch.empty(m, dtype=torch.float32, device=dev)
-    with on_device_of(x):
-        check(lib.kmb_quantize_rows(code, ptr(x), n, d, ptr(rows), m, ptr(q), pitch, ptr(scales), stream_ptr(dev)),
-              "kmb_quantize_rows")
+    launch("kmb_quantize_rows", dev, code, x.data_ptr(), n, d, None if rows is None else rows.data_ptr(), m,
+           q.data_ptr(), pitch, scales.data_ptr())
     return (q if pitch == d else q[:, :d]), scales
 
 
@@ -104,9 +103,9 @@ def int8_matmul(a, a_scales, b, b_scales, bias=None, offsets=None, out_dtype=tor
         raise ValueError("d and the number of groups must be at least 1")
     a, lda = _pitched(a, "a")
     b, ldb = _pitched(b, "b")
-    with on_device_of(a):
-        check(lib.kmb_int8_matmul(code, ptr(a), lda, ptr(a_scales), ptr(b), ldb, ptr(b_scales), ptr(bias),
-                                  ptr(offsets), g, ptr(out), m, n, d, stream_ptr(dev)), "kmb_int8_matmul")
+    launch("kmb_int8_matmul", dev, code, a.data_ptr(), lda, a_scales.data_ptr(), b.data_ptr(), ldb,
+           b_scales.data_ptr(), None if bias is None else bias.data_ptr(),
+           None if offsets is None else offsets.data_ptr(), g, out.data_ptr(), m, n, d)
     return out
 
 

@@ -12,8 +12,8 @@ namespace kmb {
 constexpr unsigned FULL = 0xffffffffu;
 
 // ================================================================================== routing
-// One warp per token.  Lane l holds the V consecutive experts l * V .. l * V + V - 1 in registers, so
-// that the lowest lane among equals is the lowest index.
+// L lanes of a warp per token (8, 16 or 32).  Lane l of them holds the V consecutive experts l * V ..
+// l * V + V - 1 in registers, so that the lowest lane among equals is the lowest index.
 constexpr int RT_WARPS = 4;
 constexpr int RT_MAX_EXPERTS = 1024;
 constexpr int RT_MAX_K = 32;       // the choices of a token live one to a lane
@@ -32,10 +32,10 @@ struct RouteParams {
 
 // Whole numbers in the order of the values, NaN on top; 0 is below everything, -inf among it.
 __device__ __forceinline__ uint32_t order_bits(float v) {
-  if (v != v) return 0xffffffffu;
   uint32_t b = __float_as_uint(v + 0.f);      // -0 and 0 are one value
   b ^= (b >> 31) ? 0xffffffffu : 0x80000000u;
-  return b == 0x007fffffu ? 0u : b;           // -inf: never chosen
+  b = b == 0x007fffffu ? 0u : b;              // -inf: never chosen
+  return v != v ? 0xffffffffu : b;
 }
 __device__ __forceinline__ unsigned long long order_bits(double v) {
   if (v != v) return 0xffffffffffffffffull;
@@ -43,15 +43,13 @@ __device__ __forceinline__ unsigned long long order_bits(double v) {
   b ^= (b >> 63) ? 0xffffffffffffffffull : 0x8000000000000000ull;
   return b == 0x000fffffffffffffull ? 0ull : b;
 }
-__device__ __forceinline__ uint32_t warp_max_bits(uint32_t v) { return __reduce_max_sync(FULL, v); }
-__device__ __forceinline__ unsigned long long warp_max_bits(unsigned long long v) {
-  const uint32_t hi = (uint32_t)(v >> 32), top = __reduce_max_sync(FULL, hi);
-  const uint32_t lo = __reduce_max_sync(FULL, hi == top ? (uint32_t)v : 0u);
-  return ((unsigned long long)top << 32) | lo;
-}
 __device__ __forceinline__ float from_order_bits(uint32_t b) {
   if (b == 0u) return __int_as_float(0xff800000);
   return __uint_as_float((b >> 31) ? b ^ 0x80000000u : ~b);
+}
+__device__ __forceinline__ double from_order_bits(unsigned long long b) {
+  if (b == 0ull) return __longlong_as_double(0xfff0000000000000LL);
+  return __longlong_as_double((long long)((b >> 63) ? b ^ 0x8000000000000000ull : ~b));
 }
 template <typename K>
 struct OrderBits;
@@ -60,20 +58,42 @@ struct OrderBits<float> { typedef uint32_t type; };
 template <>
 struct OrderBits<double> { typedef unsigned long long type; };
 
+// Greatest value and sum over the L lanes of a token.
+template <int L, typename B>
+__device__ __forceinline__ B lanes_max(B v) {
+  if constexpr (L == 32 && sizeof(B) == 4) {
+    return __reduce_max_sync(FULL, v);
+  } else {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+      const B u = __shfl_xor_sync(FULL, v, o);
+      v = u > v ? u : v;
+    }
+    return v;
+  }
+}
+template <int L, typename K>
+__device__ __forceinline__ K lanes_sum(K v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  return v;
+}
+template <typename K>
+__device__ __forceinline__ K warp_sum_of(K v) { return lanes_sum<32>(v); }
+
+// The bits of a ballot that belong to this token's lanes.
+template <int L>
+__device__ __forceinline__ unsigned lanes_of(unsigned ballot, int lane) {
+  if constexpr (L == 32) return ballot;
+  else return (ballot >> (lane & ~(L - 1))) & ((1u << L) - 1u);
+}
+
 __device__ __forceinline__ float exp_of(float x) { return expf(x); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 
-template <typename K>
-__device__ __forceinline__ K warp_sum_of(K v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
-  return v;
-}
-
-// What a pass over one token finds: lane j < k holds choice j.
+// What a pass over one token finds: lane j < k of its lanes holds choice j.
 struct Chosen {
   int expert;      // or -1
-  float logit;
   bool unsure;     // (32 bits) two values that the choice hangs on lie closer than they are exact
 };
 
@@ -85,12 +105,12 @@ struct Chosen {
 // each, the quotient, the bias's addition.  (V + 16) 2^-24 of the largest score and key covers both
 // keys of a pair.  A token with such a pair (about one in a hundred) is done again in 64 bits, which
 // is what the definition says.  Equal logits with equal biases have equal keys and need no second look.
-template <typename K, int V>
-__device__ __noinline__ Chosen route_token(const RouteParams& p, const float (&x)[V], int lane, bool by_logit,
-                                           float* s_keys) {
+template <typename K, int L, int V, typename T>
+__device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row, const float (&x)[V], int lane,
+                                              bool by_logit, float* s_keys) {
   typedef typename OrderBits<K>::type B;
   constexpr bool narrow = sizeof(K) == 4;
-  const int e0 = lane * V;
+  const int sub = lane & (L - 1), e0 = sub * V;
   const K ninf = -(K)INFINITY;
   K key[V];
   K margin = 0;
@@ -106,7 +126,7 @@ __device__ __noinline__ Chosen route_token(const RouteParams& p, const float (&x
       uint32_t t = 0;
 #pragma unroll
       for (int i = 0; i < V; ++i) t = max(t, order_bits(x[i]));
-      t = warp_max_bits(t);
+      t = lanes_max<L>(t);
       const K top = t == 0xffffffffu ? (K)NAN : t == 0u ? (K)0 : (K)from_order_bits(t);
       K sum = 0;
 #pragma unroll
@@ -114,7 +134,7 @@ __device__ __noinline__ Chosen route_token(const RouteParams& p, const float (&x
         key[i] = exp_of((K)x[i] - top);
         sum += key[i];
       }
-      sum = warp_sum_of(sum);
+      sum = lanes_sum<L>(sum);
       sum = sum == (K)0 ? (K)1 : sum;
 #pragma unroll
       for (int i = 0; i < V; ++i) key[i] = key[i] / sum;
@@ -134,14 +154,13 @@ __device__ __noinline__ Chosen route_token(const RouteParams& p, const float (&x
       if (narrow && key[i] > ninf) most = fmaxf((float)most, fabsf((float)key[i]));
     }
     if (narrow) {
-      uint32_t m = __float_as_uint((float)most);
-      m = __reduce_max_sync(FULL, m);
+      const uint32_t m = lanes_max<L>(__float_as_uint((float)most));
       margin = (K)((float)(V + 16) * 0x1p-24f) * (top_score + (K)__uint_as_float(m));
     }
   }
   bool unsure = false;
 
-  if (p.groups > 1) {
+  if (L == 32 && p.groups > 1) {
     // lane g works out the score of group g from the keys in shared memory
     K* keys = reinterpret_cast<K*>(s_keys);
     __syncwarp();
@@ -199,85 +218,49 @@ __device__ __noinline__ Chosen route_token(const RouteParams& p, const float (&x
   B bits[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) bits[i] = e0 + i < p.n_experts ? order_bits(key[i]) : (B)0;
-  B best = 0;
-  int best_i = 0;
-  float best_x = 0.f;
-  K best_key = ninf;
-  auto rescan = [&]() {
-    best = 0;
-#pragma unroll
-    for (int i = V - 1; i >= 0; --i)
-      if (bits[i] >= best) {
-        best = bits[i];
-        best_i = i;
-        best_x = x[i];
-        best_key = key[i];
-      }
-  };
-  rescan();
-  Chosen c = {-1, 0.f, false};
-  K mine = ninf, next = ninf;
-  float next_x = 0.f;
+  Chosen c = {-1, false};
+  B mine = 0, next = 0;
   int next_e = -1;
   const bool check = narrow && p.bias != nullptr;
   const int rounds = check ? p.k + 1 : p.k;      // the first that is left out counts too
   for (int j = 0; j < rounds; ++j) {
-    const B top = warp_max_bits(best);
-    if (top == 0) break;
-    const int w = __ffs(__ballot_sync(FULL, best == top)) - 1;
-    const int e = __shfl_sync(FULL, e0 + best_i, w);
-    const float ex = __shfl_sync(FULL, best_x, w);
-    const K ek = check ? __shfl_sync(FULL, best_key, w) : (K)0;
-    if (lane == j && j < p.k) {
-      c.expert = e;
-      c.logit = ex;
-      mine = ek;
-    }
-    if (lane == j - 1) {
-      next = ek;
-      next_x = ex;
-      next_e = e;
-    }
-    if (lane == w) {
+    B best = bits[0];
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i == best_i) bits[i] = 0;
-      rescan();
+    for (int i = 1; i < V; ++i) best = best > bits[i] ? best : bits[i];
+    const B top = lanes_max<L>(best);
+    const unsigned won = lanes_of<L>(__ballot_sync(FULL, best == top), lane);
+    const int w = __ffs(won) - 1;
+    int at = V - 1;
+#pragma unroll
+    for (int i = V - 2; i >= 0; --i) at = bits[i] == best ? i : at;
+    if (sub == w) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) bits[i] = i == at ? (B)0 : bits[i];
+    }
+    const int at_w = __shfl_sync(FULL, at, (lane & ~(L - 1)) + w);
+    const int e = top == 0 ? -1 : at_w + w * V;
+    if (sub == j && j < p.k) {
+      c.expert = e;
+      mine = top;
+    }
+    if (sub == j - 1) {
+      next = top;
+      next_e = e;
     }
   }
   if (check) {
-    bool close = lane < p.k && next_e >= 0 && !(mine - next > margin);
-    if (close && c.logit == next_x && p.bias[c.expert] == p.bias[next_e]) close = false;
-    unsure = unsure || __any_sync(FULL, close);
+    bool close = sub < p.k && c.expert >= 0 && next_e >= 0 && !(from_order_bits(mine) - from_order_bits(next) > margin);
+    // the same bias on the same logit: the same key
+    if (close && p.bias[c.expert] == p.bias[next_e] && to_float(row[c.expert]) == to_float(row[next_e])) close = false;
+    unsure = unsure || lanes_of<L>(__ballot_sync(FULL, close), lane) != 0;
   }
   c.unsure = unsure;
   return c;
 }
 
-// exp(-|x|) never leaves the range, and keeps the small scores of negative logits.
-__device__ __forceinline__ float sigmoid_of(float x) {
-  const float t = expf(-fabsf(x));
-  return (x < 0.f ? t : 1.f) / (1.f + t);
-}
-
-// Share of each lane's choice among the choices of its token (sum 1), 0 where there is none.
-// Softmax: exp(x - top of the chosen) over its sum.  Sigmoid: s over its sum, with exp(x) for s
-// where all chosen logits lie below -60 (there s = exp(x) to 2^-80, and s itself runs out of range).
-__device__ __forceinline__ float share_of(bool there, float x, bool sigmoid) {
-  uint32_t t = warp_max_bits(there ? order_bits(x) : 0u);
-  const float top = from_order_bits(t);
-  float s;
-  if (sigmoid && !(top < -60.f)) s = sigmoid_of(x);
-  else s = expf(x - top);
-  if (t == 0xffffffffu) s = __uint_as_float(0x7fffffffu);
-  if (!there) s = 0.f;
-  float sum = warp_sum_of(s);
-  return there ? s / sum : 0.f;
-}
-
 template <typename T, int V>
-__device__ __forceinline__ void route_load(const T* row, int lane, int n_experts, int vec, float (&x)[V]) {
-  const int e0 = lane * V;
+__device__ __forceinline__ void route_load(const T* row, int sub, int n_experts, int vec, float (&x)[V]) {
+  const int e0 = sub * V;
   constexpr int BYTES = V * (int)sizeof(T);
   if (vec && e0 + V <= n_experts) {
     if constexpr (BYTES >= 16) {
@@ -286,67 +269,99 @@ __device__ __forceinline__ void route_load(const T* row, int lane, int n_experts
       for (int j = 0; j < BYTES / 16; ++j) r.u[j] = reinterpret_cast<const uint4*>(row + e0)[j];
 #pragma unroll
       for (int i = 0; i < V; ++i) x[i] = to_float(r.t[i]);
-      return;
-    } else if constexpr (BYTES == 8) {
+    } else {
       union { uint2 u; T t[V]; } r;
       r.u = *reinterpret_cast<const uint2*>(row + e0);
 #pragma unroll
       for (int i = 0; i < V; ++i) x[i] = to_float(r.t[i]);
-      return;
-    } else if constexpr (BYTES == 4) {
-      union { uint32_t u; T t[V]; } r;
-      r.u = *reinterpret_cast<const uint32_t*>(row + e0);
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[i] = to_float(r.t[i]);
-      return;
     }
+    return;
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) x[i] = e0 + i < n_experts ? to_float(row[e0 + i]) : -INFINITY;
 }
 
+// The pass in 64 bits, for the tokens that asked for it; all lanes of the warp take part.
+template <typename T, int L, int V>
+__device__ __noinline__ int route_again(const RouteParams& p, const T* row, int lane, float* s_keys) {
+  float x[V];
+  route_load<T, V>(row, lane & (L - 1), p.n_experts, p.vec, x);
+  return route_token<double, L, V>(p, row, x, lane, false, s_keys).expert;
+}
+
+__device__ __forceinline__ float sigmoid_of(float x) {
+  // exp(-|x|) never leaves the range, and keeps the small scores of negative logits
+  const float t = expf(-fabsf(x));
+  return (x < 0.f ? t : 1.f) / (1.f + t);
+}
+
+// Share of each lane's choice among the choices of its token (sum 1), 0 where there is none.
+// Softmax: exp(x - top of the chosen) over its sum.  Sigmoid: s over its sum, with exp(x) for s
+// where all chosen logits lie below -60 (there s = exp(x) to 2^-80, and s itself runs out of range).
+template <int L>
+__device__ __forceinline__ float share_of(bool there, float x, bool sigmoid) {
+  const uint32_t t = lanes_max<L>(there ? order_bits(x) : 0u);
+  const float top = from_order_bits(t);
+  float s;
+  if (sigmoid && !(top < -60.f)) s = sigmoid_of(x);
+  else s = expf(x - top);
+  if (t == 0xffffffffu) s = __uint_as_float(0x7fffffffu);
+  if (!there) s = 0.f;
+  const float sum = lanes_sum<L>(s);
+  return there ? s / sum : 0.f;
+}
+
 // (top, sum of exp(x - top)) of a token's logits; top 0 where nothing but -inf is there.
-template <int V>
+template <int L, int V>
 __device__ __forceinline__ void softmax_stats(const float (&x)[V], float& top, float& sum) {
   uint32_t t = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) t = max(t, order_bits(x[i]));
-  t = warp_max_bits(t);
+  t = lanes_max<L>(t);
   top = t == 0u ? 0.f : t == 0xffffffffu ? __uint_as_float(0x7fffffffu) : from_order_bits(t);
   sum = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) sum += expf(x[i] - top);
-  sum = warp_sum_of(sum);
+  sum = lanes_sum<L>(sum);
   if (sum == 0.f) sum = 1.f;
 }
 
-template <typename T, int V>
+template <typename T, int L, int V>
 __global__ void __launch_bounds__(RT_WARPS * 32)
-route_topk_kernel(const RouteParams p) {
+route_topk_kernel(const __grid_constant__ RouteParams p) {
   // groups: one row of keys per warp, wide enough for 64-bit keys
   extern __shared__ __align__(16) float s_route[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int PER = 32 / L;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (L - 1);
   float* s_keys = s_route + (size_t)warp * 2 * p.n_experts;
   const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_best == 1);
-  for (int64_t i = (int64_t)blockIdx.x * RT_WARPS + warp; i < p.n; i += (int64_t)gridDim.x * RT_WARPS) {
+  const int64_t step = (int64_t)gridDim.x * RT_WARPS * PER;
+  for (int64_t i0 = ((int64_t)blockIdx.x * RT_WARPS + warp) * PER; i0 < p.n; i0 += step) {
+    const int64_t mine = i0 + lane / L;
+    const int64_t i = mine < p.n ? mine : p.n - 1;       // lanes without a token repeat the last one
+    const T* row = (const T*)p.logits + i * p.n_experts;
     float x[V];
-    route_load<T, V>((const T*)p.logits + i * p.n_experts, lane, p.n_experts, p.vec, x);
-    Chosen c = route_token<float, V>(p, x, lane, by_logit, s_keys);
-    if (c.unsure) c = route_token<double, V>(p, x, lane, by_logit, s_keys);
+    route_load<T, V>(row, sub, p.n_experts, p.vec, x);
+    Chosen c = route_token<float, L, V>(p, row, x, lane, by_logit, s_keys);
+    if (!by_logit && __any_sync(FULL, c.unsure)) {
+      const int e = route_again<T, L, V>(p, row, lane, s_keys);
+      if (c.unsure) c.expert = e;
+    }
     const bool there = c.expert >= 0;
+    const float xe = there ? to_float(row[c.expert]) : 0.f;
     float w;
     float top = 0.f, sum = 1.f;
     const bool stats = !p.sigmoid && (!p.renormalize || !by_logit);
-    if (stats) softmax_stats<V>(x, top, sum);
+    if (stats) softmax_stats<L, V>(x, top, sum);
     if (p.renormalize) {
-      w = share_of(there, c.logit, p.sigmoid != 0);
+      w = share_of<L>(there, xe, p.sigmoid != 0);
       if (stats && sum != sum) w = sum;            // a NaN that was not chosen still is in every score
     } else {
-      w = p.sigmoid ? sigmoid_of(c.logit) : expf(c.logit - top) / sum;
+      w = p.sigmoid ? sigmoid_of(xe) : expf(xe - top) / sum;
     }
-    if (lane < p.k) {
-      p.weights[i * p.k + lane] = there ? w * p.scale : 0.f;
-      p.experts[i * p.k + lane] = c.expert;
+    if (sub < p.k && mine < p.n) {
+      p.weights[i * p.k + sub] = there ? w * p.scale : 0.f;
+      p.experts[i * p.k + sub] = c.expert;
     }
   }
 }
@@ -367,22 +382,27 @@ struct RouteGradParams {
 //   sigmoid, renormalised   p_j (g_j - sum p g) (1 - s_j)       on the chosen
 //   sigmoid                 g_j s_j (1 - s_j)                   on the chosen
 //   softmax                 s_e ([e chosen] g_e - sum s g)      everywhere
-// The warp writes the row's dense part and then, ordered by __syncwarp, the chosen places.
-template <typename T, int V>
+// A token's lanes write the row's dense part and then, ordered by __syncwarp, the chosen places.
+template <typename T, int L, int V>
 __global__ void __launch_bounds__(RT_WARPS * 32)
-route_topk_grad_kernel(const RouteGradParams p) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = lane * V;
+route_topk_grad_kernel(const __grid_constant__ RouteGradParams p) {
+  constexpr int PER = 32 / L;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (L - 1), e0 = sub * V;
   const bool dense = !p.sigmoid && !p.renormalize;
-  for (int64_t i = (int64_t)blockIdx.x * RT_WARPS + warp; i < p.n; i += (int64_t)gridDim.x * RT_WARPS) {
+  const int64_t step = (int64_t)gridDim.x * RT_WARPS * PER;
+  for (int64_t i0 = ((int64_t)blockIdx.x * RT_WARPS + warp) * PER; i0 < p.n; i0 += step) {
+    const int64_t mine = i0 + lane / L;
+    const bool live = mine < p.n;
+    const int64_t i = live ? mine : p.n - 1;
     const T* row = (const T*)p.logits + i * p.n_experts;
     T* out = (T*)p.grad_logits + i * p.n_experts;
     int e = -1;
     float g = 0.f, xe = -INFINITY;
-    if (lane < p.k) {
-      e = p.experts[i * p.k + lane];
+    if (sub < p.k) {
+      e = p.experts[i * p.k + sub];
       if (e >= p.n_experts) e = -1;
       if (e >= 0) {
-        g = p.grad_weights[i * p.k + lane] * p.scale;
+        g = p.grad_weights[i * p.k + sub] * p.scale;
         xe = to_float(row[e]);
       }
     }
@@ -393,17 +413,17 @@ route_topk_grad_kernel(const RouteGradParams p) {
     for (int j = 0; j < V; ++j) v[j] = 0.f;
     if (dense) {
       float x[V], top, sum;
-      route_load<T, V>(row, lane, p.n_experts, p.vec, x);
-      softmax_stats<V>(x, top, sum);
+      route_load<T, V>(row, sub, p.n_experts, p.vec, x);
+      softmax_stats<L, V>(x, top, sum);
       const float s = there ? expf(xe - top) / sum : 0.f;
-      const float dot = warp_sum_of(s * g);
+      const float dot = lanes_sum<L>(s * g);
       const float inv = 1.f / sum;
 #pragma unroll
       for (int j = 0; j < V; ++j) v[j] = -(expf(x[j] - top) * inv) * dot;
       d = s * (g - dot);
     } else if (p.renormalize) {
-      const float share = share_of(there, xe, p.sigmoid != 0);
-      const float dot = warp_sum_of(share * g);
+      const float share = share_of<L>(there, xe, p.sigmoid != 0);
+      const float dot = lanes_sum<L>(share * g);
       d = share * (g - dot);
       if (p.sigmoid) d *= 1.f - sigmoid_of(xe);
     } else {
@@ -411,19 +431,16 @@ route_topk_grad_kernel(const RouteGradParams p) {
       d = g * s * (1.f - s);
     }
     constexpr int BYTES = V * (int)sizeof(T);
-    if (p.vec && e0 + V <= p.n_experts) {
-      union { uint4 u4[(BYTES + 15) / 16]; uint2 u2; uint32_t u1; T t[V]; } r;
+    if (!live) {
+    } else if (p.vec && e0 + V <= p.n_experts) {
+      union { uint4 u4[(BYTES + 15) / 16]; uint2 u2; T t[V]; } r;
 #pragma unroll
       for (int j = 0; j < V; ++j) r.t[j] = from_float<T>(v[j]);
       if constexpr (BYTES >= 16) {
 #pragma unroll
         for (int j = 0; j < BYTES / 16; ++j) reinterpret_cast<uint4*>(out + e0)[j] = r.u4[j];
-      } else if constexpr (BYTES == 8) {
-        *reinterpret_cast<uint2*>(out + e0) = r.u2;
-      } else if constexpr (BYTES == 4) {
-        *reinterpret_cast<uint32_t*>(out + e0) = r.u1;
       } else {
-        out[e0] = r.t[0];
+        *reinterpret_cast<uint2*>(out + e0) = r.u2;
       }
     } else {
 #pragma unroll
@@ -431,7 +448,7 @@ route_topk_grad_kernel(const RouteGradParams p) {
         if (e0 + j < p.n_experts) out[e0 + j] = from_float<T>(v[j]);
     }
     __syncwarp();
-    if (there) out[e] = from_float<T>(d);
+    if (there && live) out[e] = from_float<T>(d);
     __syncwarp();
   }
 }
@@ -442,28 +459,31 @@ bool route_rows_are_vec(const void* a, const void* b, int n_experts, int v) {
   return (((uintptr_t)a | (uintptr_t)b) % bytes) == 0 && (n_experts * (int64_t)sizeof(T)) % bytes == 0;
 }
 
-#define KMB_ROUTE_WIDTHS(RUN)                                                                   \
+// Lanes and experts per lane: eight experts in registers, and as few lanes as hold the token's experts
+// and its choices, so that a reduction serves several tokens.
+#define KMB_ROUTE_WIDTHS(wide, RUN)                                                             \
   do {                                                                                          \
-    if (p.n_experts <= 32) { RUN(1); }                                                          \
-    else if (p.n_experts <= 64) { RUN(2); }                                                     \
-    else if (p.n_experts <= 128) { RUN(4); }                                                    \
-    else if (p.n_experts <= 256) { RUN(8); }                                                    \
-    else if (p.n_experts <= 512) { RUN(16); }                                                   \
-    else { RUN(32); }                                                                           \
+    if (!(wide) && p.n_experts <= 32 && p.k <= 8) { RUN(8, 4); }                                \
+    else if (!(wide) && p.n_experts <= 64 && p.k <= 8) { RUN(8, 8); }                           \
+    else if (!(wide) && p.n_experts <= 128 && p.k <= 16) { RUN(16, 8); }                        \
+    else if (p.n_experts <= 128) { RUN(32, 4); }                                                \
+    else if (p.n_experts <= 256) { RUN(32, 8); }                                                \
+    else if (p.n_experts <= 512) { RUN(32, 16); }                                               \
+    else { RUN(32, 32); }                                                                       \
   } while (0)
 
-static unsigned route_grid(int64_t n) {
-  const int64_t blocks = ceil_div(n, RT_WARPS), cap = (int64_t)sm_count() * 16;
+static unsigned route_grid(int64_t n, int lanes) {
+  const int64_t blocks = ceil_div(n, RT_WARPS * (32 / lanes)), cap = (int64_t)sm_count() * 16;
   return (unsigned)(blocks < cap ? blocks : cap);
 }
 
 template <typename T>
 int route_run(RouteParams p, cudaStream_t s) {
   const size_t smem = p.groups > 1 ? (size_t)RT_WARPS * 2 * p.n_experts * sizeof(float) : 0;
-#define KMB_RUN(V)                                                                              \
+#define KMB_RUN(L, V)                                                                           \
   p.vec = route_rows_are_vec<T>(p.logits, nullptr, p.n_experts, V);                             \
-  route_topk_kernel<T, V><<<route_grid(p.n), RT_WARPS * 32, smem, s>>>(p)
-  KMB_ROUTE_WIDTHS(KMB_RUN);
+  route_topk_kernel<T, L, V><<<route_grid(p.n, L), RT_WARPS * 32, smem, s>>>(p)
+  KMB_ROUTE_WIDTHS(p.groups > 1, KMB_RUN);
 #undef KMB_RUN
   KMB_CHECK_LAUNCH();
   return KMB_OK;
@@ -471,10 +491,10 @@ int route_run(RouteParams p, cudaStream_t s) {
 
 template <typename T>
 int route_grad_run(RouteGradParams p, cudaStream_t s) {
-#define KMB_RUN(V)                                                                              \
+#define KMB_RUN(L, V)                                                                           \
   p.vec = route_rows_are_vec<T>(p.logits, p.grad_logits, p.n_experts, V);                       \
-  route_topk_grad_kernel<T, V><<<route_grid(p.n), RT_WARPS * 32, 0, s>>>(p)
-  KMB_ROUTE_WIDTHS(KMB_RUN);
+  route_topk_grad_kernel<T, L, V><<<route_grid(p.n, L), RT_WARPS * 32, 0, s>>>(p)
+  KMB_ROUTE_WIDTHS(false, KMB_RUN);
 #undef KMB_RUN
   KMB_CHECK_LAUNCH();
   return KMB_OK;
@@ -482,9 +502,10 @@ int route_grad_run(RouteGradParams p, cudaStream_t s) {
 
 // ============================================================================= expert order
 // A stable counting sort of the choices by expert.  A block takes SL_CHUNK consecutive choices, a warp
-// of it SL_ROUNDS * 32 of them; match_any ranks the equal experts of 32 choices, the warp's own
-// counters carry the rank from round to round, and the counters of the warps before it, the chunks
-// before it and the experts before it make the place.
+// of it SL_ROUNDS * 32 of them; one ballot for each bit of the expert finds the equal ones of 32 choices
+// (match_any, which walks the distinct values, took twice as long), the warp's own counters carry the
+// rank from round to round, and the counters of the warps before it, the chunks before it and the
+// experts before it make the place.
 constexpr int SL_WARPS = 16, SL_ROUNDS = 8;
 constexpr int SL_THREADS = SL_WARPS * 32;
 constexpr int SL_CHUNK = SL_THREADS * SL_ROUNDS;
@@ -552,14 +573,20 @@ slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, in
     e_r[r] = e >= 0 && e < n_experts ? e : -1;
   }
   uint16_t* mine = s_warp + warp * n_experts;
+  const int bits = 32 - __clz(n_experts - 1);      // of an expert's number
   for (int e = lane; e < n_experts; e += 32) mine[e] = 0;
   __syncwarp();
   uint32_t rank[SL_ROUNDS];
 #pragma unroll
   for (int r = 0; r < SL_ROUNDS; ++r) {
-    const unsigned same = __match_any_sync(FULL, e_r[r]);
-    const int before = __popc(same & ((1u << lane) - 1u));
     const bool valid = e_r[r] >= 0;
+    unsigned same = __ballot_sync(FULL, valid);
+    for (int b = 0; b < bits; ++b) {
+      const bool one = (e_r[r] >> b) & 1;
+      const unsigned m = __ballot_sync(FULL, one);
+      same &= one ? m : ~m;
+    }
+    const int before = __popc(same & ((1u << lane) - 1u));
     const uint32_t seen = valid ? mine[e_r[r]] : 0u;
     rank[r] = seen + before;
     __syncwarp();
@@ -627,25 +654,81 @@ slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, in
 constexpr int CB_THREADS = 128;
 constexpr int CB_K = 8;        // rows in flight per thread
 
-template <typename T>
+// Eight elements of a row as they lie in memory.  VEC: consecutive ones of a row of whole 16-byte pieces
+// (eight floats are two of them, the second of which may lie behind the row); else one in CB_THREADS,
+// so that neighbouring threads read neighbouring elements of a row that starts anywhere.
+template <typename T, bool VEC>
+struct RowPiece {
+  alignas(16) T t[8];
+  static constexpr int SPAN = CB_THREADS * 8;          // elements of a block's pass
+  static constexpr int PER_QUAD = 16 / (int)sizeof(T), QUADS = 8 / PER_QUAD;
+  __device__ __forceinline__ static int at(int f0, int j) {
+    return VEC ? f0 + threadIdx.x * 8 + j : f0 + threadIdx.x + j * CB_THREADS;
+  }
+  __device__ __forceinline__ void load(const T* __restrict__ row, int f0, int d) {
+    if constexpr (VEC) {
+      uint4* dst = reinterpret_cast<uint4*>(t);
+#pragma unroll
+      for (int q = 0; q < QUADS; ++q)
+        if (at(f0, q * PER_QUAD) < d) dst[q] = *reinterpret_cast<const uint4*>(row + at(f0, q * PER_QUAD));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (at(f0, j) < d) t[j] = row[at(f0, j)];
+    }
+  }
+  __device__ __forceinline__ void store(T* __restrict__ row, int f0, int d) const {
+    if constexpr (VEC) {
+      const uint4* src = reinterpret_cast<const uint4*>(t);
+#pragma unroll
+      for (int q = 0; q < QUADS; ++q)
+        if (at(f0, q * PER_QUAD) < d) *reinterpret_cast<uint4*>(row + at(f0, q * PER_QUAD)) = src[q];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (at(f0, j) < d) row[at(f0, j)] = t[j];
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = from_float<T>(0.f);
+  }
+};
+
+// Bound by HBM: each thread has the pieces of up to CB_K rows in flight before it adds the first.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(CB_THREADS)
 combine_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __restrict__ slots,
-               const float* __restrict__ weights, int k, int d, T* __restrict__ out, int vec) {
+               const float* __restrict__ weights, int k, int d, T* __restrict__ out) {
+  typedef RowPiece<T, VEC> Piece;
   const int64_t t = blockIdx.x;
-  for (int f = (blockIdx.y * CB_THREADS + threadIdx.x) * 8; f < d; f += gridDim.y * CB_THREADS * 8) {
+  for (int f0 = blockIdx.y * Piece::SPAN; f0 < d; f0 += gridDim.y * Piece::SPAN) {
+    if (VEC && Piece::at(f0, 0) >= d) continue;
     float acc[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    for (int j = 0; j < k; ++j) {
-      const int slot = slots[t * k + j];
-      if (slot < 0 || slot >= n_values) continue;
-      const float w = weights[t * k + j];
-      float v[8];
-      load_vec8(values + (int64_t)slot * d, f, d, vec != 0, v);
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    for (int j0 = 0; j0 < k; j0 += CB_K) {
+      Piece v[CB_K];
+      float w[CB_K];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+      for (int j = 0; j < CB_K; ++j) {
+        const int slot = j0 + j < k ? slots[t * k + j0 + j] : -1;
+        w[j] = 0.f;
+        v[j].clear();
+        if (slot >= 0 && slot < n_values) {
+          w[j] = weights[t * k + j0 + j];
+          v[j].load(values + (int64_t)slot * d, f0, d);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < CB_K; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], to_float(v[j].t[i]), acc[i]);
     }
-    store_vec8(out + t * d, f, d, vec != 0, acc);
+    Piece o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.t[i] = from_float<T>(acc[i]);
+    o.store(out + t * d, f0, d);
   }
 }
 
@@ -662,12 +745,13 @@ __global__ void combine_users_kernel(const int32_t* __restrict__ slots, int64_t 
   atomicMin(&first[slot], (int32_t)c);
 }
 
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(CB_THREADS)
 combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __restrict__ slots,
                     const float* __restrict__ weights, const T* __restrict__ grad_out, int64_t n, int k, int d,
                     const int32_t* __restrict__ users, const int32_t* __restrict__ first,
-                    T* __restrict__ grad_values, float* __restrict__ grad_weights, int vec) {
+                    T* __restrict__ grad_values, float* __restrict__ grad_weights) {
+  typedef RowPiece<T, VEC> Piece;
   __shared__ float red[CB_THREADS / 32][CB_K];
   __shared__ int32_t list[CB_THREADS];
   __shared__ int list_n[CB_THREADS / 32];
@@ -675,38 +759,54 @@ combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_
   if ((int64_t)blockIdx.x >= n) {
     // the blocks behind the tokens': zeros for the rows that nobody chose
     const int64_t step = (int64_t)gridDim.x - n;
+    Piece z;
+    z.clear();
     for (int64_t r = (int64_t)blockIdx.x - n; r < n_values; r += step) {
       if (users[r] != 0) continue;
-      float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int f = threadIdx.x * 8; f < d; f += CB_THREADS * 8) store_vec8(grad_values + r * d, f, d, vec != 0, z);
+      for (int f0 = 0; f0 < d; f0 += Piece::SPAN)
+        if (!VEC || Piece::at(f0, 0) < d) z.store(grad_values + r * d, f0, d);
     }
     return;
   }
   const int64_t t = blockIdx.x;
   const T* g_row = grad_out + t * d;
+  bool shared = false;
   for (int j0 = 0; j0 < k; j0 += CB_K) {
-    float dot[CB_K];
+    int slot[CB_K];
+    float w[CB_K], dot[CB_K];
+    unsigned alone = 0;         // bit j: nobody else uses the row
 #pragma unroll
-    for (int j = 0; j < CB_K; ++j) dot[j] = 0.f;
-    for (int f = threadIdx.x * 8; f < d; f += CB_THREADS * 8) {
-      float g[8];
-      load_vec8(g_row, f, d, vec != 0, g);
+    for (int j = 0; j < CB_K; ++j) {
+      slot[j] = j0 + j < k ? slots[t * k + j0 + j] : -1;
+      if (slot[j] >= n_values) slot[j] = -1;
+      w[j] = slot[j] >= 0 ? weights[t * k + j0 + j] : 0.f;
+      dot[j] = 0.f;
+      if (slot[j] >= 0) {
+        if (users[slot[j]] == 1) alone |= 1u << j;
+        else shared = true;
+      }
+    }
+    for (int f0 = 0; f0 < d; f0 += Piece::SPAN) {
+      if (VEC && Piece::at(f0, 0) >= d) continue;
+      Piece g, v[CB_K];
+      g.clear();
+      g.load(g_row, f0, d);
 #pragma unroll
       for (int j = 0; j < CB_K; ++j) {
-        if (j0 + j >= k) continue;
-        const int64_t c = t * k + j0 + j;
-        const int slot = slots[c];
-        if (slot < 0 || slot >= n_values) continue;
-        float v[8];
-        load_vec8(values + (int64_t)slot * d, f, d, vec != 0, v);
+        v[j].clear();
+        if (slot[j] >= 0) v[j].load(values + (int64_t)slot[j] * d, f0, d);
+      }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dot[j] = fmaf(v[i], g[i], dot[j]);
-        if (users[slot] == 1) {
-          const float w = weights[c];
+      for (int j = 0; j < CB_K; ++j) {
+        if (slot[j] < 0) continue;
+        Piece o;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = w * g[i];
-          store_vec8(grad_values + (int64_t)slot * d, f, d, vec != 0, v);
+        for (int i = 0; i < 8; ++i) {
+          const float gi = to_float(g.t[i]);
+          dot[j] = fmaf(to_float(v[j].t[i]), gi, dot[j]);
+          o.t[i] = from_float<T>(w[j] * gi);
         }
+        if ((alone >> j) & 1u) o.store(grad_values + (int64_t)slot[j] * d, f0, d);
       }
     }
 #pragma unroll
@@ -718,19 +818,20 @@ combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_
     if (threadIdx.x < CB_K && j0 + threadIdx.x < k) {
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < CB_THREADS / 32; ++w) sum += red[w][threadIdx.x];
+      for (int q = 0; q < CB_THREADS / 32; ++q) sum += red[q][threadIdx.x];
       grad_weights[t * k + j0 + threadIdx.x] = sum;     // 0 where there is no row
     }
     __syncthreads();
   }
+  if (!shared) return;
   // rows with several users: the block of the lowest of them finds the others by walking the choices
   // behind it, CB_THREADS at a time, and adds them up in ascending order
   for (int j = 0; j < k; ++j) {
     const int64_t c0 = t * k + j;
     const int slot = slots[c0];
     if (slot < 0 || slot >= n_values || users[slot] == 1 || first[slot] != c0) continue;
-    for (int fb = 0; fb < d; fb += CB_THREADS * 8) {
-      const int f = fb + threadIdx.x * 8;
+    for (int f0 = 0; f0 < d; f0 += Piece::SPAN) {
+      const bool in = !VEC || Piece::at(f0, 0) < d;
       float acc[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] = 0.f;
@@ -742,25 +843,29 @@ combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_
         if (lane == 0) list_n[warp] = __popc(m);
         __syncthreads();
         int at = 0, found = 0;
-        for (int w = 0; w < CB_THREADS / 32; ++w) {
-          if (w < warp) at += list_n[w];
-          found += list_n[w];
+        for (int q = 0; q < CB_THREADS / 32; ++q) {
+          if (q < warp) at += list_n[q];
+          found += list_n[q];
         }
         if (hit) list[at + __popc(m & ((1u << lane) - 1u))] = (int32_t)(c - cb);
         __syncthreads();
-        if (f < d)
+        if (in)
           for (int q = 0; q < found; ++q) {
             const int64_t cc = cb + list[q];
             const float w = weights[cc];
-            float g[8];
-            load_vec8(grad_out + (cc / k) * d, f, d, vec != 0, g);
+            Piece g;
+            g.clear();
+            g.load(grad_out + (cc / k) * d, f0, d);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, g[i], acc[i]);
+            for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, to_float(g.t[i]), acc[i]);
           }
         left -= found;
         __syncthreads();
       }
-      if (f < d) store_vec8(grad_values + (int64_t)slot * d, f, d, vec != 0, acc);
+      Piece o;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o.t[i] = from_float<T>(acc[i]);
+      if (in) o.store(grad_values + (int64_t)slot * d, f0, d);
     }
   }
 }
@@ -889,8 +994,8 @@ int kmb_combine_experts(int dtype, const void* values, int64_t n_values, const i
     const int vec = rows_are_vec((const T*)values, d) && rows_are_vec((const T*)out, d);
     dim3 grid((unsigned)n, (unsigned)ceil_div(d, CB_THREADS * 8));
     if (grid.y > 65535) grid.y = 65535;
-    combine_kernel<T><<<grid, CB_THREADS, 0, (cudaStream_t)stream>>>((const T*)values, n_values, slots, weights, k,
-                                                                     d, (T*)out, vec);
+    const auto kernel = vec ? combine_kernel<T, true> : combine_kernel<T, false>;
+    kernel<<<grid, CB_THREADS, 0, (cudaStream_t)stream>>>((const T*)values, n_values, slots, weights, k, d, (T*)out);
     KMB_CHECK_LAUNCH();
   });
   return KMB_OK;
@@ -929,9 +1034,9 @@ int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, co
     const int vec = rows_are_vec((const T*)values, d) && rows_are_vec((const T*)grad_out, d) &&
                     rows_are_vec((const T*)grad_values, d);
     const int64_t fill = n_values == 0 ? 0 : (ceil_div(n_values, 64) < sm_count() ? ceil_div(n_values, 64) : sm_count());
-    combine_grad_kernel<T><<<(unsigned)(n + fill), CB_THREADS, 0, s>>>(
-        (const T*)values, n_values, slots, weights, (const T*)grad_out, n, k, d, users, first, (T*)grad_values,
-        grad_weights, vec);
+    const auto kernel = vec ? combine_grad_kernel<T, true> : combine_grad_kernel<T, false>;
+    kernel<<<(unsigned)(n + fill), CB_THREADS, 0, s>>>((const T*)values, n_values, slots, weights, (const T*)grad_out,
+                                                       n, k, d, users, first, (T*)grad_values, grad_weights);
     KMB_CHECK_LAUNCH();
   });
   return KMB_OK;

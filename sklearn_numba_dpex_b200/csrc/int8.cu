@@ -20,27 +20,71 @@
 namespace kmb {
 
 // =============================================================================== quantisation
-// One block per row.  The row stays in registers between the maximum and the rounding when it fits
-// (QR_REGS vectors of eight elements a thread), longer rows are read a second time (from L1 / L2).
-constexpr int QR_VEC = 8;
-
-// round_half_even(127 x / top) as exact arithmetic has it.  r = x * (127 / top) in 32 bits is off by
-// less than 127 * 3 * 2^-24 < 1e-4, so only values that lie closer than that to the middle between
-// two whole numbers are decided by the quotient in 64 bits: 127 x is exact there, and a quotient of
-// such short numbers is never rounded onto a middle that it does not hit.
-__device__ __forceinline__ int quantize_one(float x, float inv, float top) {
-  const float r = x * inv;
-  float n = rintf(r);
-  if (!(fabsf(r - n) < 0.4999f)) n = (float)rint((double)x * 127.0 / (double)top);
-  return (int)n;
+// THREADS threads per row, ROWS rows per block.  A row of up to THREADS * VECS pieces of eight elements
+// stays in registers, as it lies in memory, between the maximum and the rounding; longer rows (VECS =
+// 0) are read a second time, from L1 and L2.
+__device__ __noinline__ uint32_t quantize_exactly(float x, float top) {
+  return (uint32_t)(int)rint((double)x * 127.0 / (double)top);
 }
 
-template <typename T, int THREADS, int REGS>
-__global__ void __launch_bounds__(THREADS)
-quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* __restrict__ rows,
+template <typename T>
+struct QrPiece {
+  alignas(16) T t[8];
+  __device__ __forceinline__ void load(const T* __restrict__ row, int f, int d, bool vec) {
+    if (vec) {       // rows of whole 16-byte pieces; a piece of eight floats may end behind the row
+      uint4* dst = reinterpret_cast<uint4*>(t);
+#pragma unroll
+      for (int q = 0; q < (int)sizeof(T) / 2; ++q)
+        dst[q] = f + q * (16 / (int)sizeof(T)) < d ? *reinterpret_cast<const uint4*>(row + f + q * (16 / (int)sizeof(T)))
+                                                   : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = f + j < d ? row[f + j] : from_float<T>(0.f);
+    }
+  }
+  // bits of the greatest |x|: whole numbers in the order of the values, NaN above infinity
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(to_float(t[j])) & 0x7fffffffu);
+    return m;
+  }
+  // The eight 8-bit numbers.  r = x * (127 / top) in 32 bits is off by less than 127 * 3 * 2^-24 < 1e-4, so
+  // round_half_even(127 x / top) as exact arithmetic has it is r's own rounding unless r lies closer than
+  // that to the middle between two whole numbers; then the quotient in 64 bits decides (127 x is exact
+  // there, and a quotient of such short numbers is never rounded onto a middle that it does not hit).
+  // Adding 1.5 * 2^23 rounds to a whole number whose low byte is the result.
+  __device__ __forceinline__ uint2 round(float inv, float topf) const {
+    const float magic = 12582912.f;
+    uint32_t n[8];
+    float off = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float r = to_float(t[j]) * inv;
+      const float s = r + magic;
+      n[j] = __float_as_uint(s);
+      off = fmaxf(off, fabsf(r - (s - magic)));
+    }
+    if (!(off < 0.4999f && inv < 1e30f)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) n[j] = quantize_exactly(to_float(t[j]), topf);
+    }
+    uint2 p;
+    p.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+    p.y = __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410);
+    return p;
+  }
+};
+
+template <typename T, int THREADS, int ROWS, int VECS>
+__global__ void __launch_bounds__(THREADS * ROWS)
+quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* __restrict__ rows, int64_t m,
                      int8_t* __restrict__ q, int64_t q_pitch, float* __restrict__ scales, int vec) {
+  static_assert(ROWS == 1 || THREADS == 32, "several rows of a block take a warp each");
   __shared__ uint32_t red[THREADS / 32];
-  const int64_t i = blockIdx.x;
+  const int tid = threadIdx.x % THREADS;
+  const int64_t i = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
+  if (ROWS > 1 && i >= m) return;
   int64_t src = i;
   if (rows) {
     src = rows[i];
@@ -48,24 +92,20 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* _
   }
   int8_t* qi = q + i * q_pitch;
   const T* xi = x + (src < 0 ? 0 : src) * d;
-  float v[REGS][QR_VEC];
-  uint32_t top = 0;   // bits of |x|: whole numbers in the order of the values, NaN above infinity
-  for (int r = 0, f = threadIdx.x * QR_VEC; f < d; ++r, f += THREADS * QR_VEC) {
-    float w[QR_VEC];
-    if (src < 0) {
+  const int end = src < 0 ? 0 : d;       // a row that is not there is a row of zeros
+  constexpr int HELD = VECS > 0 ? VECS : 1;
+  QrPiece<T> v[HELD];
+  uint32_t top = 0;
+  if (VECS > 0) {
 #pragma unroll
-      for (int j = 0; j < QR_VEC; ++j) w[j] = 0.f;
-    } else {
-      load_vec8(xi, f, d, vec != 0, w);
+    for (int r = 0; r < HELD; ++r) v[r].load(xi, (r * THREADS + tid) * 8, end, vec != 0);
+#pragma unroll
+    for (int r = 0; r < HELD; ++r) top = max(top, v[r].top());
+  } else {
+    for (int f = tid * 8; f < end; f += THREADS * 8) {
+      v[0].load(xi, f, end, vec != 0);
+      top = max(top, v[0].top());
     }
-#pragma unroll
-    for (int j = 0; j < QR_VEC; ++j) top = max(top, __float_as_uint(w[j]) & 0x7fffffffu);
-#pragma unroll
-    for (int rr = 0; rr < REGS; ++rr)
-      if (r == rr) {
-#pragma unroll
-        for (int j = 0; j < QR_VEC; ++j) v[rr][j] = w[j];
-      }
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if (THREADS > 32) {
@@ -78,35 +118,21 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* _
   const float topf = __uint_as_float(top);
   // a row that holds an infinity or NaN has no 8-bit image: NaN as its scale makes its products NaN
   const bool bad = top >= 0x7f800000u;
-  if (threadIdx.x == 0) scales[i] = bad ? __uint_as_float(0x7fffffffu) : topf / 127.f;
+  if (tid == 0) scales[i] = bad ? __uint_as_float(0x7fffffffu) : topf / 127.f;
   const bool zero = bad || top == 0u;
-  const float inv = 127.f / topf;   // infinite below 4e-37: quantize_one then takes the 64-bit quotient
-  for (int r = 0, f = threadIdx.x * QR_VEC; f < d; ++r, f += THREADS * QR_VEC) {
-    float w[QR_VEC];
-    bool kept = false;
+  const float inv = 127.f / topf;
+  // the pitch is a multiple of 16, so the eight bytes of a piece lie inside the row's own storage
+  if (VECS > 0) {
 #pragma unroll
-    for (int rr = 0; rr < REGS; ++rr)
-      if (r == rr) {
-        kept = true;
-#pragma unroll
-        for (int j = 0; j < QR_VEC; ++j) w[j] = v[rr][j];
-      }
-    if (!kept) {
-      if (zero) {
-#pragma unroll
-        for (int j = 0; j < QR_VEC; ++j) w[j] = 0.f;
-      } else {
-        load_vec8(xi, f, d, vec != 0, w);
-      }
+    for (int r = 0; r < HELD; ++r) {
+      const int f = (r * THREADS + tid) * 8;
+      if (f < d) *reinterpret_cast<uint2*>(qi + f) = zero ? make_uint2(0u, 0u) : v[r].round(inv, topf);
     }
-    uint32_t p[2] = {0u, 0u};
-    if (!zero) {
-#pragma unroll
-      for (int j = 0; j < QR_VEC; ++j)
-        p[j >> 2] |= ((uint32_t)quantize_one(w[j], inv, topf) & 0xffu) << (8 * (j & 3));
+  } else {
+    for (int f = tid * 8; f < d; f += THREADS * 8) {
+      if (!zero) v[0].load(xi, f, end, vec != 0);
+      *reinterpret_cast<uint2*>(qi + f) = zero ? make_uint2(0u, 0u) : v[0].round(inv, topf);
     }
-    // the pitch is a multiple of 16, so the eight bytes lie inside the row's own storage
-    *reinterpret_cast<uint2*>(qi + f) = make_uint2(p[0], p[1]);
   }
 }
 
@@ -114,13 +140,18 @@ template <typename T>
 int quantize_run(const T* x, int64_t n, int d, const int32_t* rows, int64_t m, int8_t* q,
                  int64_t q_pitch, float* scales, cudaStream_t s) {
   const int vec = rows_are_vec(x, d) ? 1 : 0;
-  const unsigned grid = (unsigned)m;
-  if (d <= 32 * QR_VEC * 2)
-    quantize_rows_kernel<T, 32, 2><<<grid, 32, 0, s>>>(x, n, d, rows, q, q_pitch, scales, vec);
-  else if (d <= 128 * QR_VEC * 2)
-    quantize_rows_kernel<T, 128, 2><<<grid, 128, 0, s>>>(x, n, d, rows, q, q_pitch, scales, vec);
-  else
-    quantize_rows_kernel<T, 256, 4><<<grid, 256, 0, s>>>(x, n, d, rows, q, q_pitch, scales, vec);
+  const unsigned one = (unsigned)m, four = (unsigned)ceil_div(m, 4);
+#define KMB_RUN(THREADS, ROWS, VECS)                                                            \
+  quantize_rows_kernel<T, THREADS, ROWS, VECS>                                                  \
+      <<<ROWS == 1 ? one : four, THREADS * ROWS, 0, s>>>(x, n, d, rows, m, q, q_pitch, scales, vec)
+  if (d <= 256) KMB_RUN(32, 4, 1);
+  else if (d <= 512) KMB_RUN(32, 4, 2);
+  else if (d <= 1024) KMB_RUN(128, 1, 1);
+  else if (d <= 2048) KMB_RUN(128, 1, 2);
+  else if (d <= 4096) KMB_RUN(256, 1, 2);
+  else if (d <= 8192) KMB_RUN(256, 1, 4);
+  else KMB_RUN(256, 1, 0);
+#undef KMB_RUN
   KMB_CHECK_LAUNCH();
   return KMB_OK;
 }

@@ -305,7 +305,8 @@ def ref_combine(values, slots, weights, grad):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,k,d,m", [(1, 1, 1, 1), (1, 8, 4096, 8), (3, 2, 7, 9), (5, 8, 1031, 40), (17, 9, 64, 153), (33, 20, 129, 700),
-                                     (9, 3, 8200, 27), (4, 2, 16, 0), (0, 2, 16, 5)])
+                                     (9, 3, 8200, 27), (4, 2, 16, 0), (0, 2, 16, 5), (40, 3, 100, 130),
+                                     (40, 2, 12, 90), (6, 2, 1028, 13)])
 @pytest.mark.parametrize("repeated", [False, True])
 def test_combine(dtype, n, k, d, m, repeated):
     """Every sum of N products is off by N u of the sum of their magnitudes at most."""
