@@ -105,7 +105,7 @@ struct Chosen {
 // each, the quotient, the bias's addition.  (V + 16) 2^-24 of the largest score and key covers both
 // keys of a pair.  A token with such a pair (about one in a hundred) is done again in 64 bits, which
 // is what the definition says.  Equal logits with equal biases have equal keys and need no second look.
-template <typename K, int L, int V, typename T>
+template <typename K, int L, int V, bool PLAIN, typename T>
 __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row, const float (&x)[V], int lane,
                                               bool by_logit, float* s_keys) {
   typedef typename OrderBits<K>::type B;
@@ -114,7 +114,7 @@ __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row
   const K ninf = -(K)INFINITY;
   K key[V];
   K margin = 0;
-  if (by_logit) {
+  if (PLAIN || by_logit) {
 #pragma unroll
     for (int i = 0; i < V; ++i) key[i] = (K)x[i];
   } else {
@@ -160,7 +160,7 @@ __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row
   }
   bool unsure = false;
 
-  if (L == 32 && p.groups > 1) {
+  if (!PLAIN && L == 32 && p.groups > 1) {
     // lane g works out the score of group g from the keys in shared memory
     K* keys = reinterpret_cast<K*>(s_keys);
     __syncwarp();
@@ -221,7 +221,7 @@ __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row
   Chosen c = {-1, false};
   B mine = 0, next = 0;
   int next_e = -1;
-  const bool check = narrow && p.bias != nullptr;
+  const bool check = !PLAIN && narrow && p.bias != nullptr;
   const int rounds = check ? p.k + 1 : p.k;      // the first that is left out counts too
   for (int j = 0; j < rounds; ++j) {
     B best = bits[0];
@@ -286,7 +286,7 @@ template <typename T, int L, int V>
 __device__ __noinline__ int route_again(const RouteParams& p, const T* row, int lane, float* s_keys) {
   float x[V];
   route_load<T, V>(row, lane & (L - 1), p.n_experts, p.vec, x);
-  return route_token<double, L, V>(p, row, x, lane, false, s_keys).expert;
+  return route_token<double, L, V, false>(p, row, x, lane, false, s_keys).expert;
 }
 
 __device__ __forceinline__ float sigmoid_of(float x) {
@@ -326,7 +326,8 @@ __device__ __forceinline__ void softmax_stats(const float (&x)[V], float& top, f
   if (sum == 0.f) sum = 1.f;
 }
 
-template <typename T, int L, int V>
+// PLAIN: experts ordered by their logits, no groups: nothing is left of the keys, and half the registers.
+template <typename T, int L, int V, bool PLAIN>
 __global__ void __launch_bounds__(RT_WARPS * 32)
 route_topk_kernel(const __grid_constant__ RouteParams p) {
   // groups: one row of keys per warp, wide enough for 64-bit keys
@@ -334,7 +335,7 @@ route_topk_kernel(const __grid_constant__ RouteParams p) {
   constexpr int PER = 32 / L;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (L - 1);
   float* s_keys = s_route + (size_t)warp * 2 * p.n_experts;
-  const bool by_logit = p.bias == nullptr && (p.groups == 1 || p.group_best == 1);
+  const bool by_logit = PLAIN || (p.bias == nullptr && (p.groups == 1 || p.group_best == 1));
   const int64_t step = (int64_t)gridDim.x * RT_WARPS * PER;
   for (int64_t i0 = ((int64_t)blockIdx.x * RT_WARPS + warp) * PER; i0 < p.n; i0 += step) {
     const int64_t mine = i0 + lane / L;
@@ -342,8 +343,8 @@ route_topk_kernel(const __grid_constant__ RouteParams p) {
     const T* row = (const T*)p.logits + i * p.n_experts;
     float x[V];
     route_load<T, V>(row, sub, p.n_experts, p.vec, x);
-    Chosen c = route_token<float, L, V>(p, row, x, lane, by_logit, s_keys);
-    if (!by_logit && __any_sync(FULL, c.unsure)) {
+    Chosen c = route_token<float, L, V, PLAIN>(p, row, x, lane, by_logit, s_keys);
+    if (!PLAIN && !by_logit && __any_sync(FULL, c.unsure)) {
       const int e = route_again<T, L, V>(p, row, lane, s_keys);
       if (c.unsure) c.expert = e;
     }
@@ -482,7 +483,10 @@ int route_run(RouteParams p, cudaStream_t s) {
   const size_t smem = p.groups > 1 ? (size_t)RT_WARPS * 2 * p.n_experts * sizeof(float) : 0;
 #define KMB_RUN(L, V)                                                                           \
   p.vec = route_rows_are_vec<T>(p.logits, nullptr, p.n_experts, V);                             \
-  route_topk_kernel<T, L, V><<<route_grid(p.n, L), RT_WARPS * 32, smem, s>>>(p)
+  if (p.bias == nullptr && p.groups == 1)                                                       \
+    route_topk_kernel<T, L, V, true><<<route_grid(p.n, L), RT_WARPS * 32, 0, s>>>(p);           \
+  else                                                                                          \
+    route_topk_kernel<T, L, V, false><<<route_grid(p.n, L), RT_WARPS * 32, smem, s>>>(p)
   KMB_ROUTE_WIDTHS(p.groups > 1, KMB_RUN);
 #undef KMB_RUN
   KMB_CHECK_LAUNCH();
@@ -530,25 +534,48 @@ slots_count_kernel(const int32_t* __restrict__ experts, int64_t total, int n_exp
     counts[(int64_t)blockIdx.x * n_experts + e] = s_cnt[e];
 }
 
-// counts[chunk][e] -> choices of expert e in the chunks before; totals[e].  One warp per expert.
-__global__ void __launch_bounds__(256)
+// counts[chunk][e] -> choices of expert e in the chunks before; totals[e].  A block takes 32 experts; each
+// of its 32 warps sums (and then rewrites) a run of SC_RUN chunks, its lanes one expert each.
+constexpr int SC_RUN = 8;
+__global__ void __launch_bounds__(1024)
 slots_scan_kernel(int32_t* __restrict__ counts, int chunks, int n_experts, int32_t* __restrict__ totals) {
-  const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (e >= n_experts) return;
-  int base = 0;
-  for (int c0 = 0; c0 < chunks; c0 += 32) {
-    const int c = c0 + lane;
-    const int v = c < chunks ? counts[(int64_t)c * n_experts + e] : 0;
-    int inc = v;
+  __shared__ int32_t s_sum[32][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = blockIdx.x * 32 + lane;
+  const bool mine = e < n_experts;
+  int carry = 0;
+  for (int c0 = 0; c0 < chunks; c0 += 32 * SC_RUN) {
+    int v[SC_RUN], sum = 0;
+#pragma unroll
+    for (int r = 0; r < SC_RUN; ++r) {
+      const int c = c0 + warp * SC_RUN + r;
+      v[r] = mine && c < chunks ? counts[(int64_t)c * n_experts + e] : 0;
+    }
+#pragma unroll
+    for (int r = 0; r < SC_RUN; ++r) sum += v[r];
+    s_sum[warp][lane] = sum;
+    __syncthreads();
+    // warp w scans the 32 runs of expert w of the block
+    const int x = s_sum[lane][warp];
+    int inc = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(FULL, inc, o);
       if (lane >= o) inc += u;
     }
-    if (c < chunks) counts[(int64_t)c * n_experts + e] = base + inc - v;
-    base += __shfl_sync(FULL, inc, 31);
+    __syncthreads();
+    s_sum[lane][warp] = inc;
+    __syncthreads();
+    int base = carry + s_sum[warp][lane] - sum;
+    carry += s_sum[31][lane];
+#pragma unroll
+    for (int r = 0; r < SC_RUN; ++r) {
+      const int c = c0 + warp * SC_RUN + r;
+      if (mine && c < chunks) counts[(int64_t)c * n_experts + e] = base;
+      base += v[r];
+    }
+    __syncthreads();
   }
-  if (lane == 0) totals[e] = base;
+  if (warp == 0 && mine) totals[e] = carry;
 }
 
 // ONE: a single chunk, whose counts are the totals.
@@ -559,8 +586,12 @@ slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, in
                    int32_t* __restrict__ slots, int32_t* __restrict__ rows, int32_t* __restrict__ offsets) {
   extern __shared__ int32_t s_dyn[];
   int32_t* s_base = s_dyn;                            // first place of each expert in this chunk
-  uint16_t* s_warp = (uint16_t*)(s_dyn + n_experts);  // [SL_WARPS][n_experts] choices in the warp
-  __shared__ int32_t s_scan[SL_WARPS];
+  int32_t* s_local = s_dyn + n_experts;               // and among the chunk's own choices
+  uint16_t* s_warp = (uint16_t*)(s_dyn + 2 * n_experts);  // [SL_WARPS][n_experts] choices in the warp
+  // the chunk's choices in expert order: (place, row), so that the rows of an expert leave side by side
+  __shared__ int2 s_out[SL_CHUNK];
+  __shared__ int32_t s_count;
+  __shared__ int2 s_scan[SL_WARPS];
   __shared__ int32_t s_end;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t first = (int64_t)blockIdx.x * SL_CHUNK + warp * (SL_ROUNDS * 32);
@@ -573,7 +604,6 @@ slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, in
     e_r[r] = e >= 0 && e < n_experts ? e : -1;
   }
   uint16_t* mine = s_warp + warp * n_experts;
-  const int bits = 32 - __clz(n_experts - 1);      // of an expert's number
   for (int e = lane; e < n_experts; e += 32) mine[e] = 0;
   __syncwarp();
   uint32_t rank[SL_ROUNDS];
@@ -581,7 +611,9 @@ slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, in
   for (int r = 0; r < SL_ROUNDS; ++r) {
     const bool valid = e_r[r] >= 0;
     unsigned same = __ballot_sync(FULL, valid);
-    for (int b = 0; b < bits; ++b) {
+#pragma unroll
+    for (int b = 0; b < 10; ++b) {
+      if (b == 8 && n_experts <= 256) break;       // no expert has these bits
       const bool one = (e_r[r] >> b) & 1;
       const unsigned m = __ballot_sync(FULL, one);
       same &= one ? m : ~m;
@@ -595,7 +627,7 @@ slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, in
   }
   __syncthreads();
   // warps' counts -> choices in the warps before; then the experts' first places
-  int carry = 0;
+  int carry = 0, carry_local = 0;
   for (int e0 = 0; e0 < n_experts; e0 += SL_THREADS) {
     const int e = e0 + threadIdx.x;
     int in_chunk = 0;
@@ -608,29 +640,40 @@ slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, in
       }
     }
     const int tot = e < n_experts ? (ONE ? in_chunk : totals[e]) : 0;
-    int inc = tot;
+    const int before = e < n_experts && !ONE ? counts[(int64_t)blockIdx.x * n_experts + e] : 0;
+    int inc = tot, inc_local = in_chunk;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(FULL, inc, o);
-      if (lane >= o) inc += u;
+      const int u = __shfl_up_sync(FULL, inc, o), ul = __shfl_up_sync(FULL, inc_local, o);
+      if (lane >= o) {
+        inc += u;
+        inc_local += ul;
+      }
     }
-    if (lane == 31) s_scan[warp] = inc;
+    if (lane == 31) s_scan[warp] = make_int2(inc, inc_local);
     __syncthreads();
-    int base = carry, all = carry;
+    int base = carry, base_local = carry_local;
+#pragma unroll
     for (int w = 0; w < SL_WARPS; ++w) {
-      if (w < warp) base += s_scan[w];
-      all += s_scan[w];
+      const int2 v = s_scan[w];
+      if (w < warp) {
+        base += v.x;
+        base_local += v.y;
+      }
+      carry += v.x;
+      carry_local += v.y;
     }
     if (e < n_experts) {
       const int start = base + inc - tot;
-      s_base[e] = start + (ONE ? 0 : counts[(int64_t)blockIdx.x * n_experts + e]);
+      s_base[e] = start + before;
+      s_local[e] = base_local + inc_local - in_chunk;
       if (blockIdx.x == 0) offsets[e] = start;
     }
-    carry = all;
     __syncthreads();
   }
   if (threadIdx.x == 0) {
     s_end = carry;
+    s_count = carry_local;
     if (blockIdx.x == 0) offsets[n_experts] = carry;
   }
   __syncthreads();
@@ -641,29 +684,33 @@ slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, in
     const int e = e_r[r];
     int place = -1;
     if (e >= 0) {
-      place = s_base[e] + mine[e] + (int)rank[r];
-      rows[place] = (int32_t)(c / k);
+      const int in_chunk = mine[e] + (int)rank[r];
+      place = s_base[e] + in_chunk;
+      s_out[s_local[e] + in_chunk] = make_int2(place, (int32_t)((uint32_t)c / (uint32_t)k));
     }
     slots[c] = place;
     if (c >= s_end) rows[c] = -1;      // places behind the last chosen row
   }
+  __syncthreads();
+  for (int i = threadIdx.x; i < s_count; i += SL_THREADS) rows[s_out[i].x] = s_out[i].y;
 }
 
 // ============================================================================= weighted sums
 // out[t] = sum_j w[t, j] values[slots[t, j]]; a slot outside [0, n_values) counts as none.
-constexpr int CB_THREADS = 128;
-constexpr int CB_K = 8;        // rows in flight per thread
+constexpr int CB_THREADS = 256;   // at most; the launch takes as many as a row needs (combine_threads)
+constexpr int CB_K = 8;           // rows in flight per thread
+constexpr int CG_THREADS = 128, CG_K = 4;   // the gradients', which hold twice as much per row
 
 // Eight elements of a row as they lie in memory.  VEC: consecutive ones of a row of whole 16-byte pieces
-// (eight floats are two of them, the second of which may lie behind the row); else one in CB_THREADS,
-// so that neighbouring threads read neighbouring elements of a row that starts anywhere.
+// (eight floats are two of them, the second of which may lie behind the row); else one in
+// blockDim.x, so that neighbouring threads read neighbouring elements of a row that starts anywhere.
 template <typename T, bool VEC>
 struct RowPiece {
   alignas(16) T t[8];
-  static constexpr int SPAN = CB_THREADS * 8;          // elements of a block's pass
+  __device__ __forceinline__ static int span() { return blockDim.x * 8; }     // elements of a block's pass
   static constexpr int PER_QUAD = 16 / (int)sizeof(T), QUADS = 8 / PER_QUAD;
   __device__ __forceinline__ static int at(int f0, int j) {
-    return VEC ? f0 + threadIdx.x * 8 + j : f0 + threadIdx.x + j * CB_THREADS;
+    return VEC ? f0 + threadIdx.x * 8 + j : f0 + threadIdx.x + j * blockDim.x;
   }
   __device__ __forceinline__ void load(const T* __restrict__ row, int f0, int d) {
     if constexpr (VEC) {
@@ -702,8 +749,8 @@ combine_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __
                const float* __restrict__ weights, int k, int d, T* __restrict__ out) {
   typedef RowPiece<T, VEC> Piece;
   const int64_t t = blockIdx.x;
-  for (int f0 = blockIdx.y * Piece::SPAN; f0 < d; f0 += gridDim.y * Piece::SPAN) {
-    if (VEC && Piece::at(f0, 0) >= d) continue;
+  for (int f0 = blockIdx.y * Piece::span(); f0 < d; f0 += gridDim.y * Piece::span()) {
+    if (Piece::at(f0, 0) >= d) continue;
     float acc[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = 0.f;
@@ -733,8 +780,8 @@ combine_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __
 }
 
 // Gradients.  A row of values that several choices share needs the sum of their gradients, in a fixed
-// order: `users` counts the choices of each row and `first` names the lowest of them, which alone
-// writes the row.  Rows that nobody chose get zeros.
+// order: `users` counts the choices of each row and `first` names the lowest of them.  The blocks of the
+// tokens write the rows with one user, the last blocks of the grid all others.
 __global__ void combine_users_kernel(const int32_t* __restrict__ slots, int64_t total, int64_t n_values,
                                      int32_t* __restrict__ users, int32_t* __restrict__ first) {
   const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -745,105 +792,35 @@ __global__ void combine_users_kernel(const int32_t* __restrict__ slots, int64_t 
   atomicMin(&first[slot], (int32_t)c);
 }
 
+// Rows `r0`, r0 + step, ... that have no user or several: zeros, or the sum over the users, which are found
+// by walking the choices from the lowest of them on, a block's width at a time, and added in ascending order.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(CB_THREADS)
-combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __restrict__ slots,
-                    const float* __restrict__ weights, const T* __restrict__ grad_out, int64_t n, int k, int d,
-                    const int32_t* __restrict__ users, const int32_t* __restrict__ first,
-                    T* __restrict__ grad_values, float* __restrict__ grad_weights) {
+__device__ __noinline__ void combine_other_rows(int64_t r0, int64_t step, int64_t n_values,
+                                                const int32_t* __restrict__ slots, const float* __restrict__ weights,
+                                                const T* __restrict__ grad_out, int64_t choices, int k, int d,
+                                                const int32_t* __restrict__ users, const int32_t* __restrict__ first,
+                                                T* __restrict__ grad_values) {
   typedef RowPiece<T, VEC> Piece;
-  __shared__ float red[CB_THREADS / 32][CB_K];
-  __shared__ int32_t list[CB_THREADS];
-  __shared__ int list_n[CB_THREADS / 32];
+  __shared__ int32_t list[CG_THREADS];
+  __shared__ int list_n[CG_THREADS / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if ((int64_t)blockIdx.x >= n) {
-    // the blocks behind the tokens': zeros for the rows that nobody chose
-    const int64_t step = (int64_t)gridDim.x - n;
-    Piece z;
-    z.clear();
-    for (int64_t r = (int64_t)blockIdx.x - n; r < n_values; r += step) {
-      if (users[r] != 0) continue;
-      for (int f0 = 0; f0 < d; f0 += Piece::SPAN)
-        if (!VEC || Piece::at(f0, 0) < d) z.store(grad_values + r * d, f0, d);
-    }
-    return;
-  }
-  const int64_t t = blockIdx.x;
-  const T* g_row = grad_out + t * d;
-  bool shared = false;
-  for (int j0 = 0; j0 < k; j0 += CB_K) {
-    int slot[CB_K];
-    float w[CB_K], dot[CB_K];
-    unsigned alone = 0;         // bit j: nobody else uses the row
-#pragma unroll
-    for (int j = 0; j < CB_K; ++j) {
-      slot[j] = j0 + j < k ? slots[t * k + j0 + j] : -1;
-      if (slot[j] >= n_values) slot[j] = -1;
-      w[j] = slot[j] >= 0 ? weights[t * k + j0 + j] : 0.f;
-      dot[j] = 0.f;
-      if (slot[j] >= 0) {
-        if (users[slot[j]] == 1) alone |= 1u << j;
-        else shared = true;
-      }
-    }
-    for (int f0 = 0; f0 < d; f0 += Piece::SPAN) {
-      if (VEC && Piece::at(f0, 0) >= d) continue;
-      Piece g, v[CB_K];
-      g.clear();
-      g.load(g_row, f0, d);
-#pragma unroll
-      for (int j = 0; j < CB_K; ++j) {
-        v[j].clear();
-        if (slot[j] >= 0) v[j].load(values + (int64_t)slot[j] * d, f0, d);
-      }
-#pragma unroll
-      for (int j = 0; j < CB_K; ++j) {
-        if (slot[j] < 0) continue;
-        Piece o;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float gi = to_float(g.t[i]);
-          dot[j] = fmaf(to_float(v[j].t[i]), gi, dot[j]);
-          o.t[i] = from_float<T>(w[j] * gi);
-        }
-        if ((alone >> j) & 1u) o.store(grad_values + (int64_t)slot[j] * d, f0, d);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < CB_K; ++j) {
-      dot[j] = warp_sum_of(dot[j]);
-      if (lane == 0) red[warp][j] = dot[j];
-    }
-    __syncthreads();
-    if (threadIdx.x < CB_K && j0 + threadIdx.x < k) {
-      float sum = 0.f;
-#pragma unroll
-      for (int q = 0; q < CB_THREADS / 32; ++q) sum += red[q][threadIdx.x];
-      grad_weights[t * k + j0 + threadIdx.x] = sum;     // 0 where there is no row
-    }
-    __syncthreads();
-  }
-  if (!shared) return;
-  // rows with several users: the block of the lowest of them finds the others by walking the choices
-  // behind it, CB_THREADS at a time, and adds them up in ascending order
-  for (int j = 0; j < k; ++j) {
-    const int64_t c0 = t * k + j;
-    const int slot = slots[c0];
-    if (slot < 0 || slot >= n_values || users[slot] == 1 || first[slot] != c0) continue;
-    for (int f0 = 0; f0 < d; f0 += Piece::SPAN) {
-      const bool in = !VEC || Piece::at(f0, 0) < d;
+  for (int64_t r = r0; r < n_values; r += step) {
+    const int count = users[r];
+    if (count == 1) continue;
+    for (int f0 = 0; f0 < d; f0 += Piece::span()) {
+      const bool in = Piece::at(f0, 0) < d;
       float acc[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-      int left = users[slot];
-      for (int64_t cb = c0; left > 0 && cb < n * k; cb += CB_THREADS) {
+      int left = count;
+      for (int64_t cb = count ? first[r] : choices; left > 0 && cb < choices; cb += blockDim.x) {
         const int64_t c = cb + threadIdx.x;
-        const bool hit = c < n * k && slots[c] == slot;
+        const bool hit = c < choices && slots[c] == r;
         const unsigned m = __ballot_sync(FULL, hit);
         if (lane == 0) list_n[warp] = __popc(m);
         __syncthreads();
         int at = 0, found = 0;
-        for (int q = 0; q < CB_THREADS / 32; ++q) {
+        for (int q = 0; q < (int)blockDim.x / 32; ++q) {
           if (q < warp) at += list_n[q];
           found += list_n[q];
         }
@@ -865,9 +842,83 @@ combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_
       Piece o;
 #pragma unroll
       for (int i = 0; i < 8; ++i) o.t[i] = from_float<T>(acc[i]);
-      if (in) o.store(grad_values + (int64_t)slot * d, f0, d);
+      if (in) o.store(grad_values + r * d, f0, d);
     }
   }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(CG_THREADS, 8)
+combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __restrict__ slots,
+                    const float* __restrict__ weights, const T* __restrict__ grad_out, int64_t n, int k, int d,
+                    const int32_t* __restrict__ users, const int32_t* __restrict__ first,
+                    T* __restrict__ grad_values, float* __restrict__ grad_weights, int64_t token_blocks) {
+  typedef RowPiece<T, VEC> Piece;
+  __shared__ float red[CG_THREADS / 32][CG_K];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if ((int64_t)blockIdx.x >= token_blocks) {
+    combine_other_rows<T, VEC>((int64_t)blockIdx.x - token_blocks, (int64_t)gridDim.x - token_blocks, n_values, slots,
+                               weights, grad_out, n * k, k, d, users, first, grad_values);
+    return;
+  }
+  // a block takes CG_K choices of a token
+  const int parts = (k + CG_K - 1) / CG_K;
+  const int64_t t = blockIdx.x / parts;
+  const int j0 = (int)(blockIdx.x - t * parts) * CG_K;
+  int slot[CG_K], used[CG_K];
+  float w[CG_K], dot[CG_K];
+#pragma unroll
+  for (int j = 0; j < CG_K; ++j) {
+    slot[j] = j0 + j < k ? slots[t * k + j0 + j] : -1;
+    if (slot[j] >= n_values) slot[j] = -1;
+  }
+#pragma unroll
+  for (int j = 0; j < CG_K; ++j) {
+    dot[j] = 0.f;
+    w[j] = slot[j] >= 0 ? weights[t * k + j0 + j] : 0.f;
+    used[j] = slot[j] >= 0 ? users[slot[j]] : 1;      // looked at when the first gradients are stored
+  }
+  for (int f0 = 0; f0 < d; f0 += Piece::span()) {
+    if (Piece::at(f0, 0) >= d) continue;
+    Piece g, v[CG_K];
+    g.clear();
+    g.load(grad_out + t * d, f0, d);
+#pragma unroll
+    for (int j = 0; j < CG_K; ++j) {
+      v[j].clear();
+      if (slot[j] >= 0) v[j].load(values + (int64_t)slot[j] * d, f0, d);
+    }
+#pragma unroll
+    for (int j = 0; j < CG_K; ++j) {
+      if (slot[j] < 0) continue;
+      Piece o;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float gi = to_float(g.t[i]);
+        dot[j] = fmaf(to_float(v[j].t[i]), gi, dot[j]);
+        o.t[i] = from_float<T>(w[j] * gi);
+      }
+      if (used[j] == 1) o.store(grad_values + (int64_t)slot[j] * d, f0, d);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < CG_K; ++j) {
+    dot[j] = warp_sum_of(dot[j]);
+    if (lane == 0) red[warp][j] = dot[j];
+  }
+  __syncthreads();
+  if (threadIdx.x < CG_K && j0 + threadIdx.x < k) {
+    float sum = 0.f;
+    for (int q = 0; q < (int)blockDim.x / 32; ++q) sum += red[q][threadIdx.x];
+    grad_weights[t * k + j0 + threadIdx.x] = sum;     // 0 where there is no row
+  }
+}
+
+// Threads for a row of d elements, eight to a thread: as few as do it in the fewest passes, so that a row a
+// little longer than a round number leaves no block nearly idle.
+static unsigned combine_threads(int d, int most) {
+  const int64_t passes = ceil_div(d, most * 8);
+  return (unsigned)(ceil_div(ceil_div(d, 8 * passes), 32) * 32);
 }
 
 static int check_route(const char* who, int n_experts, int k) {
@@ -966,7 +1017,11 @@ int kmb_expert_slots(const int32_t* experts, int64_t n, int k, int n_experts, in
   cudaStream_t s = (cudaStream_t)stream;
   const int64_t total = n * k;
   const int chunks = (int)ceil_div(total, SL_CHUNK);
-  const size_t smem = (size_t)n_experts * (sizeof(int32_t) + SL_WARPS * sizeof(uint16_t));
+  const size_t smem = (size_t)n_experts * (2 * sizeof(int32_t) + SL_WARPS * sizeof(uint16_t));
+  // the counters of 16 warps and the ordered chunk may pass the 48 KB that need no asking
+  const auto place = chunks <= 1 ? slots_place_kernel<true> : slots_place_kernel<false>;
+  if (smem > 8 * 1024)
+    KMB_CHECK_CUDA(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   if (chunks <= 1) {
     slots_place_kernel<true><<<1, SL_THREADS, smem, s>>>(experts, total, k, n_experts, nullptr, nullptr, slots,
                                                          rows, offsets);
@@ -977,7 +1032,7 @@ int kmb_expert_slots(const int32_t* experts, int64_t n, int k, int n_experts, in
   int32_t* totals = counts + (int64_t)chunks * n_experts;
   slots_count_kernel<<<chunks, SL_THREADS, 0, s>>>(experts, total, n_experts, counts);
   KMB_CHECK_LAUNCH();
-  slots_scan_kernel<<<(unsigned)ceil_div(n_experts, 8), 256, 0, s>>>(counts, chunks, n_experts, totals);
+  slots_scan_kernel<<<(unsigned)ceil_div(n_experts, 32), 1024, 0, s>>>(counts, chunks, n_experts, totals);
   KMB_CHECK_LAUNCH();
   slots_place_kernel<false><<<chunks, SL_THREADS, smem, s>>>(experts, total, k, n_experts, counts, totals, slots,
                                                              rows, offsets);
@@ -992,10 +1047,11 @@ int kmb_combine_experts(int dtype, const void* values, int64_t n_values, const i
   KMB_REQUIRE((values || n_values == 0) && slots && weights && out, "kmb_combine_experts: NULL argument");
   KMB_DISPATCH_ROWS(dtype, {
     const int vec = rows_are_vec((const T*)values, d) && rows_are_vec((const T*)out, d);
-    dim3 grid((unsigned)n, (unsigned)ceil_div(d, CB_THREADS * 8));
+    const unsigned threads = combine_threads(d, CB_THREADS);
+    dim3 grid((unsigned)n, (unsigned)ceil_div(d, threads * 8));
     if (grid.y > 65535) grid.y = 65535;
     const auto kernel = vec ? combine_kernel<T, true> : combine_kernel<T, false>;
-    kernel<<<grid, CB_THREADS, 0, (cudaStream_t)stream>>>((const T*)values, n_values, slots, weights, k, d, (T*)out);
+    kernel<<<grid, threads, 0, (cudaStream_t)stream>>>((const T*)values, n_values, slots, weights, k, d, (T*)out);
     KMB_CHECK_LAUNCH();
   });
   return KMB_OK;
@@ -1035,8 +1091,11 @@ int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, co
                     rows_are_vec((const T*)grad_values, d);
     const int64_t fill = n_values == 0 ? 0 : (ceil_div(n_values, 64) < sm_count() ? ceil_div(n_values, 64) : sm_count());
     const auto kernel = vec ? combine_grad_kernel<T, true> : combine_grad_kernel<T, false>;
-    kernel<<<(unsigned)(n + fill), CB_THREADS, 0, s>>>((const T*)values, n_values, slots, weights, (const T*)grad_out,
-                                                       n, k, d, users, first, (T*)grad_values, grad_weights);
+    const unsigned threads = combine_threads(d, CG_THREADS);
+    const int64_t token_blocks = n * ceil_div(k, CG_K);
+    kernel<<<(unsigned)(token_blocks + fill), threads, 0, s>>>((const T*)values, n_values, slots, weights,
+                                                               (const T*)grad_out, n, k, d, users, first,
+                                                               (T*)grad_values, grad_weights, token_blocks);
     KMB_CHECK_LAUNCH();
   });
   return KMB_OK;

@@ -20,12 +20,26 @@
 namespace kmb {
 
 // =============================================================================== quantisation
-// THREADS threads per row, ROWS rows per block.  A row of up to THREADS * VECS pieces of eight elements
-// stays in registers, as it lies in memory, between the maximum and the rounding; longer rows (VECS =
-// 0) are read a second time, from L1 and L2.
-__device__ __noinline__ uint32_t quantize_exactly(float x, float top) {
-  return (uint32_t)(int)rint((double)x * 127.0 / (double)top);
+// THREADS threads per row, ROWS rows per block.  Where there are rows enough to fill the GPU, a thread
+// holds four pieces of eight elements, so that enough bytes are on their way while other blocks wait at
+// their barrier or round; with few rows it holds one or two, for the latency of a row.  (A warp per row
+// with 16 pieces a lane had 12 warps on an SM and took 80 us for 8192 rows of 4096 bf16, a block of 256
+// with two pieces 32 us.)  The pieces stay in registers, as they lie in memory, between the maximum and the
+// rounding; rows longer than 8192 (VECS = 0) are read a second time, from L1 and L2.
+// The numbers of a piece in 64 bits, one at a time from memory: few pieces come here, and the registers of
+// the others are not indexed for their sake.
+template <typename T>
+__device__ __noinline__ void quantize_exactly(const T* row, int f, int d, float top, int8_t* q) {
+  for (int j = 0; j < 8 && f + j < d; ++j)
+    q[f + j] = (int8_t)(int)rint((double)to_float(row[f + j]) * 127.0 / (double)top);
 }
+
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> { typedef __half2 type; };
+template <>
+struct Pair<__nv_bfloat16> { typedef __nv_bfloat162 type; };
 
 template <typename T>
 struct QrPiece {
@@ -44,31 +58,37 @@ struct QrPiece {
   }
   // bits of the greatest |x|: whole numbers in the order of the values, NaN above infinity
   __device__ __forceinline__ uint32_t top() const {
-    uint32_t m = 0;
+    if constexpr (sizeof(T) == 2) {
+      typedef typename Pair<T>::type P;
+      const P* pairs = reinterpret_cast<const P*>(t);
+      const P m = __hmax2_nan(__hmax2_nan(__habs2(pairs[0]), __habs2(pairs[1])),
+                              __hmax2_nan(__habs2(pairs[2]), __habs2(pairs[3])));
+      return max(__float_as_uint(to_float(m.x)), __float_as_uint(to_float(m.y)));
+    } else {
+      uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(to_float(t[j])) & 0x7fffffffu);
-    return m;
+      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(to_float(t[j])) & 0x7fffffffu);
+      return m;
+    }
   }
-  // The eight 8-bit numbers.  r = x * (127 / top) in 32 bits is off by less than 127 * 3 * 2^-24 < 1e-4, so
-  // round_half_even(127 x / top) as exact arithmetic has it is r's own rounding unless r lies closer than
-  // that to the middle between two whole numbers; then the quotient in 64 bits decides (127 x is exact
-  // there, and a quotient of such short numbers is never rounded onto a middle that it does not hit).
-  // Adding 1.5 * 2^23 rounds to a whole number whose low byte is the result.
-  __device__ __forceinline__ uint2 round(float inv, float topf) const {
+  // The eight 8-bit numbers, and whether one of them is in doubt.  With f = 127 / top in 32 bits, x f is off
+  // 127 x / top by less than 127 * 2^-24 < 1e-5, so round_half_even(127 x / top) as exact arithmetic has it is
+  // the rounding of x f unless that lies closer than 1e-4 to the middle between two whole numbers; then the
+  // quotient in 64 bits decides (127 x is exact there, and a quotient of such short numbers is never rounded
+  // onto a middle that it does not hit).  x f + 1.5 * 2^23 in one operation is rounded to a whole number, whose
+  // low byte is the result; a second one gives what the rounding took away.
+  __device__ __forceinline__ uint2 round(float inv, bool& doubt) const {
     const float magic = 12582912.f;
     uint32_t n[8];
     float off = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float r = to_float(t[j]) * inv;
-      const float s = r + magic;
+      const float x = to_float(t[j]);
+      const float s = fmaf(x, inv, magic);
       n[j] = __float_as_uint(s);
-      off = fmaxf(off, fabsf(r - (s - magic)));
+      off = fmaxf(off, fabsf(fmaf(x, inv, magic - s)));
     }
-    if (!(off < 0.4999f && inv < 1e30f)) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) n[j] = quantize_exactly(to_float(t[j]), topf);
-    }
+    doubt = !(off < 0.4999f);
     uint2 p;
     p.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
     p.y = __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410);
@@ -77,7 +97,7 @@ struct QrPiece {
 };
 
 template <typename T, int THREADS, int ROWS, int VECS>
-__global__ void __launch_bounds__(THREADS * ROWS)
+__global__ void __launch_bounds__(THREADS * ROWS, (sizeof(T) == 2 ? 1536 : 1024) / (THREADS * ROWS))
 quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* __restrict__ rows, int64_t m,
                      int8_t* __restrict__ q, int64_t q_pitch, float* __restrict__ scales, int vec) {
   static_assert(ROWS == 1 || THREADS == 32, "several rows of a block take a warp each");
@@ -121,17 +141,22 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* _
   if (tid == 0) scales[i] = bad ? __uint_as_float(0x7fffffffu) : topf / 127.f;
   const bool zero = bad || top == 0u;
   const float inv = 127.f / topf;
+  const bool tiny = topf < 1e-30f;       // the factor runs out of range
   // the pitch is a multiple of 16, so the eight bytes of a piece lie inside the row's own storage
+  auto put = [&](const QrPiece<T>& piece, int f) {
+    bool doubt;
+    const uint2 p = piece.round(inv, doubt);
+    *reinterpret_cast<uint2*>(qi + f) = zero ? make_uint2(0u, 0u) : p;
+    if ((doubt || tiny) && !zero) quantize_exactly(xi, f, end, topf, qi);
+  };
   if (VECS > 0) {
 #pragma unroll
-    for (int r = 0; r < HELD; ++r) {
-      const int f = (r * THREADS + tid) * 8;
-      if (f < d) *reinterpret_cast<uint2*>(qi + f) = zero ? make_uint2(0u, 0u) : v[r].round(inv, topf);
-    }
+    for (int r = 0; r < HELD; ++r)
+      if ((r * THREADS + tid) * 8 < d) put(v[r], (r * THREADS + tid) * 8);
   } else {
     for (int f = tid * 8; f < d; f += THREADS * 8) {
-      if (!zero) v[0].load(xi, f, end, vec != 0);
-      *reinterpret_cast<uint2*>(qi + f) = zero ? make_uint2(0u, 0u) : v[0].round(inv, topf);
+      v[0].load(xi, f, end, vec != 0);
+      put(v[0], f);
     }
   }
 }
@@ -144,8 +169,12 @@ int quantize_run(const T* x, int64_t n, int d, const int32_t* rows, int64_t m, i
 #define KMB_RUN(THREADS, ROWS, VECS)                                                            \
   quantize_rows_kernel<T, THREADS, ROWS, VECS>                                                  \
       <<<ROWS == 1 ? one : four, THREADS * ROWS, 0, s>>>(x, n, d, rows, m, q, q_pitch, scales, vec)
+  const bool many = m >= (int64_t)sm_count() * 8;
   if (d <= 256) KMB_RUN(32, 4, 1);
   else if (d <= 512) KMB_RUN(32, 4, 2);
+  else if (many && d <= 1024) KMB_RUN(32, 4, 4);
+  else if (many && d <= 2048) KMB_RUN(64, 1, 4);
+  else if (many && d <= 4096) KMB_RUN(128, 1, 4);
   else if (d <= 1024) KMB_RUN(128, 1, 1);
   else if (d <= 2048) KMB_RUN(128, 1, 2);
   else if (d <= 4096) KMB_RUN(256, 1, 2);
