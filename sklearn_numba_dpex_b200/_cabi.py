@@ -158,17 +158,6 @@ def dtype_code(torch_dtype):
     raise ValueError(f"Expected float32 or float64 data but got {torch_dtype}")
 
 
-_ROW_TYPES = {torch.float32: KMB_F32, torch.float16: KMB_F16, torch.bfloat16: KMB_BF16}
-
-
-def row_dtype_code(torch_dtype, name):
-    """Type code of the expert and 8-bit calls, which take rows in 16 or 32 bits."""
-    code = _ROW_TYPES.get(torch_dtype)
-    if code is None:
-        raise ValueError(f"{name} must have dtype float32, float16 or bfloat16, got {torch_dtype}")
-    return code
-
-
 def ptr(t):
     """Device (or host) address of a tensor's first element; None -> NULL."""
     if t is None:
@@ -178,17 +167,6 @@ def ptr(t):
 
 def stream_ptr(device=None):
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
-def launch(name, device, *args):
-    """Enqueues a library call on `device`'s current stream, which it gets as its last argument, with
-    `device` the current one: the library asks the current device for its size.  Addresses may be
-    plain numbers here (a small call costs a few microseconds on the host, and wrapping them shows)."""
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return launch(name, device, *args)
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    return check(getattr(lib, name)(*args, stream), name)
 
 
 def require_cuda_tensor(t, name, dtype=None, contiguous=True):

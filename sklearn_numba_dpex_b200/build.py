@@ -1,4 +1,5 @@
-"""Builds csrc/*.cu into libkmb200.so (sm_100a) next to this file.
+"""Builds csrc/*.cu into libkmb200.so (sm_100a) and csrc/torch_calls.cpp into _torch_calls.so, next to
+this file.
 
     python -m sklearn_numba_dpex_b200.build [--force] [--verbose]
 
@@ -18,6 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OBJ_DIR = os.path.join(CSRC, "build")
 LIB_PATH = os.path.join(HERE, "libkmb200.so")
+CALLS_PATH = os.path.join(HERE, "_torch_calls.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -79,7 +81,30 @@ def build(force=False, verbose=False):
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
+    build_calls(force)
     return LIB_PATH
+
+
+def build_calls(force=False):
+    """The binding of the calls whose host time counts: a Python extension over torch's C++ tensors."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    src = os.path.join(CSRC, "torch_calls.cpp")
+    newest = max(os.path.getmtime(src), _headers_mtime())
+    if not force and os.path.exists(CALLS_PATH) and os.path.getmtime(CALLS_PATH) >= newest:
+        return CALLS_PATH
+    includes = include_paths("cuda") + [sysconfig.get_paths()["include"], INCLUDE]
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", CALLS_PATH]
+    cmd += [f"-I{path}" for path in includes] + [f"-L{path}" for path in library_paths("cuda")]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-L{HERE}", "-l:libkmb200.so", "-Wl,-rpath,$ORIGIN"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed on torch_calls.cpp:\n{proc.stdout}\n{proc.stderr}")
+    return CALLS_PATH
 
 
 if __name__ == "__main__":

@@ -14,21 +14,10 @@ All tensors live on one CUDA device; a call is enqueued on that device's current
 """
 import torch
 
-from .._cabi import ROUTE_RENORMALIZE, ROUTE_SIGMOID, launch, lib, require_cuda_tensor, row_dtype_code
+from .._cabi import ROUTE_RENORMALIZE, ROUTE_SIGMOID
+from . import _calls
 
 _SCORINGS = {"softmax": 0, "sigmoid": ROUTE_SIGMOID}
-
-
-def _matrix(t, name, dtype=None):
-    require_cuda_tensor(t, name, dtype, contiguous=False)
-    if t.dim() != 2:
-        raise ValueError(f"{name} must have two dimensions, got {t.dim()}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _same_device(t, name, other):
-    if t.device != other.device:
-        raise ValueError(f"{name} must be on {other.device}, got {t.device}")
 
 
 def _flags(scoring, renormalize):
@@ -38,24 +27,12 @@ def _flags(scoring, renormalize):
 
 
 # ------------------------------------------------------------------------------- routing
-def _route(logits, k, bias, flags, n_groups, topk_groups, group_best, scale):
-    n, e = logits.shape
-    dev = logits.device
-    weights = torch.empty((n, k), dtype=torch.float32, device=dev)
-    experts = torch.empty((n, k), dtype=torch.int32, device=dev)
-    launch("kmb_route_topk", dev, row_dtype_code(logits.dtype, "logits"), logits.data_ptr(),
-           None if bias is None else bias.data_ptr(), n, e, k, flags, n_groups, topk_groups, group_best, scale,
-           weights.data_ptr(), experts.data_ptr())
-    return weights, experts
-
-
 class _RouteTopk(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, k, bias, scoring, n_groups, topk_groups, group_best, renormalize, scale):
-        weights, experts = _route(logits, k, bias, _flags(scoring, renormalize), n_groups, topk_groups,
-                                  group_best, scale)
+    def forward(ctx, logits, k, bias, flags, n_groups, topk_groups, group_best, scale):
+        weights, experts = _calls.route_topk(logits, k, bias, flags, n_groups, topk_groups, group_best, scale)
         ctx.save_for_backward(logits, experts)
-        ctx.settings = (scoring, renormalize, scale)
+        ctx.settings = (flags, scale)
         ctx.mark_non_differentiable(experts)
         return weights, experts
 
@@ -63,9 +40,7 @@ class _RouteTopk(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_weights, _):
         logits, experts = ctx.saved_tensors
-        scoring, renormalize, scale = ctx.settings
-        grad = route_topk_grad(logits, experts, grad_weights, scoring, renormalize, scale)
-        return (grad,) + (None,) * 8
+        return (_calls.route_topk_grad(logits, experts, grad_weights, *ctx.settings),) + (None,) * 7
 
 
 def route_topk(logits, k, bias=None, scoring="softmax", n_groups=1, topk_groups=None, group_best=1,
@@ -86,40 +61,17 @@ def route_topk(logits, k, bias=None, scoring="softmax", n_groups=1, topk_groups=
 
     Differentiable in `logits`, the choice being held fixed.
     """
-    logits = _matrix(logits, "logits")
-    if bias is not None:
-        require_cuda_tensor(bias, "bias", torch.float32)
-        _same_device(bias, "bias", logits)
-        if bias.shape != (logits.shape[1],):
-            raise ValueError(f"bias must have shape ({logits.shape[1]},), got {tuple(bias.shape)}")
-    k, n_groups = int(k), int(n_groups)
-    topk_groups = n_groups if topk_groups is None else int(topk_groups)
-    if k < 1:
-        raise ValueError(f"k must be at least 1, got {k}")
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _RouteTopk.apply(logits, k, bias, scoring, n_groups, topk_groups, int(group_best),
-                                bool(renormalize), float(scale))
-    return _route(logits, k, bias, _flags(scoring, renormalize), n_groups, topk_groups, int(group_best),
-                  float(scale))
+    flags = _flags(scoring, renormalize)
+    topk_groups = n_groups if topk_groups is None else topk_groups
+    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
+        return _RouteTopk.apply(logits, k, bias, flags, n_groups, topk_groups, group_best, scale)
+    return _calls.route_topk(logits, k, bias, flags, n_groups, topk_groups, group_best, scale)
 
 
 def route_topk_grad(logits, experts, grad_weights, scoring="softmax", renormalize=True, scale=1.0):
     """Gradient of the weights of `route_topk` to its logits (n, n_experts), in their dtype, for callers
     that keep their own backward pass; `experts` is what `route_topk` returned."""
-    logits = _matrix(logits, "logits")
-    experts = _matrix(experts, "experts", torch.int32)
-    grad_weights = _matrix(grad_weights, "grad_weights", torch.float32)
-    n, e = logits.shape
-    if experts.shape[0] != n or grad_weights.shape != experts.shape:
-        raise ValueError(f"experts and grad_weights must both have shape ({n}, k), got {tuple(experts.shape)} "
-                         f"and {tuple(grad_weights.shape)}")
-    _same_device(experts, "experts", logits)
-    _same_device(grad_weights, "grad_weights", logits)
-    grad = torch.empty_like(logits)
-    launch("kmb_route_topk_grad", logits.device, row_dtype_code(logits.dtype, "logits"), logits.data_ptr(),
-           experts.data_ptr(), grad_weights.data_ptr(), n, e, experts.shape[1], _flags(scoring, renormalize),
-           float(scale), grad.data_ptr())
-    return grad
+    return _calls.route_topk_grad(logits, experts, grad_weights, _flags(scoring, renormalize), scale)
 
 
 # --------------------------------------------------------------------------- expert order
@@ -131,53 +83,20 @@ def expert_slots(experts, n_experts):
     ``offsets[e]:offsets[e + 1]``.  A choice that is no expert (-1) has slot -1 and takes no place; the
     places behind ``offsets[n_experts]`` then hold -1.  Nothing waits for the GPU.
     """
-    experts = _matrix(experts, "experts", torch.int32)
-    n, k = experts.shape
-    n_experts = int(n_experts)
-    if k < 1:
-        raise ValueError("experts must have at least one column")
-    dev = experts.device
-    slots = torch.empty_like(experts)
-    rows = torch.empty(n * k, dtype=torch.int32, device=dev)
-    offsets = torch.empty(max(n_experts, 0) + 1, dtype=torch.int32, device=dev)
-    nbytes = lib.kmb_expert_slots_workspace_bytes(n, k, n_experts)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    launch("kmb_expert_slots", dev, experts.data_ptr(), n, k, n_experts, slots.data_ptr(), rows.data_ptr(),
-           offsets.data_ptr(), ws.data_ptr() if nbytes else None, nbytes)
-    return slots, rows, offsets
+    return _calls.expert_slots(experts, n_experts)
 
 
 # --------------------------------------------------------------------------- weighted sums
-def _combine_args(values, slots, weights):
-    values = _matrix(values, "values")
-    slots = _matrix(slots, "slots", torch.int32)
-    weights = _matrix(weights, "weights", torch.float32)
-    if weights.shape != slots.shape:
-        raise ValueError(f"weights must have the shape of slots {tuple(slots.shape)}, got {tuple(weights.shape)}")
-    _same_device(slots, "slots", values)
-    _same_device(weights, "weights", values)
-    return values, slots, weights
-
-
-def _combine(values, slots, weights):
-    n, k = slots.shape
-    dev = values.device
-    out = torch.empty((n, values.shape[1]), dtype=values.dtype, device=dev)
-    launch("kmb_combine_experts", dev, row_dtype_code(values.dtype, "values"), values.data_ptr(), values.shape[0],
-           slots.data_ptr(), weights.data_ptr(), n, k, values.shape[1], out.data_ptr())
-    return out
-
-
 class _CombineExperts(torch.autograd.Function):
     @staticmethod
     def forward(ctx, values, slots, weights):
         ctx.save_for_backward(values, slots, weights)
-        return _combine(values, slots, weights)
+        return _calls.combine_experts(values, slots, weights)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        grad_values, grad_weights = combine_experts_grad(*ctx.saved_tensors, grad_out)
+        grad_values, grad_weights = _calls.combine_experts_grad(*ctx.saved_tensors, grad_out)
         return grad_values, None, grad_weights
 
 
@@ -189,27 +108,13 @@ def combine_experts(values, slots, weights):
     slot outside ``[0, m)`` adds nothing.  Sums are held in 32 bits; the result has the dtype of `values`
     (float32, float16 or bfloat16).  Differentiable in `values` and `weights`.
     """
-    values, slots, weights = _combine_args(values, slots, weights)
-    if torch.is_grad_enabled() and (values.requires_grad or weights.requires_grad):
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (values, weights)):
         return _CombineExperts.apply(values, slots, weights)
-    return _combine(values, slots, weights)
+    return _calls.combine_experts(values, slots, weights)
 
 
 def combine_experts_grad(values, slots, weights, grad_out):
     """``(grad_values, grad_weights)`` of `combine_experts`, for callers that keep their own backward pass.
     Rows of `values` that several slots name get the sum of their gradients, in a fixed order; rows that
     none names get zeros."""
-    values, slots, weights = _combine_args(values, slots, weights)
-    grad_out = _matrix(grad_out, "grad_out", values.dtype)
-    n, k = slots.shape
-    if grad_out.shape != (n, values.shape[1]):
-        raise ValueError(f"grad_out must have shape ({n}, {values.shape[1]}), got {tuple(grad_out.shape)}")
-    _same_device(grad_out, "grad_out", values)
-    dev = values.device
-    grad_values, grad_weights = torch.empty_like(values), torch.empty_like(weights)
-    nbytes = lib.kmb_combine_experts_grad_workspace_bytes(values.shape[0])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    launch("kmb_combine_experts_grad", dev, row_dtype_code(values.dtype, "values"), values.data_ptr(),
-           values.shape[0], slots.data_ptr(), weights.data_ptr(), grad_out.data_ptr(), n, k, values.shape[1],
-           grad_values.data_ptr(), grad_weights.data_ptr(), ws.data_ptr(), nbytes)
-    return grad_values, grad_weights
+    return _calls.combine_experts_grad(values, slots, weights, grad_out)
