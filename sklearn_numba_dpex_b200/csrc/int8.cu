@@ -13,6 +13,7 @@
 #include <cuda_fp16.h>
 #include <stdlib.h>
 
+#include "early_launch.cuh"
 #include "kmb_common.cuh"
 #include "row_types.cuh"
 #include "tc_ptx.cuh"
@@ -101,6 +102,8 @@ __global__ void __launch_bounds__(THREADS * ROWS, (sizeof(T) == 2 ? 1536 : 1024)
 quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* __restrict__ rows, int64_t m,
                      int8_t* __restrict__ q, int64_t q_pitch, float* __restrict__ scales, int vec) {
   static_assert(ROWS == 1 || THREADS == 32, "several rows of a block take a warp each");
+  next_grid_may_start();
+  grid_dependency_wait();
   __shared__ uint32_t red[THREADS / 32];
   const int tid = threadIdx.x % THREADS;
   const int64_t i = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
@@ -167,8 +170,8 @@ int quantize_run(const T* x, int64_t n, int d, const int32_t* rows, int64_t m, i
   const int vec = rows_are_vec(x, d) ? 1 : 0;
   const unsigned one = (unsigned)m, four = (unsigned)ceil_div(m, 4);
 #define KMB_RUN(THREADS, ROWS, VECS)                                                            \
-  quantize_rows_kernel<T, THREADS, ROWS, VECS>                                                  \
-      <<<ROWS == 1 ? one : four, THREADS * ROWS, 0, s>>>(x, n, d, rows, m, q, q_pitch, scales, vec)
+  return launch_early(quantize_rows_kernel<T, THREADS, ROWS, VECS>, ROWS == 1 ? one : four, THREADS * ROWS, 0, 1, s, x, \
+                      n, d, rows, m, q, q_pitch, scales, vec)
   const bool many = m >= (int64_t)sm_count() * 8;
   if (d <= 256) KMB_RUN(32, 4, 1);
   else if (d <= 512) KMB_RUN(32, 4, 2);
@@ -181,8 +184,6 @@ int quantize_run(const T* x, int64_t n, int d, const int32_t* rows, int64_t m, i
   else if (d <= 8192) KMB_RUN(256, 1, 4);
   else KMB_RUN(256, 1, 0);
 #undef KMB_RUN
-  KMB_CHECK_LAUNCH();
-  return KMB_OK;
 }
 
 // ==================================================================================== product
@@ -191,12 +192,20 @@ int quantize_run(const T* x, int64_t n, int d, const int32_t* rows, int64_t m, i
 // a few tokens then cost a narrow instruction, and the weights, which bound small batches, stream
 // through at full width.
 //
-// One persistent CTA per SM, eight warps: 0 loads (TMA, 128-byte swizzle, a ring of stages of 128
-// bytes of the contraction), 1 issues the MMAs, 2 owns tensor memory, 4..7 scale and store (one
-// feature per lane).  Two accumulators, so that the stores of a tile overlap the MMAs of the next.
+// One persistent CTA per SM, twelve warps: 0 loads (TMA, 128-byte swizzle, a ring of stages of 128
+// bytes of the contraction), 1 issues the MMAs, 2 owns tensor memory, 4..11 scale and store (one
+// feature per lane, half of the tokens each).  Two accumulators, so that the stores of a tile overlap the
+// MMAs of the next.  (With four storing warps a tile of 256 tokens and 2056 features took longer to store
+// than to multiply: 88 us for 16 396 rows of 32 groups and 1408 outputs.)
+//
+// SPLIT: few tiles.  A cluster of CTAs shares a tile, each summing a run of the contraction, so that more
+// SMs stream weights; the int32 partial sums meet through distributed shared memory, exactly, and each
+// CTA stores a share of the tokens.  A cluster has one tile at most.
 constexpr int I8_BM = 128;
 constexpr int I8_KB = 128;            // bytes (= 8-bit features) per stage
-constexpr int I8_THREADS = 256;
+constexpr int I8_EPI_WARPS = 8;
+constexpr int I8_THREADS = 128 + I8_EPI_WARPS * 32;
+constexpr int I8_SCAN_THREADS = 256;
 constexpr int I8_MAX_GROUPS = 1024;
 constexpr long long I8_TIMEOUT_CYCLES = 4000000000LL;   // ~2 s at 2 GHz
 
@@ -215,8 +224,9 @@ struct I8Smem {
   unsigned char a[I8Cfg<BN>::STAGES][I8Cfg<BN>::A_BYTES];
   unsigned char b[I8Cfg<BN>::STAGES][I8Cfg<BN>::B_BYTES];
   int first_tile[I8_MAX_GROUPS + 1];   // tiles before each group
-  int scan[I8_THREADS / 32];
+  int scan[I8_SCAN_THREADS / 32];
   float sa[BN];
+  int bad;                             // SPLIT: this CTA's partial sums are not to be used
   unsigned long long full[I8Cfg<BN>::STAGES], empty[I8Cfg<BN>::STAGES];
   unsigned long long acc_full[2], acc_empty[2], drain;
   long long timeout_cycles;
@@ -315,14 +325,50 @@ __device__ __forceinline__ I8Tile i8_tile(const I8Params& p, const int* first_ti
   return r;
 }
 
-template <int BN, typename T>
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+// A word of the shared memory of CTA `rank` of the cluster, at the place `p` has in this one's.
+__device__ __forceinline__ int load_from(const void* p, uint32_t rank) {
+  uint32_t addr;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Scales COLS accumulator columns (tokens) of one feature and stores them; FULL: all of them are rows.
+template <int COLS, bool FULL, typename T>
+__device__ __forceinline__ void i8_store(const uint32_t (&v)[COLS], const float* sa, float sb, float bias, T* o,
+                                         int64_t stride, int rows) {
+#pragma unroll
+  for (int j = 0; j < COLS; ++j) {
+    if (FULL || j < rows) *o = from_float<T>((float)(int)v[j] * (sa[j] * sb) + bias);
+    o += stride;
+  }
+}
+
+template <int BN, typename T, bool SPLIT>
 __global__ void __launch_bounds__(I8_THREADS, 1)
 int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
-                   const I8Params p) {
+                   const __grid_constant__ I8Params p) {
   using Cfg = I8Cfg<BN>;
   extern __shared__ __align__(16) unsigned char i8_dyn[];
   I8Smem<BN>* sm = reinterpret_cast<I8Smem<BN>*>(((uintptr_t)i8_dyn + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int splits = SPLIT ? (int)cluster_size() : 1, split = SPLIT ? (int)cluster_rank() : 0;
+  const int first = SPLIT ? blockIdx.x / splits : blockIdx.x;    // this CTA's (or cluster's) first tile
+  const int step = SPLIT ? gridDim.x / splits : gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::STAGES; ++s) {
@@ -331,25 +377,36 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sm->acc_full[b], 1);
-      mbar_init(&sm->acc_empty[b], 4);
+      mbar_init(&sm->acc_empty[b], I8_EPI_WARPS);
     }
     mbar_init(&sm->drain, 1);
     sm->timeout_cycles = p.timeout_cycles;
     sm->abort_flag = 0;
+    sm->bad = 0;
     fence_barrier_init();
   }
   if (warp == 2) {
     tmem_alloc(&sm->tmem_base, Cfg::TMEM_COLS);
     tmem_relinquish();
   }
+  // what came before on the stream is not waited for until here: the set-up above overlaps it
+  grid_dependency_wait();
   // tiles before each group: a block-wide exclusive sum, four consecutive groups per thread
-  {
-    int cnt[I8_MAX_GROUPS / I8_THREADS], sum = 0;
+  if (p.groups == 1) {
+    if (threadIdx.x == 0) {
+      const int64_t rows = i8_row_of(p, 1) - i8_row_of(p, 0);
+      sm->first_tile[0] = 0;
+      sm->first_tile[1] = rows > 0 ? (int)((rows + BN - 1) / BN) * p.feature_tiles : 0;
+    }
+  } else {
+    constexpr int PER = I8_MAX_GROUPS / I8_SCAN_THREADS;
+    const bool scans = threadIdx.x < I8_SCAN_THREADS;
+    int cnt[PER], sum = 0;
 #pragma unroll
-    for (int j = 0; j < I8_MAX_GROUPS / I8_THREADS; ++j) {
-      const int g = threadIdx.x * (I8_MAX_GROUPS / I8_THREADS) + j;
+    for (int j = 0; j < PER; ++j) {
+      const int g = threadIdx.x * PER + j;
       cnt[j] = 0;
-      if (g < p.groups) {
+      if (scans && g < p.groups) {
         const int64_t rows = i8_row_of(p, g + 1) - i8_row_of(p, g);
         cnt[j] = rows > 0 ? (int)((rows + BN - 1) / BN) * p.feature_tiles : 0;
       }
@@ -361,34 +418,39 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       const int v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
-    if (lane == 31) sm->scan[warp] = inc;
+    if (scans && lane == 31) sm->scan[warp] = inc;
     __syncthreads();
-    int base = inc - sum;
-    for (int w = 0; w < warp; ++w) base += sm->scan[w];
+    if (scans) {
+      int base = inc - sum;
+      for (int w = 0; w < warp; ++w) base += sm->scan[w];
 #pragma unroll
-    for (int j = 0; j < I8_MAX_GROUPS / I8_THREADS; ++j) {
-      const int g = threadIdx.x * (I8_MAX_GROUPS / I8_THREADS) + j;
-      if (g <= p.groups) sm->first_tile[g] = base;
-      base += cnt[j];
+      for (int j = 0; j < PER; ++j) {
+        const int g = threadIdx.x * PER + j;
+        if (g <= p.groups) sm->first_tile[g] = base;
+        base += cnt[j];
+      }
+      if (threadIdx.x == I8_SCAN_THREADS - 1 && p.groups == I8_MAX_GROUPS) sm->first_tile[I8_MAX_GROUPS] = base;
     }
-    if (threadIdx.x == I8_THREADS - 1 && p.groups == I8_MAX_GROUPS) sm->first_tile[I8_MAX_GROUPS] = base;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = sm->tmem_base;
   const int tiles = sm->first_tile[p.groups];
-  const int chunks = (p.d + I8_KB - 1) / I8_KB;
+  const int all_chunks = (p.d + I8_KB - 1) / I8_KB;
+  // this CTA's run of the contraction (each has one chunk at least: the host sees to it)
+  const int c_begin = SPLIT ? (int)((int64_t)all_chunks * split / splits) : 0;
+  const int c_end = SPLIT ? (int)((int64_t)all_chunks * (split + 1) / splits) : all_chunks;
 
   if (warp == 0) {
     // ------------------------------------------------------------------------ loads
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int t = first; t < tiles && ok; t += step) {
         const I8Tile tile = i8_tile<BN>(p, sm->first_tile, t);
         const int w_row = tile.g * p.n + tile.feature0;
-        for (int c = 0; c < chunks; ++c, ++it) {
+        for (int c = c_begin; c < c_end; ++c, ++it) {
           const uint32_t s = it % Cfg::STAGES, lap = it / Cfg::STAGES;
           if (!i8_wait(&sm->empty[s], (lap & 1u) ^ 1u, sm)) {
             ok = false;
@@ -397,23 +459,27 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
           mbar_expect_tx(&sm->full[s], Cfg::A_BYTES + Cfg::B_BYTES);
           tma_load_2d(sm->a[s], &map_w, c * I8_KB, w_row, &sm->full[s]);
           tma_load_2d(sm->b[s], &map_x, c * I8_KB, (int)tile.row0, &sm->full[s]);
+          if (p.test_stall && c == c_end - 1 - SPLIT) ok = false;
+          if (!ok) {
+            ++it;
+            break;
+          }
         }
-        if (p.test_stall) break;
       }
       if (sm->abort_flag) drain_ring(sm->full, Cfg::STAGES, it);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------------- MMAs
     const uint64_t a0 = make_sdesc(smem_u32(sm->a[0])), b0 = make_sdesc(smem_u32(sm->b[0]));
-    const int last_steps = ((p.d - (chunks - 1) * I8_KB) + 31) / 32;   // 32 features per instruction
+    const int last_steps = ((p.d - (all_chunks - 1) * I8_KB) + 31) / 32;   // 32 features per instruction
     uint32_t it = 0, nt = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++nt) {
+    for (int t = first; t < tiles && ok; t += step, ++nt) {
       const uint32_t ab = nt & 1u;
       if (!__all_sync(0xffffffffu, i8_wait(&sm->acc_empty[ab], ((nt >> 1) & 1u) ^ 1u, sm))) break;
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + ab * BN;
-      for (int c = 0; c < chunks; ++c, ++it) {
+      for (int c = c_begin; c < c_end; ++c, ++it) {
         const uint32_t s = it % Cfg::STAGES, lap = it / Cfg::STAGES;
         if (!__all_sync(0xffffffffu, i8_wait(&sm->full[s], lap & 1u, sm))) {
           ok = false;
@@ -423,11 +489,11 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         if (elect_one()) {
           const uint64_t ad = a0 + (uint64_t)(s * (Cfg::A_BYTES >> 4));
           const uint64_t bd = b0 + (uint64_t)(s * (Cfg::B_BYTES >> 4));
-          const int steps = c == chunks - 1 ? last_steps : 4;
+          const int steps = c == all_chunks - 1 ? last_steps : 4;
           for (int ks = 0; ks < steps; ++ks)
-            umma_i8_ss(d_tmem, ad + 2 * ks, bd + 2 * ks, Cfg::IDESC, (c | ks) != 0);
+            umma_i8_ss(d_tmem, ad + 2 * ks, bd + 2 * ks, Cfg::IDESC, (c > c_begin || ks > 0) ? 1u : 0u);
           umma_commit(&sm->empty[s]);
-          if (c == chunks - 1) umma_commit(&sm->acc_full[ab]);
+          if (c == c_end - 1) umma_commit(&sm->acc_full[ab]);
         }
         __syncwarp();
       }
@@ -435,41 +501,66 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (sm->abort_flag) mma_drain(&sm->drain);
   } else if (warp >= 4) {
     // --------------------------------------------------------------- scales and stores
-    const int q = warp & 3;
+    const int q = warp & 3, half = (warp - 4) >> 2;
     const int etid = threadIdx.x - 128;
+    constexpr int EPI = I8_EPI_WARPS * 32;
     T* out = reinterpret_cast<T*>(p.out);
     if (p.offsets) {
       // rows behind the last group belong to nobody: zeros
       const int64_t end = i8_row_of(p, p.groups);
-      const int64_t first = end * p.n, last = p.m * p.n;
-      for (int64_t e = first + (int64_t)blockIdx.x * 128 + etid; e < last; e += (int64_t)gridDim.x * 128)
+      const int64_t from = end * p.n, to = p.m * p.n;
+      for (int64_t e = from + (int64_t)blockIdx.x * EPI + etid; e < to; e += (int64_t)gridDim.x * EPI)
         out[e] = from_float<T>(0.f);
     }
+    // columns of this warp: half of the tile's tokens (all, where that would be less than 16)
+    constexpr int COLS = BN >= 64 ? 32 : 16;
+    constexpr int MINE = BN >= 32 ? BN / 2 : BN;
+    const int col0 = BN >= 32 ? half * MINE : 0;
+    const bool works = BN >= 32 || half == 0;
     uint32_t nt = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++nt) {
+    for (int t = first; t < tiles; t += step, ++nt) {
       const I8Tile tile = i8_tile<BN>(p, sm->first_tile, t);
       const uint32_t ab = nt & 1u;
-      asm volatile("bar.sync 1, 128;" ::: "memory");   // everybody is done with the last tile's scales
-      for (int r = etid; r < BN; r += 128) sm->sa[r] = r < tile.rows ? p.sa[tile.row0 + r] : 0.f;
+      asm volatile("bar.sync 1, 256;" ::: "memory");   // everybody is done with the last tile's scales
+      for (int r = etid; r < BN; r += EPI) sm->sa[r] = r < tile.rows ? p.sa[tile.row0 + r] : 0.f;
       const int feature = tile.feature0 + q * 32 + lane;
       const bool mine = feature < p.n;
       const int64_t wrow = (int64_t)tile.g * p.n + feature;
       float sb = mine ? p.sb[wrow] : 0.f;
       const float bias = (mine && p.bias) ? p.bias[wrow] : 0.f;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       const bool ok = __all_sync(0xffffffffu, i8_wait(&sm->acc_full[ab], (nt >> 1) & 1u, sm));
-      if (!ok) sb = __uint_as_float(0x7fffffffu);      // a wait ran out: the tile becomes NaN
       tc_fence_after();
-      T* o = out + tile.row0 * p.n + feature;
+      const uint32_t acc = tmem_base + ab * BN + ((uint32_t)(q * 32) << 16);
+      if (SPLIT) {
+        // partial sums [token][feature] into the stages, which nobody needs any more
+        int* part = reinterpret_cast<int*>(sm->a[0]);
+        if (!ok && lane == 0) sm->bad = 1;
+        if (works) {
 #pragma unroll 1
-      for (int c0 = 0; c0 < BN; c0 += 16) {
-        uint32_t v[16];
-        tmem_ld16(tmem_base + ab * BN + c0 + ((uint32_t)(q * 32) << 16), v);
-        tmem_ld_wait();
+          for (int c = 0; c < MINE; c += 16) {
+            uint32_t v[16];
+            tmem_ld16(acc + col0 + c, v);
+            tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (mine && c0 + j < tile.rows)
-            o[(int64_t)(c0 + j) * p.n] = from_float<T>((float)(int)v[j] * (sm->sa[c0 + j] * sb) + bias);
+            for (int j = 0; j < 16; ++j) part[(col0 + c + j) * I8_BM + q * 32 + lane] = (int)v[j];
+          }
+        }
+      } else {
+        if (!ok) sb = __uint_as_float(0x7fffffffu);      // a wait ran out: the tile becomes NaN
+        if (works) {
+          T* o = out + (tile.row0 + col0) * p.n + feature;
+          const int rows = mine ? tile.rows - col0 : 0;
+#pragma unroll 1
+          for (int c = 0; c < MINE; c += COLS, o += (int64_t)COLS * p.n) {
+            uint32_t v[COLS];
+            if constexpr (COLS == 32) tmem_ld32(acc + col0 + c, v);
+            else tmem_ld16(acc + col0 + c, v);
+            tmem_ld_wait();
+            if (rows - c >= COLS) i8_store<COLS, true>(v, sm->sa + col0 + c, sb, bias, o, p.n, 0);
+            else i8_store<COLS, false>(v, sm->sa + col0 + c, sb, bias, o, p.n, rows - c);
+          }
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -477,7 +568,33 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
   }
   tc_fence_before();
-  __syncthreads();
+  if (SPLIT) {
+    __syncwarp();
+    cluster_sync();        // every partial sum of the cluster lies in shared memory
+    if (warp >= 4 && first < tiles) {
+      const I8Tile tile = i8_tile<BN>(p, sm->first_tile, first);
+      const int q = warp & 3, half = (warp - 4) >> 2;
+      const int feature = tile.feature0 + q * 32 + lane;
+      bool bad = false;
+      for (int r = 0; r < splits; ++r) bad = bad || load_from(&sm->bad, r) != 0;
+      if (feature < p.n) {
+        const int64_t wrow = (int64_t)tile.g * p.n + feature;
+        const float sb = bad ? __uint_as_float(0x7fffffffu) : p.sb[wrow];
+        const float bias = p.bias ? p.bias[wrow] : 0.f;
+        const int* part = reinterpret_cast<const int*>(sm->a[0]);
+        for (int c = split * 2 + half; c < tile.rows; c += splits * 2) {
+          int sum = 0;
+          for (int r = 0; r < splits; ++r) sum += load_from(part + c * I8_BM + q * 32 + lane, r);
+          reinterpret_cast<T*>(p.out)[(tile.row0 + c) * p.n + feature] =
+              from_float<T>((float)sum * (sm->sa[c] * sb) + bias);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync();        // and nobody reads this CTA's any more
+  } else {
+    __syncthreads();
+  }
   if (warp == 2) {
     tc_fence_after();
     tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
@@ -506,20 +623,26 @@ static int i8_make_map(CUtensorMap* map, const int8_t* base, int64_t rows, int d
   return KMB_OK;
 }
 
-template <int BN, typename T>
+template <int BN, typename T, bool SPLIT>
 int i8_launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const I8Params& p, unsigned grid,
-              cudaStream_t s) {
+              int splits, cudaStream_t s) {
   const int smem = (int)sizeof(I8Smem<BN>) + 1024;
-  KMB_CHECK_CUDA(cudaFuncSetAttribute(int8_matmul_kernel<BN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      smem));
-  int8_matmul_kernel<BN, T><<<grid, I8_THREADS, smem, s>>>(map_w, map_x, p);
-  KMB_CHECK_LAUNCH();
-  return KMB_OK;
+  const auto kernel = int8_matmul_kernel<BN, T, SPLIT>;
+  KMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  return launch_early(kernel, grid, I8_THREADS, smem, splits, s, map_w, map_x, p);
 }
 
-template <int BN>
-int i8_run(int out_dtype, const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, I8Params p,
-           cudaStream_t s) {
+// CTAs that share a tile: as many as the SMs allow, while each has two stages' worth of the contraction
+// at least.
+static int i8_splits(int64_t tiles, int d) {
+  const int chunks = (d + I8_KB - 1) / I8_KB;
+  int s = 8;
+  while (s > 1 && (tiles * s > sm_count() || chunks < 2 * s)) s >>= 1;
+  return s;
+}
+
+template <int BN, typename T>
+int i8_run_as(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, I8Params p, cudaStream_t s) {
   CUtensorMap map_w, map_x;
   int rc = i8_make_map(&map_w, b, (int64_t)p.groups * p.n, p.d, ldb, I8_BM);
   if (rc != KMB_OK) return rc;
@@ -528,10 +651,17 @@ int i8_run(int out_dtype, const int8_t* a, int64_t lda, const int8_t* b, int64_t
   // an upper bound of the tiles: every group may end inside one
   const int64_t most = (ceil_div(p.m, BN) + p.groups - 1) * p.feature_tiles;
   KMB_REQUIRE(most < (1ll << 31), "kmb_int8_matmul: too many output tiles");
-  const unsigned grid = (unsigned)(most < sm_count() ? most : sm_count());
-  if (out_dtype == KMB_F32) return i8_launch<BN, float>(map_w, map_x, p, grid, s);
-  if (out_dtype == KMB_F16) return i8_launch<BN, __half>(map_w, map_x, p, grid, s);
-  return i8_launch<BN, __nv_bfloat16>(map_w, map_x, p, grid, s);
+  const int splits = i8_splits(most, p.d);
+  if (splits > 1) return i8_launch<BN, T, true>(map_w, map_x, p, (unsigned)(most * splits), splits, s);
+  return i8_launch<BN, T, false>(map_w, map_x, p, (unsigned)(most < sm_count() ? most : sm_count()), 1, s);
+}
+
+template <int BN>
+int i8_run(int out_dtype, const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, const I8Params& p,
+           cudaStream_t s) {
+  if (out_dtype == KMB_F32) return i8_run_as<BN, float>(a, lda, b, ldb, p, s);
+  if (out_dtype == KMB_F16) return i8_run_as<BN, __half>(a, lda, b, ldb, p, s);
+  return i8_run_as<BN, __nv_bfloat16>(a, lda, b, ldb, p, s);
 }
 
 }  // namespace kmb

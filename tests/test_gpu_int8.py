@@ -104,7 +104,8 @@ def _check(out, want, size):
 
 @pytest.mark.parametrize("m,n,d", [(1, 1, 1), (1, 128, 16), (2, 300, 31), (15, 7, 32), (16, 129, 33), (17, 128, 127), (33, 200, 128),
                                    (64, 127, 129), (65, 256, 255), (128, 130, 1000), (130, 64, 96), (257, 300, 160), (300, 512, 64),
-                                   (513, 129, 2049), (1, 4096, 4096), (2000, 1500, 272)])
+                                   (513, 129, 2049), (1, 4096, 4096), (2000, 1500, 272), (300, 200, 3000),
+                                   (100, 256, 2100), (33, 128, 5000), (20, 1000, 600)])
 @pytest.mark.parametrize("out", TYPES)
 def test_product_sizes(m, n, d, out):
     from sklearn_numba_dpex_b200.common import int8_matmul
@@ -166,7 +167,8 @@ def _group_offsets(kind, g, m, rng):
 
 
 @pytest.mark.parametrize("g,m,n,d", [(1, 5, 20, 40), (3, 50, 129, 64), (8, 333, 200, 100), (64, 300, 70, 144), (40, 3000, 130, 48),
-                                     (255, 700, 16, 32), (1024, 2048, 9, 16), (1023, 10, 9, 17), (4, 4000, 64, 272)])
+                                     (255, 700, 16, 32), (1024, 2048, 9, 16), (1023, 10, 9, 17), (4, 4000, 64, 272),
+                                     (4, 40, 130, 2048), (2, 300, 256, 4096), (3, 200, 100, 1500)])
 @pytest.mark.parametrize("kind", ["whole", "tail", "empty", "one"])
 def test_product_by_group(g, m, n, d, kind):
     from sklearn_numba_dpex_b200.common import int8_matmul
@@ -255,10 +257,10 @@ CHILD = textwrap.dedent("""
     from sklearn_numba_dpex_b200._cabi import KmbError
     from sklearn_numba_dpex_b200.common import check_int8_waits, int8_matmul
 
-    m = int(sys.argv[1])
+    m, n, d = (int(v) for v in sys.argv[1:])
     g = torch.Generator(device="cuda").manual_seed(5)
-    a = torch.randint(-128, 128, (m, 256), device="cuda", generator=g, dtype=torch.int8)
-    b = torch.randint(-128, 128, (148 * 128 * 3, 256), device="cuda", generator=g, dtype=torch.int8)   # three tiles per CTA
+    a = torch.randint(-128, 128, (m, d), device="cuda", generator=g, dtype=torch.int8)
+    b = torch.randint(-128, 128, (n, d), device="cuda", generator=g, dtype=torch.int8)
     sa, sb = torch.ones(m, device="cuda"), torch.ones(b.shape[0], device="cuda")
     want = int8_matmul(a, sa, b, sb, out_dtype=torch.float32)
     check_int8_waits()
@@ -282,10 +284,12 @@ CHILD = textwrap.dedent("""
 """)
 
 
-@pytest.mark.parametrize("m", [1, 20, 40, 100, 256])
-def test_wait_that_runs_out_is_reported_and_the_context_survives(m):
-    """No GPU fault is involved: the loading warp stops after its first tile, the others give up after 200 ms."""
-    proc = subprocess.run([sys.executable, "-c", CHILD, str(m)], cwd=ROOT, capture_output=True, text=True, timeout=600)
+# three tiles per CTA, and few tiles that clusters of CTAs share
+@pytest.mark.parametrize("m,n,d", [(1, 56832, 256), (20, 56832, 256), (40, 56832, 256), (100, 56832, 256), (256, 56832, 256),
+                                   (1, 4096, 4096), (100, 300, 3000), (256, 256, 2048)])
+def test_wait_that_runs_out_is_reported_and_the_context_survives(m, n, d):
+    """No GPU fault is involved: the loading warp stops early, the others give up after 200 ms."""
+    proc = subprocess.run([sys.executable, "-c", CHILD, str(m), str(n), str(d)], cwd=ROOT, capture_output=True, text=True, timeout=600)
     tail = (proc.stdout + proc.stderr)[-3000:]
     assert proc.returncode == 0, tail
     assert "stall-ok" in proc.stdout, tail
