@@ -198,6 +198,11 @@ int quantize_run(const T* x, int64_t n, int d, const int32_t* rows, int64_t m, i
 // MMAs of the next.  (With four storing warps a tile of 256 tokens and 2056 features took longer to store
 // than to multiply: 88 us for 16 396 rows of 32 groups and 1408 outputs.)
 //
+// PAIR: many wide tiles.  Two CTAs multiply 256 features by BN tokens with one instruction
+// (cta_group::2); each loads its own 128 features and HALF of the tokens, 32 KB a stage instead of 48.  One
+// CTA alone asks for 94 bytes a cycle to keep its tensor core busy and an SM receives 64 from L2: 8192 x 8192 x
+// 4096 took 192 us that way, at 16.7 TB/s from L2 and 61 bytes a cycle and SM.
+//
 // SPLIT: few tiles.  A cluster of CTAs shares a tile, each summing a run of the contraction, so that more
 // SMs stream weights; the int32 partial sums meet through distributed shared memory, exactly, and each
 // CTA stores a share of the tokens.  A cluster has one tile at most.
@@ -209,35 +214,40 @@ constexpr int I8_SCAN_THREADS = 256;
 constexpr int I8_MAX_GROUPS = 1024;
 constexpr long long I8_TIMEOUT_CYCLES = 4000000000LL;   // ~2 s at 2 GHz
 
-template <int BN>
+enum I8Mode { I8_SINGLE, I8_SPLIT, I8_PAIR };
+
+template <int BN, I8Mode MODE>
 struct I8Cfg {
-  static constexpr int A_BYTES = I8_BM * I8_KB, B_BYTES = BN * I8_KB;
+  static constexpr int CTAS = MODE == I8_PAIR ? 2 : 1;          // that one instruction spans
+  static constexpr int A_BYTES = I8_BM * I8_KB, B_BYTES = BN / CTAS * I8_KB;
   static constexpr int FIT = (212 * 1024) / (A_BYTES + B_BYTES);
   static constexpr int STAGES = FIT > 12 ? 12 : FIT;
   static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
   static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) |
-                                    ((uint32_t)(I8_BM >> 4) << 24);   // int32 += s8 * s8, both K-major
+                                    ((uint32_t)(CTAS * I8_BM >> 4) << 24);   // int32 += s8 * s8, K-major
 };
 
-template <int BN>
+template <int BN, I8Mode MODE>
 struct I8Smem {
-  unsigned char a[I8Cfg<BN>::STAGES][I8Cfg<BN>::A_BYTES];
-  unsigned char b[I8Cfg<BN>::STAGES][I8Cfg<BN>::B_BYTES];
+  typedef I8Cfg<BN, MODE> Cfg;
+  unsigned char a[Cfg::STAGES][Cfg::A_BYTES];
+  unsigned char b[Cfg::STAGES][Cfg::B_BYTES];
   int first_tile[I8_MAX_GROUPS + 1];   // tiles before each group
   int scan[I8_SCAN_THREADS / 32];
   float sa[BN];
   int bad;                             // SPLIT: this CTA's partial sums are not to be used
-  unsigned long long full[I8Cfg<BN>::STAGES], empty[I8Cfg<BN>::STAGES];
+  unsigned long long full[Cfg::STAGES], empty[Cfg::STAGES];
   unsigned long long acc_full[2], acc_empty[2], drain;
   long long timeout_cycles;
   unsigned int tmem_base;
   volatile int abort_flag;
 };
-static_assert(sizeof(I8Smem<256>) + 1024 <= 232448, "I8Smem exceeds the 227 KB a CTA may use");
-static_assert(sizeof(I8Smem<128>) + 1024 <= 232448, "I8Smem exceeds the 227 KB a CTA may use");
-static_assert(sizeof(I8Smem<64>) + 1024 <= 232448, "I8Smem exceeds the 227 KB a CTA may use");
-static_assert(sizeof(I8Smem<32>) + 1024 <= 232448, "I8Smem exceeds the 227 KB a CTA may use");
-static_assert(sizeof(I8Smem<16>) + 1024 <= 232448, "I8Smem exceeds the 227 KB a CTA may use");
+constexpr size_t I8_SMEM_LIMIT = 232448 - 1024;      // 227 KB, less the alignment of the stages
+static_assert(sizeof(I8Smem<256, I8_PAIR>) <= I8_SMEM_LIMIT && sizeof(I8Smem<128, I8_PAIR>) <= I8_SMEM_LIMIT &&
+                  sizeof(I8Smem<256, I8_SINGLE>) <= I8_SMEM_LIMIT && sizeof(I8Smem<128, I8_SINGLE>) <= I8_SMEM_LIMIT &&
+                  sizeof(I8Smem<64, I8_SINGLE>) <= I8_SMEM_LIMIT && sizeof(I8Smem<32, I8_SINGLE>) <= I8_SMEM_LIMIT &&
+                  sizeof(I8Smem<16, I8_SINGLE>) <= I8_SMEM_LIMIT,
+              "the stages exceed the 227 KB a CTA may use");
 
 struct I8Params {
   const float* sa;
@@ -252,16 +262,36 @@ struct I8Params {
   int test_stall;             // test hook: the loading warp stops after its first tile
 };
 
+__device__ __forceinline__ bool mbar_try_wait_cluster(void* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Address that `p` has in the shared memory of CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t address_in(const void* p, uint32_t rank) {
+  uint32_t addr;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
+  return addr;
+}
+
 // Raised by a wait that ran out, on the GPU that ran it; read and cleared by kmb_int8_wait_error.
 static __device__ int g_i8_wait_error;
 
-template <typename Smem>
+// REMOTE: the other CTA of a pair arrives there too.
+template <bool REMOTE = false, typename Smem>
 __device__ __forceinline__ bool i8_wait(void* bar, uint32_t parity, Smem* sm) {
-  if (mbar_try_wait(bar, parity)) return true;
+  const auto done = [&] { return REMOTE ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+  if (done()) return true;
   const long long t0 = clock64();
   while (true) {
     for (int i = 0; i < 64; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
+      if (done()) return true;
     if (sm->abort_flag) return false;
     if (clock64() - t0 > sm->timeout_cycles) {
       sm->abort_flag = 1;
@@ -269,6 +299,43 @@ __device__ __forceinline__ bool i8_wait(void* bar, uint32_t parity, Smem* sm) {
       return false;
     }
   }
+}
+
+// The forms that span the two CTAs of a pair: tensor memory in both, loads that report to CTA 0's barrier, the
+// product, and completion that arrives at the same place in both.
+__device__ __forceinline__ void pair_tmem_alloc(void* smem_dst, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_dst)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void pair_tma_load(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar0) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar0), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void pair_umma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pair_commit(void* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t remote_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_bar) : "memory");
 }
 
 __device__ __forceinline__ void umma_i8_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
@@ -306,8 +373,10 @@ struct I8Tile {
   int feature0;
 };
 
+// `wide`: features of a tile; `skip`: where this CTA's 128 of them begin.
 template <int BN>
-__device__ __forceinline__ I8Tile i8_tile(const I8Params& p, const int* first_tile, int t) {
+__device__ __forceinline__ I8Tile i8_tile(const I8Params& p, const int* first_tile, int t, int wide = I8_BM,
+                                          int skip = 0) {
   int lo = 0, hi = p.groups;                 // last group with first_tile[g] <= t
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -317,7 +386,7 @@ __device__ __forceinline__ I8Tile i8_tile(const I8Params& p, const int* first_ti
   I8Tile r;
   r.g = lo;
   const int mt = local / p.feature_tiles;
-  r.feature0 = (local - mt * p.feature_tiles) * I8_BM;
+  r.feature0 = (local - mt * p.feature_tiles) * wide + skip;
   const int64_t start = i8_row_of(p, lo);
   r.row0 = start + (int64_t)mt * BN;
   const int64_t left = i8_row_of(p, lo + 1) - r.row0;
@@ -340,10 +409,8 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 // A word of the shared memory of CTA `rank` of the cluster, at the place `p` has in this one's.
 __device__ __forceinline__ int load_from(const void* p, uint32_t rank) {
-  uint32_t addr;
   int v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(address_in(p, rank)) : "memory");
   return v;
 }
 
@@ -358,17 +425,21 @@ __device__ __forceinline__ void i8_store(const uint32_t (&v)[COLS], const float*
   }
 }
 
-template <int BN, typename T, bool SPLIT>
+template <int BN, typename T, I8Mode MODE>
 __global__ void __launch_bounds__(I8_THREADS, 1)
 int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const __grid_constant__ I8Params p) {
-  using Cfg = I8Cfg<BN>;
+  using Cfg = I8Cfg<BN, MODE>;
+  constexpr bool SPLIT = MODE == I8_SPLIT, PAIR = MODE == I8_PAIR;
   extern __shared__ __align__(16) unsigned char i8_dyn[];
-  I8Smem<BN>* sm = reinterpret_cast<I8Smem<BN>*>(((uintptr_t)i8_dyn + 1023) & ~(uintptr_t)1023);
+  I8Smem<BN, MODE>* sm = reinterpret_cast<I8Smem<BN, MODE>*>(((uintptr_t)i8_dyn + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = SPLIT ? (int)cluster_size() : 1, split = SPLIT ? (int)cluster_rank() : 0;
-  const int first = SPLIT ? blockIdx.x / splits : blockIdx.x;    // this CTA's (or cluster's) first tile
-  const int step = SPLIT ? gridDim.x / splits : gridDim.x;
+  const int in_pair = PAIR ? (int)cluster_rank() : 0;            // CTA 0 of a pair issues its products
+  const int per_tile = PAIR ? 2 : splits;                        // CTAs that work on a tile
+  const int first = blockIdx.x / per_tile;                       // this CTA's (or cluster's) first tile
+  const int step = gridDim.x / per_tile;
+  const int wide = PAIR ? 2 * I8_BM : I8_BM, skip = in_pair * I8_BM;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::STAGES; ++s) {
@@ -377,7 +448,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sm->acc_full[b], 1);
-      mbar_init(&sm->acc_empty[b], I8_EPI_WARPS);
+      mbar_init(&sm->acc_empty[b], Cfg::CTAS * I8_EPI_WARPS);
     }
     mbar_init(&sm->drain, 1);
     sm->timeout_cycles = p.timeout_cycles;
@@ -386,8 +457,12 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     fence_barrier_init();
   }
   if (warp == 2) {
-    tmem_alloc(&sm->tmem_base, Cfg::TMEM_COLS);
-    tmem_relinquish();
+    if (PAIR) {
+      pair_tmem_alloc(&sm->tmem_base, Cfg::TMEM_COLS);
+    } else {
+      tmem_alloc(&sm->tmem_base, Cfg::TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   // what came before on the stream is not waited for until here: the set-up above overlaps it
   grid_dependency_wait();
@@ -433,7 +508,12 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
   }
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) {
+    __syncwarp();
+    cluster_sync();        // the barriers of both CTAs are set up
+  } else {
+    __syncthreads();
+  }
   tc_fence_after();
   const uint32_t tmem_base = sm->tmem_base;
   const int tiles = sm->first_tile[p.groups];
@@ -448,7 +528,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       uint32_t it = 0;
       bool ok = true;
       for (int t = first; t < tiles && ok; t += step) {
-        const I8Tile tile = i8_tile<BN>(p, sm->first_tile, t);
+        const I8Tile tile = i8_tile<BN>(p, sm->first_tile, t, wide, skip);
         const int w_row = tile.g * p.n + tile.feature0;
         for (int c = c_begin; c < c_end; ++c, ++it) {
           const uint32_t s = it % Cfg::STAGES, lap = it / Cfg::STAGES;
@@ -456,9 +536,17 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             ok = false;
             break;
           }
-          mbar_expect_tx(&sm->full[s], Cfg::A_BYTES + Cfg::B_BYTES);
-          tma_load_2d(sm->a[s], &map_w, c * I8_KB, w_row, &sm->full[s]);
-          tma_load_2d(sm->b[s], &map_x, c * I8_KB, (int)tile.row0, &sm->full[s]);
+          if (PAIR) {
+            // both CTAs' bytes count at CTA 0's barrier; its phase needs CTA 0's own arrival as well
+            if (in_pair == 0) mbar_expect_tx(&sm->full[s], 2 * (Cfg::A_BYTES + Cfg::B_BYTES));
+            const uint32_t full0 = address_in(&sm->full[s], 0);
+            pair_tma_load(sm->a[s], &map_w, c * I8_KB, w_row, full0);
+            pair_tma_load(sm->b[s], &map_x, c * I8_KB, (int)tile.row0 + in_pair * (BN / 2), full0);
+          } else {
+            mbar_expect_tx(&sm->full[s], Cfg::A_BYTES + Cfg::B_BYTES);
+            tma_load_2d(sm->a[s], &map_w, c * I8_KB, w_row, &sm->full[s]);
+            tma_load_2d(sm->b[s], &map_x, c * I8_KB, (int)tile.row0, &sm->full[s]);
+          }
           if (p.test_stall && c == c_end - 1 - SPLIT) ok = false;
           if (!ok) {
             ++it;
@@ -466,9 +554,11 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
           }
         }
       }
-      if (sm->abort_flag) drain_ring(sm->full, Cfg::STAGES, it);
+      // (CTA 0 of a pair waits for both CTAs' copies, as far as it issued its own; the other one does not
+      // leave before it)
+      if (sm->abort_flag && in_pair == 0) drain_ring(sm->full, Cfg::STAGES, it);
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 && in_pair == 0) {
     // ------------------------------------------------------------------------- MMAs
     const uint64_t a0 = make_sdesc(smem_u32(sm->a[0])), b0 = make_sdesc(smem_u32(sm->b[0]));
     const int last_steps = ((p.d - (all_chunks - 1) * I8_KB) + 31) / 32;   // 32 features per instruction
@@ -476,7 +566,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     bool ok = true;
     for (int t = first; t < tiles && ok; t += step, ++nt) {
       const uint32_t ab = nt & 1u;
-      if (!__all_sync(0xffffffffu, i8_wait(&sm->acc_empty[ab], ((nt >> 1) & 1u) ^ 1u, sm))) break;
+      if (!__all_sync(0xffffffffu, i8_wait<PAIR>(&sm->acc_empty[ab], ((nt >> 1) & 1u) ^ 1u, sm))) break;
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + ab * BN;
       for (int c = c_begin; c < c_end; ++c, ++it) {
@@ -491,14 +581,30 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
           const uint64_t bd = b0 + (uint64_t)(s * (Cfg::B_BYTES >> 4));
           const int steps = c == all_chunks - 1 ? last_steps : 4;
           for (int ks = 0; ks < steps; ++ks)
-            umma_i8_ss(d_tmem, ad + 2 * ks, bd + 2 * ks, Cfg::IDESC, (c > c_begin || ks > 0) ? 1u : 0u);
-          umma_commit(&sm->empty[s]);
-          if (c == c_end - 1) umma_commit(&sm->acc_full[ab]);
+            if (PAIR) pair_umma_i8(d_tmem, ad + 2 * ks, bd + 2 * ks, Cfg::IDESC, (c > c_begin || ks > 0) ? 1u : 0u);
+            else umma_i8_ss(d_tmem, ad + 2 * ks, bd + 2 * ks, Cfg::IDESC, (c > c_begin || ks > 0) ? 1u : 0u);
+          if (PAIR) {
+            pair_commit(&sm->empty[s]);
+            if (c == c_end - 1) pair_commit(&sm->acc_full[ab]);
+          } else {
+            umma_commit(&sm->empty[s]);
+            if (c == c_end - 1) umma_commit(&sm->acc_full[ab]);
+          }
         }
         __syncwarp();
       }
     }
-    if (sm->abort_flag) mma_drain(&sm->drain);
+    if (sm->abort_flag) {
+      if (PAIR) {
+        if (elect_one()) {
+          pair_commit(&sm->drain);
+          drain_wait(&sm->drain, 0u);
+        }
+        __syncwarp();
+      } else {
+        mma_drain(&sm->drain);
+      }
+    }
   } else if (warp >= 4) {
     // --------------------------------------------------------------- scales and stores
     const int q = warp & 3, half = (warp - 4) >> 2;
@@ -518,8 +624,9 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const int col0 = BN >= 32 ? half * MINE : 0;
     const bool works = BN >= 32 || half == 0;
     uint32_t nt = 0;
+    bool ok = true;        // no wait has run out; one that did says nothing about the phases after it
     for (int t = first; t < tiles; t += step, ++nt) {
-      const I8Tile tile = i8_tile<BN>(p, sm->first_tile, t);
+      const I8Tile tile = i8_tile<BN>(p, sm->first_tile, t, wide, skip);
       const uint32_t ab = nt & 1u;
       asm volatile("bar.sync 1, 256;" ::: "memory");   // everybody is done with the last tile's scales
       for (int r = etid; r < BN; r += EPI) sm->sa[r] = r < tile.rows ? p.sa[tile.row0 + r] : 0.f;
@@ -529,7 +636,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       float sb = mine ? p.sb[wrow] : 0.f;
       const float bias = (mine && p.bias) ? p.bias[wrow] : 0.f;
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      const bool ok = __all_sync(0xffffffffu, i8_wait(&sm->acc_full[ab], (nt >> 1) & 1u, sm));
+      ok = ok && __all_sync(0xffffffffu, i8_wait(&sm->acc_full[ab], (nt >> 1) & 1u, sm));
       tc_fence_after();
       const uint32_t acc = tmem_base + ab * BN + ((uint32_t)(q * 32) << 16);
       if (SPLIT) {
@@ -564,11 +671,17 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm->acc_empty[ab]);
+      if (lane == 0) {
+        if (PAIR) arrive_at(address_in(&sm->acc_empty[ab], 0));
+        else mbar_arrive(&sm->acc_empty[ab]);
+      }
     }
   }
   tc_fence_before();
-  if (SPLIT) {
+  if (PAIR) {
+    __syncwarp();
+    cluster_sync();        // nothing of either CTA is in the other's hands any more
+  } else if (SPLIT) {
     __syncwarp();
     cluster_sync();        // every partial sum of the cluster lies in shared memory
     if (warp >= 4 && first < tiles) {
@@ -597,7 +710,8 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   }
   if (warp == 2) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+    if (PAIR) pair_tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+    else tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
   }
 }
 
@@ -623,13 +737,13 @@ static int i8_make_map(CUtensorMap* map, const int8_t* base, int64_t rows, int d
   return KMB_OK;
 }
 
-template <int BN, typename T, bool SPLIT>
-int i8_launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const I8Params& p, unsigned grid,
-              int splits, cudaStream_t s) {
-  const int smem = (int)sizeof(I8Smem<BN>) + 1024;
-  const auto kernel = int8_matmul_kernel<BN, T, SPLIT>;
+template <int BN, typename T, I8Mode MODE>
+int i8_launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const I8Params& p, int64_t grid,
+              int cluster, cudaStream_t s) {
+  const int smem = (int)sizeof(I8Smem<BN, MODE>) + 1024;
+  const auto kernel = int8_matmul_kernel<BN, T, MODE>;
   KMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  return launch_early(kernel, grid, I8_THREADS, smem, splits, s, map_w, map_x, p);
+  return launch_early(kernel, (unsigned)grid, I8_THREADS, smem, cluster, s, map_w, map_x, p);
 }
 
 // CTAs that share a tile: as many as the SMs allow, while each has two stages' worth of the contraction
@@ -643,17 +757,27 @@ static int i8_splits(int64_t tiles, int d) {
 
 template <int BN, typename T>
 int i8_run_as(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, I8Params p, cudaStream_t s) {
+  // an upper bound of the tiles: every group may end inside one
+  const int64_t token_tiles = ceil_div(p.m, BN) + p.groups - 1;
+  const int64_t most = token_tiles * ceil_div(p.n, I8_BM);
+  KMB_REQUIRE(most < (1ll << 31), "kmb_int8_matmul: too many output tiles");
+  const int sms = sm_count(), splits = i8_splits(most, p.d);
+  // pairs where there is a wide tile for each of them
+  const bool pairs = BN >= 128 && p.n > I8_BM && token_tiles * ceil_div(p.n, 2 * I8_BM) >= sms / 2;
   CUtensorMap map_w, map_x;
   int rc = i8_make_map(&map_w, b, (int64_t)p.groups * p.n, p.d, ldb, I8_BM);
   if (rc != KMB_OK) return rc;
-  rc = i8_make_map(&map_x, a, p.m, p.d, lda, BN);
+  rc = i8_make_map(&map_x, a, p.m, p.d, lda, pairs ? BN / 2 : BN);
   if (rc != KMB_OK) return rc;
-  // an upper bound of the tiles: every group may end inside one
-  const int64_t most = (ceil_div(p.m, BN) + p.groups - 1) * p.feature_tiles;
-  KMB_REQUIRE(most < (1ll << 31), "kmb_int8_matmul: too many output tiles");
-  const int splits = i8_splits(most, p.d);
-  if (splits > 1) return i8_launch<BN, T, true>(map_w, map_x, p, (unsigned)(most * splits), splits, s);
-  return i8_launch<BN, T, false>(map_w, map_x, p, (unsigned)(most < sm_count() ? most : sm_count()), 1, s);
+  if constexpr (BN >= 128) {
+    if (pairs) {
+      p.feature_tiles = (int)ceil_div(p.n, 2 * I8_BM);
+      return i8_launch<BN, T, I8_PAIR>(map_w, map_x, p, sms / 2 * 2, 2, s);
+    }
+  }
+  p.feature_tiles = (int)ceil_div(p.n, I8_BM);
+  if (splits > 1) return i8_launch<BN, T, I8_SPLIT>(map_w, map_x, p, most * splits, splits, s);
+  return i8_launch<BN, T, I8_SINGLE>(map_w, map_x, p, most < sms ? most : sms, 1, s);
 }
 
 template <int BN>
@@ -708,7 +832,6 @@ int kmb_int8_matmul(int out_dtype, const int8_t* a, int64_t lda, const float* a_
   p.groups = groups;
   p.n = n;
   p.d = d;
-  p.feature_tiles = (int)ceil_div(n, I8_BM);
   const char* e = getenv("KMB_TC_TIMEOUT_MS");
   const long ms = e ? atol(e) : 0;
   p.timeout_cycles = ms > 0 ? ms * 2000000LL : I8_TIMEOUT_CYCLES;

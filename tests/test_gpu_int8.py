@@ -105,7 +105,8 @@ def _check(out, want, size):
 @pytest.mark.parametrize("m,n,d", [(1, 1, 1), (1, 128, 16), (2, 300, 31), (15, 7, 32), (16, 129, 33), (17, 128, 127), (33, 200, 128),
                                    (64, 127, 129), (65, 256, 255), (128, 130, 1000), (130, 64, 96), (257, 300, 160), (300, 512, 64),
                                    (513, 129, 2049), (1, 4096, 4096), (2000, 1500, 272), (300, 200, 3000),
-                                   (100, 256, 2100), (33, 128, 5000), (20, 1000, 600)])
+                                   (100, 256, 2100), (33, 128, 5000), (20, 1000, 600),
+                                   (5000, 1000, 400), (4000, 2700, 136), (100, 19000, 130), (2561, 1921, 1300)])
 @pytest.mark.parametrize("out", TYPES)
 def test_product_sizes(m, n, d, out):
     from sklearn_numba_dpex_b200.common import int8_matmul
@@ -168,7 +169,8 @@ def _group_offsets(kind, g, m, rng):
 
 @pytest.mark.parametrize("g,m,n,d", [(1, 5, 20, 40), (3, 50, 129, 64), (8, 333, 200, 100), (64, 300, 70, 144), (40, 3000, 130, 48),
                                      (255, 700, 16, 32), (1024, 2048, 9, 16), (1023, 10, 9, 17), (4, 4000, 64, 272),
-                                     (4, 40, 130, 2048), (2, 300, 256, 4096), (3, 200, 100, 1500)])
+                                     (4, 40, 130, 2048), (2, 300, 256, 4096), (3, 200, 100, 1500), (5, 5000, 700, 400),
+                                     (20, 2500, 1100, 150)])
 @pytest.mark.parametrize("kind", ["whole", "tail", "empty", "one"])
 def test_product_by_group(g, m, n, d, kind):
     from sklearn_numba_dpex_b200.common import int8_matmul
@@ -286,7 +288,8 @@ CHILD = textwrap.dedent("""
 
 # three tiles per CTA, and few tiles that clusters of CTAs share
 @pytest.mark.parametrize("m,n,d", [(1, 56832, 256), (20, 56832, 256), (40, 56832, 256), (100, 56832, 256), (256, 56832, 256),
-                                   (1, 4096, 4096), (100, 300, 3000), (256, 256, 2048)])
+                                   (1, 4096, 4096), (100, 300, 3000), (256, 256, 2048), (700, 16000, 300), (128, 58000, 300),
+                                   (16, 148 * 128 * 7, 128)])
 def test_wait_that_runs_out_is_reported_and_the_context_survives(m, n, d):
     """No GPU fault is involved: the loading warp stops early, the others give up after 200 ms."""
     proc = subprocess.run([sys.executable, "-c", CHILD, str(m), str(n), str(d)], cwd=ROOT, capture_output=True, text=True, timeout=600)
