@@ -4,6 +4,7 @@
 // top-k of topk.cu and keeps its order (greatest first, lowest index among equals, NaN greatest).
 #include <limits.h>
 
+#include "early_launch.cuh"
 #include "kmb_common.cuh"
 #include "row_types.cuh"
 
@@ -332,6 +333,8 @@ __global__ void __launch_bounds__(RT_WARPS * 32)
 route_topk_kernel(const __grid_constant__ RouteParams p) {
   // groups: one row of keys per warp, wide enough for 64-bit keys
   extern __shared__ __align__(16) float s_route[];
+  next_grid_may_start();
+  grid_dependency_wait();
   constexpr int PER = 32 / L;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (L - 1);
   float* s_keys = s_route + (size_t)warp * 2 * p.n_experts;
@@ -387,6 +390,8 @@ struct RouteGradParams {
 template <typename T, int L, int V>
 __global__ void __launch_bounds__(RT_WARPS * 32)
 route_topk_grad_kernel(const __grid_constant__ RouteGradParams p) {
+  next_grid_may_start();
+  grid_dependency_wait();
   constexpr int PER = 32 / L;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (L - 1), e0 = sub * V;
   const bool dense = !p.sigmoid && !p.renormalize;
@@ -483,25 +488,20 @@ int route_run(RouteParams p, cudaStream_t s) {
   const size_t smem = p.groups > 1 ? (size_t)RT_WARPS * 2 * p.n_experts * sizeof(float) : 0;
 #define KMB_RUN(L, V)                                                                           \
   p.vec = route_rows_are_vec<T>(p.logits, nullptr, p.n_experts, V);                             \
-  if (p.bias == nullptr && p.groups == 1)                                                       \
-    route_topk_kernel<T, L, V, true><<<route_grid(p.n, L), RT_WARPS * 32, 0, s>>>(p);           \
-  else                                                                                          \
-    route_topk_kernel<T, L, V, false><<<route_grid(p.n, L), RT_WARPS * 32, smem, s>>>(p)
+  return launch_early(p.bias == nullptr && p.groups == 1 ? route_topk_kernel<T, L, V, true>     \
+                                                         : route_topk_kernel<T, L, V, false>,   \
+                      route_grid(p.n, L), RT_WARPS * 32, smem, 1, s, p)
   KMB_ROUTE_WIDTHS(p.groups > 1, KMB_RUN);
 #undef KMB_RUN
-  KMB_CHECK_LAUNCH();
-  return KMB_OK;
 }
 
 template <typename T>
 int route_grad_run(RouteGradParams p, cudaStream_t s) {
 #define KMB_RUN(L, V)                                                                           \
   p.vec = route_rows_are_vec<T>(p.logits, p.grad_logits, p.n_experts, V);                       \
-  route_topk_grad_kernel<T, L, V><<<route_grid(p.n, L), RT_WARPS * 32, 0, s>>>(p)
+  return launch_early(route_topk_grad_kernel<T, L, V>, route_grid(p.n, L), RT_WARPS * 32, 0, 1, s, p)
   KMB_ROUTE_WIDTHS(false, KMB_RUN);
 #undef KMB_RUN
-  KMB_CHECK_LAUNCH();
-  return KMB_OK;
 }
 
 // ============================================================================= expert order
@@ -520,6 +520,8 @@ __global__ void __launch_bounds__(SL_THREADS)
 slots_count_kernel(const int32_t* __restrict__ experts, int64_t total, int n_experts,
                    int32_t* __restrict__ counts) {
   __shared__ int32_t s_cnt[SL_MAX_EXPERTS];
+  next_grid_may_start();
+  grid_dependency_wait();
   for (int e = threadIdx.x; e < n_experts; e += SL_THREADS) s_cnt[e] = 0;
   __syncthreads();
   const int64_t first = (int64_t)blockIdx.x * SL_CHUNK;
@@ -540,6 +542,8 @@ constexpr int SC_RUN = 8;
 __global__ void __launch_bounds__(1024)
 slots_scan_kernel(int32_t* __restrict__ counts, int chunks, int n_experts, int32_t* __restrict__ totals) {
   __shared__ int32_t s_sum[32][33];
+  next_grid_may_start();
+  grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = blockIdx.x * 32 + lane;
   const bool mine = e < n_experts;
   int carry = 0;
@@ -593,6 +597,8 @@ slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, in
   __shared__ int32_t s_count;
   __shared__ int2 s_scan[SL_WARPS];
   __shared__ int32_t s_end;
+  next_grid_may_start();
+  grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t first = (int64_t)blockIdx.x * SL_CHUNK + warp * (SL_ROUNDS * 32);
 
@@ -698,7 +704,7 @@ slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, in
 // ============================================================================= weighted sums
 // out[t] = sum_j w[t, j] values[slots[t, j]]; a slot outside [0, n_values) counts as none.
 constexpr int CB_THREADS = 256;   // at most; the launch takes as many as a row needs (combine_threads)
-constexpr int CB_K = 8;           // rows in flight per thread
+constexpr int CB_K = 8;           // rows that a thread asks for before it adds the first
 constexpr int CG_THREADS = 128, CG_K = 4;   // the gradients', which hold twice as much per row
 
 // Eight elements of a row as they lie in memory.  VEC: consecutive ones of a row of whole 16-byte pieces
@@ -744,12 +750,15 @@ struct RowPiece {
 
 // Bound by HBM: each thread has the pieces of up to CB_K rows in flight before it adds the first.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(CB_THREADS)
+__global__ void __maxnreg__(96)      // four blocks of 160 threads on an SM
 combine_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __restrict__ slots,
-               const float* __restrict__ weights, int k, int d, T* __restrict__ out) {
+               const float* __restrict__ weights, int k, int d, T* __restrict__ out, int parts) {
   typedef RowPiece<T, VEC> Piece;
-  const int64_t t = blockIdx.x;
-  for (int f0 = blockIdx.y * Piece::span(); f0 < d; f0 += gridDim.y * Piece::span()) {
+  next_grid_may_start();
+  grid_dependency_wait();
+  const int64_t t = blockIdx.x / (unsigned)parts;
+  const int part = (int)(blockIdx.x - t * parts);
+  for (int f0 = part * Piece::span(); f0 < d; f0 += parts * Piece::span()) {
     if (Piece::at(f0, 0) >= d) continue;
     float acc[8];
 #pragma unroll
@@ -782,8 +791,19 @@ combine_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __
 // Gradients.  A row of values that several choices share needs the sum of their gradients, in a fixed
 // order: `users` counts the choices of each row and `first` names the lowest of them.  The blocks of the
 // tokens write the rows with one user, the last blocks of the grid all others.
+__global__ void combine_clear_kernel(int64_t n_values, int32_t* __restrict__ users, int32_t* __restrict__ first) {
+  next_grid_may_start();
+  grid_dependency_wait();
+  const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (r >= n_values) return;
+  users[r] = 0;
+  first[r] = INT_MAX;
+}
+
 __global__ void combine_users_kernel(const int32_t* __restrict__ slots, int64_t total, int64_t n_values,
                                      int32_t* __restrict__ users, int32_t* __restrict__ first) {
+  next_grid_may_start();
+  grid_dependency_wait();
   const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= total) return;
   const int slot = slots[c];
@@ -792,57 +812,73 @@ __global__ void combine_users_kernel(const int32_t* __restrict__ slots, int64_t 
   atomicMin(&first[slot], (int32_t)c);
 }
 
-// Rows `r0`, r0 + step, ... that have no user or several: zeros, or the sum over the users, which are found
-// by walking the choices from the lowest of them on, a block's width at a time, and added in ascending order.
+// The rows that have no user or several: zeros, or the sum over the users, which are found by walking the
+// choices from the lowest of them on, a block's width at a time, and added in ascending order.  Block `block`
+// of `blocks` looks at as many rows at once as it has threads.
 template <typename T, bool VEC>
-__device__ __noinline__ void combine_other_rows(int64_t r0, int64_t step, int64_t n_values,
+__device__ __noinline__ void combine_other_rows(int64_t block, int64_t blocks, int64_t n_values,
                                                 const int32_t* __restrict__ slots, const float* __restrict__ weights,
                                                 const T* __restrict__ grad_out, int64_t choices, int k, int d,
                                                 const int32_t* __restrict__ users, const int32_t* __restrict__ first,
                                                 T* __restrict__ grad_values) {
   typedef RowPiece<T, VEC> Piece;
-  __shared__ int32_t list[CG_THREADS];
-  __shared__ int list_n[CG_THREADS / 32];
+  __shared__ int32_t list[CG_THREADS], other[CG_THREADS];
+  __shared__ int list_n[CG_THREADS / 32], other_n[CG_THREADS / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int64_t r = r0; r < n_values; r += step) {
-    const int count = users[r];
-    if (count == 1) continue;
-    for (int f0 = 0; f0 < d; f0 += Piece::span()) {
-      const bool in = Piece::at(f0, 0) < d;
-      float acc[8];
+  for (int64_t base = block * blockDim.x; base < n_values; base += blocks * blockDim.x) {
+    const int64_t mine = base + threadIdx.x;
+    const bool odd = mine < n_values && users[mine] != 1;
+    const unsigned odd_m = __ballot_sync(FULL, odd);
+    __syncthreads();
+    if (lane == 0) other_n[warp] = __popc(odd_m);
+    __syncthreads();
+    int place = 0, others = 0;
+    for (int q = 0; q < (int)blockDim.x / 32; ++q) {
+      if (q < warp) place += other_n[q];
+      others += other_n[q];
+    }
+    if (odd) other[place + __popc(odd_m & ((1u << lane) - 1u))] = (int32_t)threadIdx.x;
+    __syncthreads();
+    for (int o = 0; o < others; ++o) {
+      const int64_t r = base + other[o];
+      const int count = users[r];
+      for (int f0 = 0; f0 < d; f0 += Piece::span()) {
+        const bool in = Piece::at(f0, 0) < d;
+        float acc[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-      int left = count;
-      for (int64_t cb = count ? first[r] : choices; left > 0 && cb < choices; cb += blockDim.x) {
-        const int64_t c = cb + threadIdx.x;
-        const bool hit = c < choices && slots[c] == r;
-        const unsigned m = __ballot_sync(FULL, hit);
-        if (lane == 0) list_n[warp] = __popc(m);
-        __syncthreads();
-        int at = 0, found = 0;
-        for (int q = 0; q < (int)blockDim.x / 32; ++q) {
-          if (q < warp) at += list_n[q];
-          found += list_n[q];
-        }
-        if (hit) list[at + __popc(m & ((1u << lane) - 1u))] = (int32_t)(c - cb);
-        __syncthreads();
-        if (in)
-          for (int q = 0; q < found; ++q) {
-            const int64_t cc = cb + list[q];
-            const float w = weights[cc];
-            Piece g;
-            g.clear();
-            g.load(grad_out + (cc / k) * d, f0, d);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, to_float(g.t[i]), acc[i]);
+        for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+        int left = count;
+        for (int64_t cb = count ? first[r] : choices; left > 0 && cb < choices; cb += blockDim.x) {
+          const int64_t c = cb + threadIdx.x;
+          const bool hit = c < choices && slots[c] == r;
+          const unsigned m = __ballot_sync(FULL, hit);
+          if (lane == 0) list_n[warp] = __popc(m);
+          __syncthreads();
+          int at = 0, found = 0;
+          for (int q = 0; q < (int)blockDim.x / 32; ++q) {
+            if (q < warp) at += list_n[q];
+            found += list_n[q];
           }
-        left -= found;
-        __syncthreads();
-      }
-      Piece o;
+          if (hit) list[at + __popc(m & ((1u << lane) - 1u))] = (int32_t)(c - cb);
+          __syncthreads();
+          if (in)
+            for (int q = 0; q < found; ++q) {
+              const int64_t cc = cb + list[q];
+              const float w = weights[cc];
+              Piece g;
+              g.clear();
+              g.load(grad_out + (cc / k) * d, f0, d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o.t[i] = from_float<T>(acc[i]);
-      if (in) o.store(grad_values + r * d, f0, d);
+              for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, to_float(g.t[i]), acc[i]);
+            }
+          left -= found;
+          __syncthreads();
+        }
+        Piece o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o.t[i] = from_float<T>(acc[i]);
+        if (in) o.store(grad_values + r * d, f0, d);
+      }
     }
   }
 }
@@ -856,6 +892,8 @@ combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_
   typedef RowPiece<T, VEC> Piece;
   __shared__ float red[CG_THREADS / 32][CG_K];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  next_grid_may_start();
+  grid_dependency_wait();
   if ((int64_t)blockIdx.x >= token_blocks) {
     combine_other_rows<T, VEC>((int64_t)blockIdx.x - token_blocks, (int64_t)gridDim.x - token_blocks, n_values, slots,
                                weights, grad_out, n * k, k, d, users, first, grad_values);
@@ -863,22 +901,25 @@ combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_
   }
   // a block takes CG_K choices of a token
   const int parts = (k + CG_K - 1) / CG_K;
-  const int64_t t = blockIdx.x / parts;
+  const int64_t t = blockIdx.x / (unsigned)parts;
   const int j0 = (int)(blockIdx.x - t * parts) * CG_K;
   int slot[CG_K], used[CG_K];
+  bool there[CG_K];
   float w[CG_K], dot[CG_K];
 #pragma unroll
   for (int j = 0; j < CG_K; ++j) {
-    slot[j] = j0 + j < k ? slots[t * k + j0 + j] : -1;
-    if (slot[j] >= n_values) slot[j] = -1;
+    const int64_t c = t * k + (j0 + j < k ? j0 + j : k - 1);
+    slot[j] = slots[c];
+    w[j] = weights[c];
+    dot[j] = 0.f;
   }
 #pragma unroll
   for (int j = 0; j < CG_K; ++j) {
-    dot[j] = 0.f;
-    w[j] = slot[j] >= 0 ? weights[t * k + j0 + j] : 0.f;
-    used[j] = slot[j] >= 0 ? users[slot[j]] : 1;      // looked at when the first gradients are stored
+    there[j] = j0 + j < k && slot[j] >= 0 && slot[j] < n_values;
+    slot[j] = there[j] ? slot[j] : 0;
+    used[j] = n_values > 0 ? users[slot[j]] : 0;      // looked at when the first gradients are stored
   }
-  for (int f0 = 0; f0 < d; f0 += Piece::span()) {
+  for (int f0 = 0; f0 < d && n_values > 0; f0 += Piece::span()) {
     if (Piece::at(f0, 0) >= d) continue;
     Piece g, v[CG_K];
     g.clear();
@@ -886,11 +927,10 @@ combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_
 #pragma unroll
     for (int j = 0; j < CG_K; ++j) {
       v[j].clear();
-      if (slot[j] >= 0) v[j].load(values + (int64_t)slot[j] * d, f0, d);
+      if (there[j]) v[j].load(values + (int64_t)slot[j] * d, f0, d);
     }
 #pragma unroll
     for (int j = 0; j < CG_K; ++j) {
-      if (slot[j] < 0) continue;
       Piece o;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -898,13 +938,14 @@ combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_
         dot[j] = fmaf(to_float(v[j].t[i]), gi, dot[j]);
         o.t[i] = from_float<T>(w[j] * gi);
       }
-      if (used[j] == 1) o.store(grad_values + (int64_t)slot[j] * d, f0, d);
+      if (there[j] && used[j] == 1) o.store(grad_values + (int64_t)slot[j] * d, f0, d);
     }
   }
 #pragma unroll
   for (int j = 0; j < CG_K; ++j) {
     dot[j] = warp_sum_of(dot[j]);
-    if (lane == 0) red[warp][j] = dot[j];
+    // 0 where there is no row, whatever the gradient holds
+    if (lane == 0) red[warp][j] = there[j] ? dot[j] : 0.f;
   }
   __syncthreads();
   if (threadIdx.x < CG_K && j0 + threadIdx.x < k) {
@@ -1022,22 +1063,19 @@ int kmb_expert_slots(const int32_t* experts, int64_t n, int k, int n_experts, in
   const auto place = chunks <= 1 ? slots_place_kernel<true> : slots_place_kernel<false>;
   if (smem > 8 * 1024)
     KMB_CHECK_CUDA(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  if (chunks <= 1) {
-    slots_place_kernel<true><<<1, SL_THREADS, smem, s>>>(experts, total, k, n_experts, nullptr, nullptr, slots,
-                                                         rows, offsets);
-    KMB_CHECK_LAUNCH();
-    return KMB_OK;
-  }
+  if (chunks <= 1)
+    return launch_early(place, 1, SL_THREADS, smem, 1, s, experts, total, k, n_experts, nullptr, nullptr, slots, rows,
+                        offsets);
   int32_t* counts = (int32_t*)workspace;
   int32_t* totals = counts + (int64_t)chunks * n_experts;
-  slots_count_kernel<<<chunks, SL_THREADS, 0, s>>>(experts, total, n_experts, counts);
-  KMB_CHECK_LAUNCH();
-  slots_scan_kernel<<<(unsigned)ceil_div(n_experts, 32), 1024, 0, s>>>(counts, chunks, n_experts, totals);
-  KMB_CHECK_LAUNCH();
-  slots_place_kernel<false><<<chunks, SL_THREADS, smem, s>>>(experts, total, k, n_experts, counts, totals, slots,
-                                                             rows, offsets);
-  KMB_CHECK_LAUNCH();
-  return KMB_OK;
+  int rc = launch_early(slots_count_kernel, chunks, SL_THREADS, 0, 1, s, experts, total, n_experts, counts);
+  if (rc == KMB_OK)
+    rc = launch_early(slots_scan_kernel, (unsigned)ceil_div(n_experts, 32), 1024, 0, 1, s, counts, chunks, n_experts,
+                      totals);
+  if (rc == KMB_OK)
+    rc = launch_early(place, chunks, SL_THREADS, smem, 1, s, experts, total, k, n_experts, counts, totals, slots, rows,
+                      offsets);
+  return rc;
 }
 
 int kmb_combine_experts(int dtype, const void* values, int64_t n_values, const int32_t* slots,
@@ -1048,13 +1086,12 @@ int kmb_combine_experts(int dtype, const void* values, int64_t n_values, const i
   KMB_DISPATCH_ROWS(dtype, {
     const int vec = rows_are_vec((const T*)values, d) && rows_are_vec((const T*)out, d);
     const unsigned threads = combine_threads(d, CB_THREADS);
-    dim3 grid((unsigned)n, (unsigned)ceil_div(d, threads * 8));
-    if (grid.y > 65535) grid.y = 65535;
-    const auto kernel = vec ? combine_kernel<T, true> : combine_kernel<T, false>;
-    kernel<<<grid, threads, 0, (cudaStream_t)stream>>>((const T*)values, n_values, slots, weights, k, d, (T*)out);
-    KMB_CHECK_LAUNCH();
+    // long rows of few tokens are shared between blocks
+    const int64_t passes = ceil_div(d, threads * 8);
+    const int parts = n * passes <= (int64_t)sm_count() * 4 ? (int)passes : 1;
+    return launch_early(vec ? combine_kernel<T, true> : combine_kernel<T, false>, (unsigned)(n * parts), (int)threads, 0,
+                        1, (cudaStream_t)stream, (const T*)values, n_values, slots, weights, k, d, (T*)out, parts);
   });
-  return KMB_OK;
 }
 
 size_t kmb_combine_experts_grad_workspace_bytes(int64_t n_values) {
@@ -1079,26 +1116,25 @@ int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, co
   int32_t* users = (int32_t*)workspace;
   int32_t* first = users + n_values;
   if (n_values > 0) {
-    KMB_CHECK_CUDA(cudaMemsetAsync(users, 0, (size_t)n_values * sizeof(int32_t), s));
-    KMB_CHECK_CUDA(cudaMemsetAsync(first, 0x7f, (size_t)n_values * sizeof(int32_t), s));
+    const int rc = launch_early(combine_clear_kernel, (unsigned)ceil_div(n_values, 256), 256, 0, 1, s, n_values, users,
+                                first);
+    if (rc != KMB_OK) return rc;
   }
   if (n > 0) {
-    combine_users_kernel<<<(unsigned)ceil_div(n * k, 256), 256, 0, s>>>(slots, n * k, n_values, users, first);
-    KMB_CHECK_LAUNCH();
+    const int rc = launch_early(combine_users_kernel, (unsigned)ceil_div(n * k, 256), 256, 0, 1, s, slots, n * k,
+                                n_values, users, first);
+    if (rc != KMB_OK) return rc;
   }
   KMB_DISPATCH_ROWS(dtype, {
     const int vec = rows_are_vec((const T*)values, d) && rows_are_vec((const T*)grad_out, d) &&
                     rows_are_vec((const T*)grad_values, d);
     const int64_t fill = n_values == 0 ? 0 : (ceil_div(n_values, 64) < sm_count() ? ceil_div(n_values, 64) : sm_count());
-    const auto kernel = vec ? combine_grad_kernel<T, true> : combine_grad_kernel<T, false>;
     const unsigned threads = combine_threads(d, CG_THREADS);
     const int64_t token_blocks = n * ceil_div(k, CG_K);
-    kernel<<<(unsigned)(token_blocks + fill), threads, 0, s>>>((const T*)values, n_values, slots, weights,
-                                                               (const T*)grad_out, n, k, d, users, first,
-                                                               (T*)grad_values, grad_weights, token_blocks);
-    KMB_CHECK_LAUNCH();
+    return launch_early(vec ? combine_grad_kernel<T, true> : combine_grad_kernel<T, false>,
+                        (unsigned)(token_blocks + fill), (int)threads, 0, 1, s, (const T*)values, n_values, slots,
+                        weights, (const T*)grad_out, n, k, d, users, first, (T*)grad_values, grad_weights, token_blocks);
   });
-  return KMB_OK;
 }
 
 }  // extern "C"

@@ -27,12 +27,17 @@ namespace kmb {
 // with 16 pieces a lane had 12 warps on an SM and took 80 us for 8192 rows of 4096 bf16, a block of 256
 // with two pieces 32 us.)  The pieces stay in registers, as they lie in memory, between the maximum and the
 // rounding; rows longer than 8192 (VECS = 0) are read a second time, from L1 and L2.
-// The numbers of a piece in 64 bits, one at a time from memory: few pieces come here, and the registers of
-// the others are not indexed for their sake.
+// How near to the middle between two whole numbers a product is in doubt (see QrPiece::round).
+constexpr float QR_SURE = 0.49999f;
+
+// The numbers in doubt of a piece in 64 bits, one at a time from memory: one piece in 600 comes here, and
+// the registers of the others are not indexed for its sake.
 template <typename T>
-__device__ __noinline__ void quantize_exactly(const T* row, int f, int d, float top, int8_t* q) {
-  for (int j = 0; j < 8 && f + j < d; ++j)
-    q[f + j] = (int8_t)(int)rint((double)to_float(row[f + j]) * 127.0 / (double)top);
+__device__ __noinline__ void quantize_exactly(const T* row, int f, int d, float top, float inv, int8_t* q) {
+  for (int j = 0; j < 8 && f + j < d; ++j) {
+    const float x = to_float(row[f + j]), r = x * inv;
+    if (!(fabsf(r - rintf(r)) < 0.4999f)) q[f + j] = (int8_t)(int)rint((double)x * 127.0 / (double)top);
+  }
 }
 
 template <typename T>
@@ -73,8 +78,8 @@ struct QrPiece {
     }
   }
   // The eight 8-bit numbers, and whether one of them is in doubt.  With f = 127 / top in 32 bits, x f is off
-  // 127 x / top by less than 127 * 2^-24 < 1e-5, so round_half_even(127 x / top) as exact arithmetic has it is
-  // the rounding of x f unless that lies closer than 1e-4 to the middle between two whole numbers; then the
+  // 127 x / top by at most 127 * 2^-24 = 7.6e-6, so round_half_even(127 x / top) as exact arithmetic has it is
+  // the rounding of x f unless that lies closer than 1e-5 to the middle between two whole numbers; then the
   // quotient in 64 bits decides (127 x is exact there, and a quotient of such short numbers is never rounded
   // onto a middle that it does not hit).  x f + 1.5 * 2^23 in one operation is rounded to a whole number, whose
   // low byte is the result; a second one gives what the rounding took away.
@@ -89,7 +94,7 @@ struct QrPiece {
       n[j] = __float_as_uint(s);
       off = fmaxf(off, fabsf(fmaf(x, inv, magic - s)));
     }
-    doubt = !(off < 0.4999f);
+    doubt = !(off < QR_SURE);
     uint2 p;
     p.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
     p.y = __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410);
@@ -98,7 +103,7 @@ struct QrPiece {
 };
 
 template <typename T, int THREADS, int ROWS, int VECS>
-__global__ void __launch_bounds__(THREADS * ROWS, (sizeof(T) == 2 ? 1536 : 1024) / (THREADS * ROWS))
+__global__ void __launch_bounds__(THREADS * ROWS, (sizeof(T) == 2 ? 1280 : 1024) / (THREADS * ROWS))
 quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* __restrict__ rows, int64_t m,
                      int8_t* __restrict__ q, int64_t q_pitch, float* __restrict__ scales, int vec) {
   static_assert(ROWS == 1 || THREADS == 32, "several rows of a block take a warp each");
@@ -150,7 +155,7 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* _
     bool doubt;
     const uint2 p = piece.round(inv, doubt);
     *reinterpret_cast<uint2*>(qi + f) = zero ? make_uint2(0u, 0u) : p;
-    if ((doubt || tiny) && !zero) quantize_exactly(xi, f, end, topf, qi);
+    if ((doubt || tiny) && !zero) quantize_exactly(xi, f, end, topf, inv, qi);
   };
   if (VECS > 0) {
 #pragma unroll

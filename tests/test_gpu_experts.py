@@ -338,6 +338,51 @@ def test_combine(dtype, n, k, d, m, repeated):
         assert torch.equal(a.grad, got_v) and torch.equal(b.grad, got_w)
 
 
+@pytest.mark.parametrize("dtype,d", [("fp32", 1024), ("fp32", 1031), ("fp32", 7), ("fp32", 2049), ("fp32", 4), ("bf16", 2048), ("bf16", 50), ("bf16", 51),
+                                     ("fp16", 4104), ("bf16", 2064), ("fp16", 2050)])
+@pytest.mark.parametrize("k", [1, 2, 3, 4, 5, 8])
+def test_combine_many_tokens(dtype, d, k):
+    """Tokens enough for the rows to be copied ahead: every warp walks several, and the last ones fewer."""
+    from sklearn_numba_dpex_b200.common import combine_experts, combine_experts_grad
+
+    t, n = TYPES[dtype], 5003
+    g = torch.Generator("cuda").manual_seed(d + k)
+    values = torch.randn(n * k + 3, d, device="cuda", generator=g).to(t)
+    slots = torch.randperm(n * k + 3, device="cuda", generator=g)[: n * k].view(n, k).to(torch.int32)
+    slots[torch.rand(n, k, device="cuda", generator=g) < 0.1] = -1
+    if k > 2:
+        slots[100:110, 1] = slots[200, 0]                # rows with several users
+    weights, grad = torch.randn(n, k, device="cuda", generator=g), torch.randn(n, d, device="cuda", generator=g).to(t)
+    there = (slots >= 0)[..., None]
+    at = slots.long().clamp_min(0)
+    weights[~there[..., 0]] = float("nan")
+    w64 = torch.where(there, weights.double()[..., None], torch.zeros((), dtype=torch.float64, device="cuda"))
+    v64 = values.double()[at] * there
+    half, tiny = torch.finfo(t).eps / 2, torch.finfo(t).smallest_normal * torch.finfo(t).eps
+    out = (v64 * w64).sum(1)
+    got = combine_experts(values, slots, weights)
+    assert ((got.double() - out).abs() <= (k + 1) * U * (v64 * w64).abs().sum(1) + half * out.abs() + tiny).all()
+    rows = (w64 * grad.double()[:, None]).reshape(-1, d)
+    gv, big = torch.zeros_like(values, dtype=torch.float64), torch.zeros_like(values, dtype=torch.float64)
+    gv.index_add_(0, at.reshape(-1), rows)
+    big.index_add_(0, at.reshape(-1), rows.abs())
+    got_v, got_w = combine_experts_grad(values, slots, weights, grad)
+    assert ((got_v.double() - gv).abs() <= 13 * U * big + half * gv.abs() + tiny).all()
+    gw, size = (v64 * grad.double()[:, None]).sum(2), (v64 * grad.double()[:, None]).abs().sum(2)
+    assert ((got_w.double() - gw).abs() <= (d + 1) * U * size).all()
+
+
+def test_combine_many_choices_of_many_tokens():
+    from sklearn_numba_dpex_b200.common import combine_experts
+
+    n, k, d = 3000, 70, 24
+    values, slots = torch.randn(500, d, device="cuda"), torch.randint(-1, 500, (n, k), device="cuda", dtype=torch.int32)
+    weights = torch.randn(n, k, device="cuda")
+    v64 = values.double()[slots.long().clamp_min(0)] * (slots >= 0)[..., None] * weights.double()[..., None]
+    err = (combine_experts(values, slots, weights).double() - v64.sum(1)).abs()
+    assert (err <= (k + 1) * U * v64.abs().sum(1)).all()
+
+
 def test_combine_many_users_of_one_row():
     from sklearn_numba_dpex_b200.common import combine_experts_grad
 
