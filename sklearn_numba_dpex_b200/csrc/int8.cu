@@ -21,12 +21,15 @@
 namespace kmb {
 
 // =============================================================================== quantisation
-// THREADS threads per row, ROWS rows per block.  Where there are rows enough to fill the GPU, a thread
-// holds four pieces of eight elements, so that enough bytes are on their way while other blocks wait at
-// their barrier or round; with few rows it holds one or two, for the latency of a row.  (A warp per row
-// with 16 pieces a lane had 12 warps on an SM and took 80 us for 8192 rows of 4096 bf16, a block of 256
-// with two pieces 32 us.)  The pieces stay in registers, as they lie in memory, between the maximum and the
-// rounding; rows longer than 8192 (VECS = 0) are read a second time, from L1 and L2.
+// A row per block, or per warp (WARP) where a warp holds one.  A thread holds up to VECS pieces of eight
+// elements, and the launch takes as many threads as a row needs: four pieces where there are rows enough to
+// fill the GPU, so that enough bytes are on their way while other blocks wait at their barrier or round; one or
+// two with few rows, for the latency of a row.  (Two pieces a thread took 32 us for 8192 rows of 4096 bf16; a
+// warp per row with 16 pieces a lane left 12 warps on an SM and took 80 us.)  The pieces stay in registers, as
+// they lie in memory, between the maximum and the rounding; rows longer than 8192 (VECS = 0) are read a second
+// time, from L1 and L2.
+constexpr int QR_THREADS = 256, QR_WARP_ROWS = 4;
+
 // How near to the middle between two whole numbers a product is in doubt (see QrPiece::round).
 constexpr float QR_SURE = 0.49999f;
 
@@ -102,17 +105,16 @@ struct QrPiece {
   }
 };
 
-template <typename T, int THREADS, int ROWS, int VECS>
-__global__ void __launch_bounds__(THREADS * ROWS, (sizeof(T) == 2 ? 1280 : 1024) / (THREADS * ROWS))
+template <typename T, bool WARP, int VECS>
+__global__ void __launch_bounds__(QR_THREADS, sizeof(T) == 2 ? 5 : 4)
 quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* __restrict__ rows, int64_t m,
                      int8_t* __restrict__ q, int64_t q_pitch, float* __restrict__ scales, int vec) {
-  static_assert(ROWS == 1 || THREADS == 32, "several rows of a block take a warp each");
   next_grid_may_start();
   grid_dependency_wait();
-  __shared__ uint32_t red[THREADS / 32];
-  const int tid = threadIdx.x % THREADS;
-  const int64_t i = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
-  if (ROWS > 1 && i >= m) return;
+  __shared__ uint32_t red[QR_THREADS / 32];
+  const int threads = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t i = WARP ? (int64_t)blockIdx.x * QR_WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
+  if (WARP && i >= m) return;
   int64_t src = i;
   if (rows) {
     src = rows[i];
@@ -126,22 +128,21 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* _
   uint32_t top = 0;
   if (VECS > 0) {
 #pragma unroll
-    for (int r = 0; r < HELD; ++r) v[r].load(xi, (r * THREADS + tid) * 8, end, vec != 0);
+    for (int r = 0; r < HELD; ++r) v[r].load(xi, (r * threads + tid) * 8, end, vec != 0);
 #pragma unroll
     for (int r = 0; r < HELD; ++r) top = max(top, v[r].top());
   } else {
-    for (int f = tid * 8; f < end; f += THREADS * 8) {
+    for (int f = tid * 8; f < end; f += threads * 8) {
       v[0].load(xi, f, end, vec != 0);
       top = max(top, v[0].top());
     }
   }
   top = __reduce_max_sync(0xffffffffu, top);
-  if (THREADS > 32) {
+  if (!WARP) {
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
     __syncthreads();
     top = red[0];
-#pragma unroll
-    for (int w = 1; w < THREADS / 32; ++w) top = max(top, red[w]);
+    for (int w = 1; w < threads / 32; ++w) top = max(top, red[w]);
   }
   const float topf = __uint_as_float(top);
   // a row that holds an infinity or NaN has no 8-bit image: NaN as its scale makes its products NaN
@@ -160,9 +161,9 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* _
   if (VECS > 0) {
 #pragma unroll
     for (int r = 0; r < HELD; ++r)
-      if ((r * THREADS + tid) * 8 < d) put(v[r], (r * THREADS + tid) * 8);
+      if ((r * threads + tid) * 8 < d) put(v[r], (r * threads + tid) * 8);
   } else {
-    for (int f = tid * 8; f < d; f += THREADS * 8) {
+    for (int f = tid * 8; f < d; f += threads * 8) {
       v[0].load(xi, f, end, vec != 0);
       put(v[0], f);
     }
@@ -173,21 +174,21 @@ template <typename T>
 int quantize_run(const T* x, int64_t n, int d, const int32_t* rows, int64_t m, int8_t* q,
                  int64_t q_pitch, float* scales, cudaStream_t s) {
   const int vec = rows_are_vec(x, d) ? 1 : 0;
-  const unsigned one = (unsigned)m, four = (unsigned)ceil_div(m, 4);
-#define KMB_RUN(THREADS, ROWS, VECS)                                                            \
-  return launch_early(quantize_rows_kernel<T, THREADS, ROWS, VECS>, ROWS == 1 ? one : four, THREADS * ROWS, 0, 1, s, x, \
-                      n, d, rows, m, q, q_pitch, scales, vec)
   const bool many = m >= (int64_t)sm_count() * 8;
-  if (d <= 256) KMB_RUN(32, 4, 1);
-  else if (d <= 512) KMB_RUN(32, 4, 2);
-  else if (many && d <= 1024) KMB_RUN(32, 4, 4);
-  else if (many && d <= 2048) KMB_RUN(64, 1, 4);
-  else if (many && d <= 4096) KMB_RUN(128, 1, 4);
-  else if (d <= 1024) KMB_RUN(128, 1, 1);
-  else if (d <= 2048) KMB_RUN(128, 1, 2);
-  else if (d <= 4096) KMB_RUN(256, 1, 2);
-  else if (d <= 8192) KMB_RUN(256, 1, 4);
-  else KMB_RUN(256, 1, 0);
+  const int pieces = (int)ceil_div(d, 8);
+#define KMB_RUN(WARP, VECS, THREADS)                                                            \
+  return launch_early(quantize_rows_kernel<T, WARP, VECS>, (unsigned)(WARP ? ceil_div(m, QR_WARP_ROWS) : m), THREADS, \
+                      0, 1, s, x, n, d, rows, m, q, q_pitch, scales, vec)
+  if (pieces <= 32) KMB_RUN(true, 1, 32 * QR_WARP_ROWS);
+  if (pieces <= 64) KMB_RUN(true, 2, 32 * QR_WARP_ROWS);
+  if (many && pieces <= 128) KMB_RUN(true, 4, 32 * QR_WARP_ROWS);
+  if (pieces > QR_THREADS * 4) KMB_RUN(false, 0, QR_THREADS);
+  // as many pieces a thread as leave the fewest threads without one
+  const auto width = [pieces](int v) { return (int)ceil_div(pieces, v * 32) * 32; };
+  if (!many && pieces <= QR_THREADS) KMB_RUN(false, 1, width(1));
+  if (!many && pieces <= QR_THREADS * 2) KMB_RUN(false, 2, width(2));
+  if (pieces <= QR_THREADS * 3 && width(3) * 3 < width(4) * 4) KMB_RUN(false, 3, width(3));
+  KMB_RUN(false, 4, width(4));
 #undef KMB_RUN
 }
 
@@ -216,6 +217,8 @@ constexpr int I8_KB = 128;            // bytes (= 8-bit features) per stage
 constexpr int I8_EPI_WARPS = 8;
 constexpr int I8_THREADS = 128 + I8_EPI_WARPS * 32;
 constexpr int I8_SCAN_THREADS = 256;
+constexpr int I8_PAIR_BOX = 32;       // token rows that one load brings for a pair's narrow tile (for whole
+                                      // tiles too, four such loads a stage took 207 us where one takes 166)
 constexpr int I8_MAX_GROUPS = 1024;
 constexpr long long I8_TIMEOUT_CYCLES = 4000000000LL;   // ~2 s at 2 GHz
 
@@ -228,8 +231,13 @@ struct I8Cfg {
   static constexpr int FIT = (212 * 1024) / (A_BYTES + B_BYTES);
   static constexpr int STAGES = FIT > 12 ? 12 : FIT;
   static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
-  static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) |
-                                    ((uint32_t)(CTAS * I8_BM >> 4) << 24);   // int32 += s8 * s8, K-major
+  // int32 += s8 * s8, both K-major, `cols` tokens wide
+  __host__ __device__ static constexpr uint32_t idesc(int cols) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(CTAS * I8_BM >> 4) << 24);
+  }
+  // tokens that a tile of `rows` is multiplied as: a group's last tile in a pair is as narrow as its rows
+  // allow, in steps of 64 (a box of 32 rows in each CTA)
+  __device__ static __forceinline__ int cols(int rows) { return MODE == I8_PAIR ? (rows + 63) / 64 * 64 : BN; }
 };
 
 template <int BN, I8Mode MODE>
@@ -433,7 +441,7 @@ __device__ __forceinline__ void i8_store(const uint32_t (&v)[COLS], const float*
 template <int BN, typename T, I8Mode MODE>
 __global__ void __launch_bounds__(I8_THREADS, 1)
 int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
-                   const __grid_constant__ I8Params p) {
+                   const __grid_constant__ CUtensorMap map_tail, const __grid_constant__ I8Params p) {
   using Cfg = I8Cfg<BN, MODE>;
   constexpr bool SPLIT = MODE == I8_SPLIT, PAIR = MODE == I8_PAIR;
   extern __shared__ __align__(16) unsigned char i8_dyn[];
@@ -446,6 +454,10 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   const int step = gridDim.x / per_tile;
   const int wide = PAIR ? 2 * I8_BM : I8_BM, skip = in_pair * I8_BM;
 
+  if (threadIdx.x == 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::STAGES; ++s) {
       mbar_init(&sm->full[s], 1);
@@ -535,6 +547,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       for (int t = first; t < tiles && ok; t += step) {
         const I8Tile tile = i8_tile<BN>(p, sm->first_tile, t, wide, skip);
         const int w_row = tile.g * p.n + tile.feature0;
+        const int my_rows = Cfg::cols(tile.rows) / 2;        // PAIR: the half of the tokens in this CTA
         for (int c = c_begin; c < c_end; ++c, ++it) {
           const uint32_t s = it % Cfg::STAGES, lap = it / Cfg::STAGES;
           if (!i8_wait(&sm->empty[s], (lap & 1u) ^ 1u, sm)) {
@@ -543,10 +556,14 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
           }
           if (PAIR) {
             // both CTAs' bytes count at CTA 0's barrier; its phase needs CTA 0's own arrival as well
-            if (in_pair == 0) mbar_expect_tx(&sm->full[s], 2 * (Cfg::A_BYTES + Cfg::B_BYTES));
+            if (in_pair == 0) mbar_expect_tx(&sm->full[s], 2 * (Cfg::A_BYTES + my_rows * I8_KB));
             const uint32_t full0 = address_in(&sm->full[s], 0);
             pair_tma_load(sm->a[s], &map_w, c * I8_KB, w_row, full0);
-            pair_tma_load(sm->b[s], &map_x, c * I8_KB, (int)tile.row0 + in_pair * (BN / 2), full0);
+            if (my_rows == BN / 2)
+              pair_tma_load(sm->b[s], &map_x, c * I8_KB, (int)tile.row0 + in_pair * my_rows, full0);
+            else
+              for (int r = 0; r < my_rows; r += I8_PAIR_BOX)
+                pair_tma_load(sm->b[s] + r * I8_KB, &map_tail, c * I8_KB, (int)tile.row0 + in_pair * my_rows + r, full0);
           } else {
             mbar_expect_tx(&sm->full[s], Cfg::A_BYTES + Cfg::B_BYTES);
             tma_load_2d(sm->a[s], &map_w, c * I8_KB, w_row, &sm->full[s]);
@@ -574,6 +591,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       if (!__all_sync(0xffffffffu, i8_wait<PAIR>(&sm->acc_empty[ab], ((nt >> 1) & 1u) ^ 1u, sm))) break;
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + ab * BN;
+      const uint32_t idesc = PAIR ? Cfg::idesc(Cfg::cols(i8_tile<BN>(p, sm->first_tile, t, wide, skip).rows)) : Cfg::idesc(BN);
       for (int c = c_begin; c < c_end; ++c, ++it) {
         const uint32_t s = it % Cfg::STAGES, lap = it / Cfg::STAGES;
         if (!__all_sync(0xffffffffu, i8_wait(&sm->full[s], lap & 1u, sm))) {
@@ -586,8 +604,8 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
           const uint64_t bd = b0 + (uint64_t)(s * (Cfg::B_BYTES >> 4));
           const int steps = c == all_chunks - 1 ? last_steps : 4;
           for (int ks = 0; ks < steps; ++ks)
-            if (PAIR) pair_umma_i8(d_tmem, ad + 2 * ks, bd + 2 * ks, Cfg::IDESC, (c > c_begin || ks > 0) ? 1u : 0u);
-            else umma_i8_ss(d_tmem, ad + 2 * ks, bd + 2 * ks, Cfg::IDESC, (c > c_begin || ks > 0) ? 1u : 0u);
+            if (PAIR) pair_umma_i8(d_tmem, ad + 2 * ks, bd + 2 * ks, idesc, (c > c_begin || ks > 0) ? 1u : 0u);
+            else umma_i8_ss(d_tmem, ad + 2 * ks, bd + 2 * ks, idesc, (c > c_begin || ks > 0) ? 1u : 0u);
           if (PAIR) {
             pair_commit(&sm->empty[s]);
             if (c == c_end - 1) pair_commit(&sm->acc_full[ab]);
@@ -650,7 +668,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         if (!ok && lane == 0) sm->bad = 1;
         if (works) {
 #pragma unroll 1
-          for (int c = 0; c < MINE; c += 16) {
+          for (int c = 0; c < MINE && col0 + c < tile.rows; c += 16) {
             uint32_t v[16];
             tmem_ld16(acc + col0 + c, v);
             tmem_ld_wait();
@@ -664,7 +682,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
           T* o = out + (tile.row0 + col0) * p.n + feature;
           const int rows = mine ? tile.rows - col0 : 0;
 #pragma unroll 1
-          for (int c = 0; c < MINE; c += COLS, o += (int64_t)COLS * p.n) {
+          for (int c = 0; c < MINE && col0 + c < tile.rows; c += COLS, o += (int64_t)COLS * p.n) {
             uint32_t v[COLS];
             if constexpr (COLS == 32) tmem_ld32(acc + col0 + c, v);
             else tmem_ld16(acc + col0 + c, v);
@@ -743,12 +761,12 @@ static int i8_make_map(CUtensorMap* map, const int8_t* base, int64_t rows, int d
 }
 
 template <int BN, typename T, I8Mode MODE>
-int i8_launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const I8Params& p, int64_t grid,
-              int cluster, cudaStream_t s) {
+int i8_launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const CUtensorMap& map_tail, const I8Params& p,
+              int64_t grid, int cluster, cudaStream_t s) {
   const int smem = (int)sizeof(I8Smem<BN, MODE>) + 1024;
   const auto kernel = int8_matmul_kernel<BN, T, MODE>;
   KMB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  return launch_early(kernel, (unsigned)grid, I8_THREADS, smem, cluster, s, map_w, map_x, p);
+  return launch_early(kernel, (unsigned)grid, I8_THREADS, smem, cluster, s, map_w, map_x, map_tail, p);
 }
 
 // CTAs that share a tile: as many as the SMs allow, while each has two stages' worth of the contraction
@@ -774,15 +792,18 @@ int i8_run_as(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, I8Para
   if (rc != KMB_OK) return rc;
   rc = i8_make_map(&map_x, a, p.m, p.d, lda, pairs ? BN / 2 : BN);
   if (rc != KMB_OK) return rc;
+  CUtensorMap map_tail = map_x;
+  if (pairs) rc = i8_make_map(&map_tail, a, p.m, p.d, lda, I8_PAIR_BOX);
+  if (rc != KMB_OK) return rc;
   if constexpr (BN >= 128) {
     if (pairs) {
       p.feature_tiles = (int)ceil_div(p.n, 2 * I8_BM);
-      return i8_launch<BN, T, I8_PAIR>(map_w, map_x, p, sms / 2 * 2, 2, s);
+      return i8_launch<BN, T, I8_PAIR>(map_w, map_x, map_tail, p, sms / 2 * 2, 2, s);
     }
   }
   p.feature_tiles = (int)ceil_div(p.n, I8_BM);
-  if (splits > 1) return i8_launch<BN, T, I8_SPLIT>(map_w, map_x, p, most * splits, splits, s);
-  return i8_launch<BN, T, I8_SINGLE>(map_w, map_x, p, most < sms ? most : sms, 1, s);
+  if (splits > 1) return i8_launch<BN, T, I8_SPLIT>(map_w, map_x, map_tail, p, most * splits, splits, s);
+  return i8_launch<BN, T, I8_SINGLE>(map_w, map_x, map_tail, p, most < sms ? most : sms, 1, s);
 }
 
 template <int BN>

@@ -253,6 +253,17 @@ CALL(combine_experts_grad, 4) {
 
 int64_t round16(int64_t d) { return (d + 15) / 16 * 16; }
 
+// Row pitch of 8-bit rows of our own: whole lines of 128 bytes where that costs an eighth at most.  The product
+// reads rows in pieces of 128 bytes, and pieces that straddle lines cost it (32 groups, 16 396 rows, 1408
+// outputs: 57 us with 2048 features, 71 us with 2056 at a pitch of 2064).
+int64_t pitch_of(int64_t d) {
+  for (int64_t line = 128; line > 16; line /= 2) {
+    const int64_t pitch = (d + line - 1) / line * line;
+    if (pitch - d <= d / 8) return pitch;
+  }
+  return round16(d);
+}
+
 // (x, rows)
 CALL(quantize_rows, 2) {
   const at::Tensor& x0 = tensor(a[0], "x");
@@ -270,7 +281,7 @@ CALL(quantize_rows, 2) {
     rows = ptr<int32_t>(r);
   }
   c10::cuda::CUDAGuard guard(x.device());
-  const int64_t pitch = round16(d);
+  const int64_t pitch = pitch_of(d);
   at::Tensor q = empty({m, pitch}, at::kChar, x), scales = empty({m}, at::kFloat, x);
   check(kmb_quantize_rows(code, ptr(x), n, d, rows, m, ptr<int8_t>(q), pitch, ptr<float>(scales), stream_of(x)),
         "kmb_quantize_rows");
@@ -285,7 +296,7 @@ at::Tensor pitched(const at::Tensor& t, int64_t* pitch) {
     *pitch = t.size(-2) == 1 && (dims == 2 || t.size(0) == 1) ? round16(t.stride(-2) > d ? t.stride(-2) : d) : t.stride(-2);
     if (*pitch % 16 == 0 && *pitch >= d && (dims == 2 || t.size(0) == 1 || t.stride(0) == t.size(1) * *pitch)) return t;
   }
-  *pitch = round16(d);
+  *pitch = pitch_of(d);
   std::vector<int64_t> sizes(t.sizes().begin(), t.sizes().end());
   sizes.back() = *pitch;
   at::Tensor copy = empty(sizes, at::kChar, t).narrow(-1, 0, d);
