@@ -444,7 +444,7 @@ int kmb_quantize_rows(int dtype, const void* x, int64_t n, int d, const int32_t*
                       int8_t* q, int64_t q_pitch, float* scales, void* stream);
 /* out[i, j] = a_scales[i] * b_scales[g, j] * sum_f a[i, f] * b[g, j, f] + bias[g, j], for the rows
  * offsets[g] <= i < offsets[g + 1] of every group g; offsets (groups + 1 int32 on the device, ascending) may
- * be NULL with groups = 1: all m rows.  Rows behind offsets[groups] become zeros.  a (m, d) and
+ * be NULL with groups = 1: all m rows.  Rows outside [offsets[0], offsets[groups]) become zeros.  a (m, d) and
  * b (groups * n, d) are row-major at pitches lda and ldb (bytes, multiples of 16) and 16-byte aligned;
  * bias (groups * n) may be NULL.  out (m, n) of out_dtype.  d <= 131071, groups <= 1024. */
 int kmb_int8_matmul(int out_dtype, const int8_t* a, int64_t lda, const float* a_scales, const int8_t* b,

@@ -28,7 +28,7 @@ def int8_matmul(a, a_scales, b, b_scales, bias=None, offsets=None, out_dtype=tor
     `a` (m, d) and `b` (n, d) int8, scales and `bias` float32; the sum is exact.  With `offsets` (g + 1
     int32, ascending, on the device) `b` is (g, n, d), `b_scales` and `bias` (g, n), and rows
     ``offsets[g]:offsets[g + 1]`` of `a` meet ``b[g]``: the experts' products, with nothing read back to the
-    host.  Rows behind ``offsets[-1]`` become zeros.  `out_dtype` is float32, float16 or bfloat16.
+    host.  Rows ahead of ``offsets[0]`` and behind ``offsets[-1]`` become zeros.  `out_dtype` is float32, float16 or bfloat16.
 
     Rows are read in pieces of 16 bytes: operands as `quantize_rows` returns them, or with d a multiple
     of 16, are read in place; others are copied first.  At most 131071 features and 1024 groups.

@@ -635,11 +635,10 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     constexpr int EPI = I8_EPI_WARPS * 32;
     T* out = reinterpret_cast<T*>(p.out);
     if (p.offsets) {
-      // rows behind the last group belong to nobody: zeros
-      const int64_t end = i8_row_of(p, p.groups);
-      const int64_t from = end * p.n, to = p.m * p.n;
-      for (int64_t e = from + (int64_t)blockIdx.x * EPI + etid; e < to; e += (int64_t)gridDim.x * EPI)
-        out[e] = from_float<T>(0.f);
+      // rows ahead of the first group and behind the last belong to nobody: zeros
+      const int64_t head = i8_row_of(p, 0) * p.n, tail = i8_row_of(p, p.groups) * p.n, all = p.m * p.n;
+      for (int64_t e = (int64_t)blockIdx.x * EPI + etid; e < head + (all - tail); e += (int64_t)gridDim.x * EPI)
+        out[e < head ? e : tail + (e - head)] = from_float<T>(0.f);
     }
     // columns of this warp: half of the tile's tokens (all, where that would be less than 16)
     constexpr int COLS = BN >= 64 ? 32 : 16;

@@ -484,6 +484,43 @@ def test_layer_on_another_stream_and_in_a_graph():
             assert torch.equal(a, b)
 
 
+def test_layers_in_a_graph_that_forks_and_joins():
+    """Calls whose kernels may start early, behind a join of two streams, captured and replayed; and two
+    graphs replayed at the same time."""
+    n, e, dim, out, k = 300, 8, 256, 192, 2
+    args = [_layer_inputs(n, e, dim, out, s) for s in (31, 32)]
+    want = [_layer(*a, k, e) for a in args]
+    from sklearn_numba_dpex_b200.common import combine_experts
+
+    def forked(a, b):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        first = _layer(*a, k, e)
+        with torch.cuda.stream(side):
+            second = _layer(*b, k, e)
+        torch.cuda.current_stream().wait_stream(side)
+        return first, second, combine_experts(first[3], second[2], second[0])
+
+    joined = forked(*args)
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(forked(*args))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for got in (joined, *held):
+        for i in (0, 1):
+            for x, y in zip(got[i], want[i]):
+                assert torch.equal(x, y)
+        assert torch.equal(got[2], joined[2])
+
+
 def test_gradients_in_a_graph():
     from sklearn_numba_dpex_b200.common import combine_experts_grad, route_topk_grad
 

@@ -188,8 +188,8 @@ def test_product_by_group(g, m, n, d, kind):
     assert (got[off[-1]:] == 0).all()
 
 
-def test_product_by_group_of_random_weights_touches_no_other_row():
-    """The rows before the first group are left alone, those behind the last become zeros."""
+def test_product_by_group_that_begins_late():
+    """The rows ahead of the first group become zeros, as those behind the last do."""
     from sklearn_numba_dpex_b200.common import int8_matmul
 
     off = _group_offsets("late", 5, 200, np.random.default_rng(0))
@@ -201,6 +201,7 @@ def test_product_by_group_of_random_weights_touches_no_other_row():
         if off[e + 1] > off[e]:
             want, size = ref_product(ops[0][r], ops[1][r], ops[2][e], ops[3][e], None)
             _check(got[r], want, size)
+    assert off[0] > 0 and (got[: off[0]] == 0).all()
 
 
 def test_product_whose_output_passes_32_bit_offsets():
