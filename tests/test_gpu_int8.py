@@ -188,6 +188,24 @@ def test_product_by_group(g, m, n, d, kind):
     assert (got[off[-1]:] == 0).all()
 
 
+@pytest.mark.parametrize("d", [50, 130, 2056])
+def test_weights_as_quantize_rows_lays_them_out(d):
+    """Rows at quantize_rows' pitch, seen as a matrix for each group, are read in place."""
+    from sklearn_numba_dpex_b200.common import int8_matmul, quantize_rows
+
+    g, n, m = 3, 37, 90
+    gen = torch.Generator("cuda").manual_seed(d)
+    w, ws = quantize_rows(torch.randn(g * n, d, device="cuda", generator=gen))
+    x, xs = quantize_rows(torch.randn(m, d, device="cuda", generator=gen))
+    assert w.stride(0) % 16 == 0 and w.stride(0) - d <= max(15, d // 8)
+    off = torch.tensor([0, 10, 60, m], dtype=torch.int32, device="cuda")
+    got = int8_matmul(x, xs, w.view(g, n, d), ws.view(g, n), offsets=off, out_dtype=torch.float32)
+    for e in range(g):
+        r = slice(int(off[e]), int(off[e + 1]))
+        want, size = ref_product(x.cpu()[r], xs.cpu()[r], w.cpu().view(g, n, d)[e], ws.cpu().view(g, n)[e], None)
+        _check(got[r], want, size)
+
+
 def test_product_by_group_that_begins_late():
     """The rows ahead of the first group become zeros, as those behind the last do."""
     from sklearn_numba_dpex_b200.common import int8_matmul
