@@ -155,6 +155,22 @@ def test_route_near_ties_are_ordered_as_64_bits_order_them(scoring):
     _same_route(xs, 20, bias=torch.zeros(64, device="cuda"), scoring=scoring, n_groups=8, topk_groups=3, group_best=2)
 
 
+@pytest.mark.parametrize("e", [30, 64, 128, 200, 1000])
+@pytest.mark.parametrize("base", [1.0, -1.0, 0.0, 37.5])
+def test_route_orders_logits_that_differ_in_their_last_bits(e, base):
+    """Neighbouring float32 numbers in random order, some of them equal: every token lies in the low bits of its
+    logits, or one does among ordinary ones."""
+    g = torch.Generator().manual_seed(e)
+    ulps = torch.randint(0, 2 * e, (9, e), generator=g)
+    x = (torch.full((9, e), base).view(torch.int32) + ulps.to(torch.int32)).view(torch.float32)
+    if base == 0.0:
+        x = x * (torch.randint(0, 2, (9, e), generator=g) * 2 - 1)         # subnormals, -0 among them
+    _same_route(x.cuda(), min(9, e))
+    y = torch.randn(9, e, generator=g)
+    y[4] = x[4]
+    _same_route(y.cuda(), min(9, e), scoring="sigmoid")
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalize", [True, False])
 def test_route_nan_and_infinity(scoring, renormalize):
