@@ -17,7 +17,7 @@ constexpr unsigned FULL = 0xffffffffu;
 // l * V + V - 1 in registers, so that the lowest lane among equals is the lowest index.  k rounds take the
 // greatest key each: a maximum in the lane, one over the lanes, a ballot for the lowest of them.
 // Bound by instruction issue (0.69 a scheduler and cycle), not by HBM: 16 384 x 128 float32, k = 8, takes
-// 10 us (0.9 TB/s), 65 521 x 64 bfloat16, k = 6, 17 us; with a whole warp per token, whatever the number of
+// 10 us (0.9 TB/s), 65 521 x 64 bfloat16, k = 6, 13 us; with a whole warp per token, whatever the number of
 // experts, 17 and 41 us.
 constexpr int RT_WARPS = 4;
 constexpr int RT_MAX_EXPERTS = 1024;
@@ -265,9 +265,10 @@ __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row
 
 // Choice by logits alone.  A key holds the upper bits of a logit's order and below them the expert, counted
 // down, so that all keys of a token differ: a round is one maximum, and what it found is struck out wherever it
-// lies.  The NB low bits that the expert takes are empty in logits of 16 bits; of two float32 logits that differ
+// lies.  The low bits that the expert takes are empty in logits of 16 bits; of two float32 logits that differ
 // in nothing else the order may be wrong, and then the token is done again with whole keys (`unsure`: about one
-// in two hundred).  16 384 x 128 float32, k = 8: 8 us, with whole keys from the start 10.
+// in two hundred).  65 521 x 64 bfloat16, k = 6, took 17 us with whole keys; float32 logits gain nothing
+// (16 384 x 128, k = 8: 10 us either way), but lose nothing either.
 template <typename T, int L, int V>
 __device__ __forceinline__ Chosen route_by_logit(const RouteParams& p, const T* row, const float (&x)[V], int lane) {
   constexpr bool exact = sizeof(T) == 2;

@@ -223,8 +223,8 @@ constexpr int I8_KB = 128;            // bytes (= 8-bit features) per stage
 constexpr int I8_EPI_WARPS = 8;
 constexpr int I8_THREADS = 128 + I8_EPI_WARPS * 32;
 constexpr int I8_SCAN_THREADS = 256;
-constexpr int I8_PAIR_BOX = 32;       // token rows that one load brings for a pair's narrow tile (for whole
-                                      // tiles too, four such loads a stage took 207 us where one takes 166)
+constexpr int I8_PAIR_BOX = 64;       // token rows that one load brings for a pair's narrow tile (boxes of 32
+                                      // for whole tiles too took 207 us where one load a stage takes 166)
 constexpr int I8_MAX_GROUPS = 1024;
 constexpr long long I8_TIMEOUT_CYCLES = 4000000000LL;   // ~2 s at 2 GHz
 
@@ -242,8 +242,10 @@ struct I8Cfg {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(CTAS * I8_BM >> 4) << 24);
   }
   // tokens that a tile of `rows` is multiplied as: a group's last tile in a pair is as narrow as its rows
-  // allow, in steps of 64 (a box of 32 rows in each CTA)
-  __device__ static __forceinline__ int cols(int rows) { return MODE == I8_PAIR ? (rows + 63) / 64 * 64 : BN; }
+  // allow, in steps of two boxes (one in each CTA)
+  __device__ static __forceinline__ int cols(int rows) {
+    return MODE == I8_PAIR ? (rows + 2 * I8_PAIR_BOX - 1) / (2 * I8_PAIR_BOX) * (2 * I8_PAIR_BOX) : BN;
+  }
 };
 
 template <int BN, I8Mode MODE>
@@ -262,8 +264,7 @@ struct I8Smem {
   volatile int abort_flag;
 };
 constexpr size_t I8_SMEM_LIMIT = 232448 - 1024;      // 227 KB, less the alignment of the stages
-static_assert(sizeof(I8Smem<256, I8_PAIR>) <= I8_SMEM_LIMIT && sizeof(I8Smem<128, I8_PAIR>) <= I8_SMEM_LIMIT &&
-                  sizeof(I8Smem<256, I8_SINGLE>) <= I8_SMEM_LIMIT && sizeof(I8Smem<128, I8_SINGLE>) <= I8_SMEM_LIMIT &&
+static_assert(sizeof(I8Smem<256, I8_PAIR>) <= I8_SMEM_LIMIT && sizeof(I8Smem<256, I8_SINGLE>) <= I8_SMEM_LIMIT && sizeof(I8Smem<128, I8_SINGLE>) <= I8_SMEM_LIMIT &&
                   sizeof(I8Smem<64, I8_SINGLE>) <= I8_SMEM_LIMIT && sizeof(I8Smem<32, I8_SINGLE>) <= I8_SMEM_LIMIT &&
                   sizeof(I8Smem<16, I8_SINGLE>) <= I8_SMEM_LIMIT,
               "the stages exceed the 227 KB a CTA may use");
@@ -722,12 +723,29 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const int64_t wrow = (int64_t)tile.g * p.n + feature;
         const float sb = bad ? __uint_as_float(0x7fffffffu) : p.sb[wrow];
         const float bias = p.bias ? p.bias[wrow] : 0.f;
-        const int* part = reinterpret_cast<const int*>(sm->a[0]);
-        for (int c = split * 2 + half; c < tile.rows; c += splits * 2) {
-          int sum = 0;
-          for (int r = 0; r < splits; ++r) sum += load_from(part + c * I8_BM + q * 32 + lane, r);
-          reinterpret_cast<T*>(p.out)[(tile.row0 + c) * p.n + feature] =
-              from_float<T>((float)sum * (sm->sa[c] * sb) + bias);
+        // this warp's tokens: every 2 * splits-th of the tile, AT_ONCE of them in flight from each CTA
+        constexpr int AT_ONCE = BN >= 64 ? 8 : 4;
+        const int hop = splits * 2;
+        const int* part = reinterpret_cast<const int*>(sm->a[0]) + q * 32 + lane;
+        for (int c0 = split * 2 + half; c0 < tile.rows; c0 += hop * AT_ONCE) {
+          int sum[AT_ONCE];
+#pragma unroll
+          for (int u = 0; u < AT_ONCE; ++u) sum[u] = 0;
+          for (int r = 0; r < splits; ++r) {
+            int v[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u)
+              v[u] = c0 + u * hop < tile.rows ? load_from(part + (c0 + u * hop) * I8_BM, r) : 0;
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) sum[u] += v[u];
+          }
+#pragma unroll
+          for (int u = 0; u < AT_ONCE; ++u) {
+            const int c = c0 + u * hop;
+            if (c < tile.rows)
+              reinterpret_cast<T*>(p.out)[(tile.row0 + c) * p.n + feature] =
+                  from_float<T>((float)sum[u] * (sm->sa[c] * sb) + bias);
+          }
         }
       }
     }
@@ -774,49 +792,91 @@ int i8_launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const CUtensor
   return launch_early(kernel, (unsigned)grid, I8_THREADS, smem, cluster, s, map_w, map_x, map_tail, p);
 }
 
-// CTAs that share a tile: as many as the SMs allow, while each has two stages' worth of the contraction
-// at least.
-static int i8_splits(int64_t tiles, int d) {
-  const int chunks = (d + I8_KB - 1) / I8_KB;
-  int s = 8;
-  while (s > 1 && (tiles * s > sm_count() || chunks < 2 * s)) s >>= 1;
-  return s;
+// How a product is cut: tokens per tile, CTAs per tile, and whether pairs of CTAs work on tiles twice as wide.
+struct I8Plan {
+  int bn, splits;
+  bool pairs;
+  int64_t tiles;      // an upper bound: every group may end inside a tile
+};
+
+// The cycles of a plan, near enough to choose by.  A CTA goes through `rounds` tiles.  A chunk of the
+// contraction takes as long as its bytes take to arrive (60 a cycle and SM) or its products (2 cycles a token);
+// a tile's stores overlap the next tile, but not the last one; partial sums in a cluster are stored, fetched and
+// added behind the last chunk.  Measured against the model (us): 500 rows x 4096 x 4096 with 64, 128, 256 tokens
+// a tile 22.3, 14.8, 17.2 (model 22.8, 14.6, 17.8); 128 x 8192 x 2048 with 32, 64, 128 12.0, 8.0, 10.6 (11.0, 8.2,
+// 10.3); 1000 x 1000 x 1000 with 32, 64, 128 7.9, 6.4, 9.4 (7.4, 6.3, 9.1).
+static int64_t i8_cycles(const I8Plan& plan, int64_t m, int groups, int feature_tiles, int chunks, int sms) {
+  // tiles to expect: half a tile is lost at the end of each group
+  int64_t token_tiles = groups == 1 ? ceil_div(m, plan.bn) : m / plan.bn + groups / 2;
+  const int64_t busy = m < groups ? m : groups;
+  if (token_tiles < busy) token_tiles = busy;
+  const int64_t tiles = token_tiles * feature_tiles;
+  const int64_t workers = plan.pairs ? sms / 2 : sms;
+  const int64_t rounds = plan.splits > 1 ? 1 : ceil_div(tiles, workers);
+  const int64_t bytes = I8_BM * I8_KB + (int64_t)plan.bn * I8_KB / (plan.pairs ? 2 : 1);
+  const int64_t chunk = bytes / 60 > 2 * plan.bn ? bytes / 60 : 2 * plan.bn;
+  const int64_t work = ceil_div(chunks, plan.splits) * chunk;
+  const int64_t store = plan.splits > 1 ? 4500 + 40 * plan.bn : 2500 + 16 * plan.bn;
+  return rounds * work + store + (rounds - 1) * (store > work ? store - work : 0);
+}
+
+static I8Plan i8_plan(int64_t m, int groups, int n, int d) {
+  const int sms = sm_count(), chunks = (d + I8_KB - 1) / I8_KB;
+  I8Plan best = {};
+  int64_t least = 0;
+  for (int bn = 16; bn <= 256; bn *= 2) {
+    const int64_t token_tiles = ceil_div(m, bn) + groups - 1;
+    I8Plan plan;
+    plan.bn = bn;
+    plan.splits = 1;
+    // pairs where there is a wide tile for each of them
+    plan.pairs = bn == 256 && n > I8_BM && token_tiles * ceil_div(n, 2 * I8_BM) >= sms / 2;
+    const int64_t feature_tiles = ceil_div(n, plan.pairs ? 2 * I8_BM : I8_BM);
+    plan.tiles = token_tiles * feature_tiles;
+    // CTAs that share a tile: as many as there are SMs for, while each has two chunks at least.  SMs come in
+    // groups of uneven size: of 148, 15 clusters of eight and 33 of four find room at once.
+    if (!plan.pairs)
+      for (int s = 8; s > 1 && plan.splits == 1; s >>= 1) {
+        const int64_t room = s == 8 ? sms / 8 * 5 / 6 : s == 4 ? sms / 4 * 9 / 10 : sms / 2;
+        if (plan.tiles <= room && chunks >= 2 * s) plan.splits = s;
+      }
+    const int64_t c = i8_cycles(plan, m, groups, (int)feature_tiles, chunks, sms);
+    if (bn == 16 || c < least) {
+      least = c;
+      best = plan;
+    }
+    if (bn >= m) break;       // wider tiles would be no fuller
+  }
+  return best;
 }
 
 template <int BN, typename T>
-int i8_run_as(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, I8Params p, cudaStream_t s) {
-  // an upper bound of the tiles: every group may end inside one
-  const int64_t token_tiles = ceil_div(p.m, BN) + p.groups - 1;
-  const int64_t most = token_tiles * ceil_div(p.n, I8_BM);
-  KMB_REQUIRE(most < (1ll << 31), "kmb_int8_matmul: too many output tiles");
-  const int sms = sm_count(), splits = i8_splits(most, p.d);
-  // pairs where there is a wide tile for each of them
-  const bool pairs = BN >= 128 && p.n > I8_BM && token_tiles * ceil_div(p.n, 2 * I8_BM) >= sms / 2;
+int i8_run_as(const I8Plan& plan, const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, I8Params p,
+              cudaStream_t s) {
+  KMB_REQUIRE(plan.tiles < (1ll << 31), "kmb_int8_matmul: too many output tiles");
+  const int sms = sm_count();
   CUtensorMap map_w, map_x;
   int rc = i8_make_map(&map_w, b, (int64_t)p.groups * p.n, p.d, ldb, I8_BM);
   if (rc != KMB_OK) return rc;
-  rc = i8_make_map(&map_x, a, p.m, p.d, lda, pairs ? BN / 2 : BN);
+  rc = i8_make_map(&map_x, a, p.m, p.d, lda, plan.pairs ? BN / 2 : BN);
   if (rc != KMB_OK) return rc;
   CUtensorMap map_tail = map_x;
-  if (pairs) rc = i8_make_map(&map_tail, a, p.m, p.d, lda, I8_PAIR_BOX);
+  if (plan.pairs) rc = i8_make_map(&map_tail, a, p.m, p.d, lda, I8_PAIR_BOX);
   if (rc != KMB_OK) return rc;
-  if constexpr (BN >= 128) {
-    if (pairs) {
-      p.feature_tiles = (int)ceil_div(p.n, 2 * I8_BM);
-      return i8_launch<BN, T, I8_PAIR>(map_w, map_x, map_tail, p, sms / 2 * 2, 2, s);
-    }
-  }
-  p.feature_tiles = (int)ceil_div(p.n, I8_BM);
-  if (splits > 1) return i8_launch<BN, T, I8_SPLIT>(map_w, map_x, map_tail, p, most * splits, splits, s);
-  return i8_launch<BN, T, I8_SINGLE>(map_w, map_x, map_tail, p, most < sms ? most : sms, 1, s);
+  p.feature_tiles = (int)ceil_div(p.n, plan.pairs ? 2 * I8_BM : I8_BM);
+  if constexpr (BN == 256)
+    if (plan.pairs) return i8_launch<BN, T, I8_PAIR>(map_w, map_x, map_tail, p, sms / 2 * 2, 2, s);
+  if (plan.splits > 1)
+    return i8_launch<BN, T, I8_SPLIT>(map_w, map_x, map_tail, p, plan.tiles * plan.splits, plan.splits, s);
+  return i8_launch<BN, T, I8_SINGLE>(map_w, map_x, map_tail, p, plan.tiles < sms ? plan.tiles : sms, 1, s);
 }
 
 template <int BN>
-int i8_run(int out_dtype, const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, const I8Params& p,
-           cudaStream_t s) {
-  if (out_dtype == KMB_F32) return i8_run_as<BN, float>(a, lda, b, ldb, p, s);
-  if (out_dtype == KMB_F16) return i8_run_as<BN, __half>(a, lda, b, ldb, p, s);
-  return i8_run_as<BN, __nv_bfloat16>(a, lda, b, ldb, p, s);
+int i8_run(const I8Plan& plan, int out_dtype, const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb,
+           const I8Params& p, cudaStream_t s) {
+  if (out_dtype == KMB_F32) return i8_run_as<BN, float>(plan, a, lda, b, ldb, p, s);
+  if (out_dtype == KMB_F16) return i8_run_as<BN, __half>(plan, a, lda, b, ldb, p, s);
+  return i8_run_as<BN, __nv_bfloat16>(plan, a, lda, b, ldb, p, s);
 }
 
 }  // namespace kmb
@@ -869,13 +929,14 @@ int kmb_int8_matmul(int out_dtype, const int8_t* a, int64_t lda, const float* a_
   e = getenv("KMB_TC_TEST_STALL");
   p.test_stall = e && atoi(e) != 0;
   cudaStream_t s = (cudaStream_t)stream;
-  // Tokens per tile: the narrowest that holds an average group.
-  const int64_t rows = ceil_div(m, groups);
-  if (rows <= 16) return i8_run<16>(out_dtype, a, lda, b, ldb, p, s);
-  if (rows <= 32) return i8_run<32>(out_dtype, a, lda, b, ldb, p, s);
-  if (rows <= 64) return i8_run<64>(out_dtype, a, lda, b, ldb, p, s);
-  if (rows <= 128) return i8_run<128>(out_dtype, a, lda, b, ldb, p, s);
-  return i8_run<256>(out_dtype, a, lda, b, ldb, p, s);
+  const I8Plan plan = i8_plan(m, groups, n, d);
+  switch (plan.bn) {
+    case 16: return i8_run<16>(plan, out_dtype, a, lda, b, ldb, p, s);
+    case 32: return i8_run<32>(plan, out_dtype, a, lda, b, ldb, p, s);
+    case 64: return i8_run<64>(plan, out_dtype, a, lda, b, ldb, p, s);
+    case 128: return i8_run<128>(plan, out_dtype, a, lda, b, ldb, p, s);
+    default: return i8_run<256>(plan, out_dtype, a, lda, b, ldb, p, s);
+  }
 }
 
 int kmb_int8_wait_error(int* flag, void* stream) {
