@@ -423,7 +423,7 @@ int kmb_expert_slots(const int32_t* experts, int64_t n, int k, int n_experts, in
 size_t kmb_expert_slots_workspace_bytes(int64_t n, int k, int n_experts);
 
 /* out (n, d): out[t] = sum_j weights[t, j] * values[slots[t, j]], values (n_values, d); a slot outside
- * [0, n_values) adds nothing, whatever its weight. */
+ * [0, n_values) adds nothing, whatever its weight.  d < 2^30. */
 int kmb_combine_experts(int dtype, const void* values, int64_t n_values, const int32_t* slots,
                         const float* weights, int64_t n, int k, int d, void* out, void* stream);
 /* grad_values (n_values, d) and grad_weights (n, k) from grad_out (n, d).  Rows that several choices share
@@ -439,7 +439,7 @@ size_t kmb_combine_experts_grad_workspace_bytes(int64_t n_values);
  * r = rows[i], or i when rows is NULL (then m = n).  x (n, d) of `dtype`; q (m, d) at a pitch of q_pitch
  * bytes (a multiple of 16; bytes between d and the pitch may be overwritten).  The rounding is that of the
  * exact quotient.  A row outside [0, n) or of zeros gives zeros and scale 0; a row that holds an
- * infinity or NaN gives zeros and scale NaN. */
+ * infinity or NaN gives zeros and scale NaN.  d < 2^30. */
 int kmb_quantize_rows(int dtype, const void* x, int64_t n, int d, const int32_t* rows, int64_t m,
                       int8_t* q, int64_t q_pitch, float* scales, void* stream);
 /* out[i, j] = a_scales[i] * b_scales[g, j] * sum_f a[i, f] * b[g, j, f] + bias[g, j], for the rows

@@ -754,6 +754,7 @@ slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, in
 // ============================================================================= weighted sums
 // out[t] = sum_j w[t, j] values[slots[t, j]]; a slot outside [0, n_values) counts as none.
 constexpr int CB_THREADS = 256;   // at most; the launch takes as many as a row needs (combine_threads)
+constexpr int CB_MAX_D = 1 << 30; // places in a row, a block's pass behind its end among them, fit 32 bits
 constexpr int CB_K = 8;           // rows that a thread asks for before it adds the first
 constexpr int CG_THREADS = 128, CG_K = 4;   // the gradients', which hold twice as much per row
 
@@ -1136,6 +1137,7 @@ int kmb_expert_slots(const int32_t* experts, int64_t n, int k, int n_experts, in
 int kmb_combine_experts(int dtype, const void* values, int64_t n_values, const int32_t* slots,
                         const float* weights, int64_t n, int k, int d, void* out, void* stream) {
   KMB_REQUIRE(n >= 0 && n < (1ll << 31) - 1 && n_values >= 0 && k >= 1 && d >= 1, "kmb_combine_experts: bad sizes");
+  KMB_REQUIRE(d < CB_MAX_D, "kmb_combine_experts: d must be below 2^30");
   if (n == 0) return KMB_OK;
   KMB_REQUIRE((values || n_values == 0) && slots && weights && out, "kmb_combine_experts: NULL argument");
   KMB_DISPATCH_ROWS(dtype, {
@@ -1158,6 +1160,7 @@ int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, co
                              void* grad_values, float* grad_weights, void* workspace, size_t workspace_bytes,
                              void* stream) {
   KMB_REQUIRE(n >= 0 && n_values >= 0 && k >= 1 && d >= 1, "kmb_combine_experts_grad: bad sizes");
+  KMB_REQUIRE(d < CB_MAX_D, "kmb_combine_experts_grad: d must be below 2^30");
   KMB_REQUIRE(n <= (1ll << 30) && n < 0x7f7f7f7fll / k, "kmb_combine_experts_grad: n * k must be below 2^31");
   if (n == 0 && n_values == 0) return KMB_OK;
   KMB_REQUIRE((n_values == 0 || (values && grad_values)) && (n == 0 || (slots && weights && grad_out && grad_weights)),

@@ -888,6 +888,7 @@ extern "C" {
 int kmb_quantize_rows(int dtype, const void* x, int64_t n, int d, const int32_t* rows, int64_t m,
                       int8_t* q, int64_t q_pitch, float* scales, void* stream) {
   KMB_REQUIRE(n >= 0 && d > 0 && m >= 0 && m < (1ll << 31), "kmb_quantize_rows: bad sizes");
+  KMB_REQUIRE(d < (1 << 30), "kmb_quantize_rows: d must be below 2^30");
   KMB_REQUIRE(rows != nullptr || m == n, "kmb_quantize_rows: m must be n when no rows are named");
   if (m == 0) return KMB_OK;
   KMB_REQUIRE((x || n == 0) && q && scales, "kmb_quantize_rows: NULL argument");

@@ -44,45 +44,4 @@ inline bool rows_are_vec(const T* x, int64_t d) {
   return ((uintptr_t)x & 15) == 0 && (d * sizeof(T)) % 16 == 0;
 }
 
-// v[j] = p[f + j] for f + j < d, else 0; `vec`: rows_are_vec holds and f is a multiple of 8.
-template <typename T>
-__device__ __forceinline__ void load_vec8(const T* __restrict__ p, int f, int d, bool vec, float (&v)[8]) {
-  if (vec && f + 8 <= d) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(p + f);
-      const float4 b = *reinterpret_cast<const float4*>(p + f + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      union { uint4 u; T t[8]; } r;
-      r.u = *reinterpret_cast<const uint4*>(p + f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_float(r.t[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = f + j < d ? to_float(p[f + j]) : 0.f;
-  }
-}
-
-// p[f + j] = v[j] for f + j < d, rounded to T.
-template <typename T>
-__device__ __forceinline__ void store_vec8(T* __restrict__ p, int f, int d, bool vec, const float (&v)[8]) {
-  if (vec && f + 8 <= d) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p + f) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(p + f + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      union { uint4 u; T t[8]; } r;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) r.t[j] = from_float<T>(v[j]);
-      *reinterpret_cast<uint4*>(p + f) = r.u;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (f + j < d) p[f + j] = from_float<T>(v[j]);
-  }
-}
-
 }  // namespace kmb

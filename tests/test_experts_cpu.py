@@ -61,6 +61,8 @@ def test_slots_and_combine_checks():
     _raises(lambda l: l.kmb_combine_experts(1, P, 4, P, P, 4, 2, 8, P, None), "dtype")
     _raises(lambda l: l.kmb_combine_experts(0, P, 4, P, P, 4, 0, 8, P, None), "sizes")
     _raises(lambda l: l.kmb_combine_experts(0, None, 4, P, P, 4, 2, 8, P, None), "NULL")
+    _raises(lambda l: l.kmb_combine_experts(0, P, 4, P, P, 4, 2, 1 << 30, P, None), "2\\^30")
+    _raises(lambda l: l.kmb_combine_experts_grad(0, P, 4, P, P, P, 4, 2, 1 << 30, P, P, P, 1 << 20, None), "2\\^30")
     need = lib.kmb_combine_experts_grad_workspace_bytes(100)
     _raises(lambda l: l.kmb_combine_experts_grad(0, P, 100, P, P, P, 4, 2, 8, P, P, P, need - 1, None), "workspace",
             _cabi.KmbError)
@@ -84,6 +86,7 @@ def test_int8_checks():
     _raises(product(n=0), "sizes")
     _raises(lambda l: l.kmb_quantize_rows(1, P, 4, 8, None, 4, P, 16, P, None), "dtype")
     _raises(lambda l: l.kmb_quantize_rows(0, P, 4, 8, None, 5, P, 16, P, None), "m must be n")
+    _raises(lambda l: l.kmb_quantize_rows(0, P, 4, 1 << 30, None, 4, P, 1 << 30, P, None), "2\\^30")
     _raises(lambda l: l.kmb_quantize_rows(0, P, 4, 8, None, 4, P, 8, P, None), "pitch")
     _raises(lambda l: l.kmb_quantize_rows(0, P, 4, 20, None, 4, P, 16, P, None), "pitch")
     _raises(lambda l: l.kmb_quantize_rows(0, None, 4, 8, None, 4, P, 16, P, None), "NULL")
