@@ -10,7 +10,10 @@ A layer whose experts multiply in 8 bits reads::
     y = int8_matmul(q, scales, w, w_scales, offsets=offsets)      # w (n_experts, n, d) int8
     out = combine_experts(y, slots, weights)
 
-All tensors live on one CUDA device; a call is enqueued on that device's current stream.
+All tensors live on one CUDA device; a call is enqueued on that device's current stream, waits for nothing
+and can be captured into a CUDA graph.  `route_topk` and `combine_experts` are differentiable; a backward pass that
+is to be captured calls `route_topk_grad` and `combine_experts_grad` itself, since autograd's own nodes belong to
+the stream that first used their leaves.
 """
 import torch
 
