@@ -868,6 +868,26 @@ __global__ void combine_users_kernel(const int32_t* __restrict__ slots, int64_t 
   atomicMin(&first[slot], (int32_t)c);
 }
 
+// Both for few rows and choices, in one launch.
+constexpr int CG_FEW = 8192;
+__global__ void __launch_bounds__(1024)
+combine_few_users_kernel(const int32_t* __restrict__ slots, int total, int n_values, int32_t* __restrict__ users,
+                         int32_t* __restrict__ first) {
+  next_grid_may_start();
+  grid_dependency_wait();
+  for (int r = threadIdx.x; r < n_values; r += blockDim.x) {
+    users[r] = 0;
+    first[r] = INT_MAX;
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < total; c += blockDim.x) {
+    const int slot = slots[c];
+    if (slot < 0 || slot >= n_values) continue;
+    atomicAdd(&users[slot], 1);
+    atomicMin(&first[slot], c);
+  }
+}
+
 // The rows that have no user or several: zeros, or the sum over the users, which are found by walking the
 // choices from the lowest of them on, a block's width at a time, and added in ascending order.  Block `block`
 // of `blocks` looks at as many rows at once as it has threads.
@@ -1173,15 +1193,20 @@ int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, co
   cudaStream_t s = (cudaStream_t)stream;
   int32_t* users = (int32_t*)workspace;
   int32_t* first = users + n_values;
-  if (n_values > 0) {
-    const int rc = launch_early(combine_clear_kernel, (unsigned)ceil_div(n_values, 256), 256, 0, 1, s, n_values, users,
-                                first);
+  if (n_values > 0 && n_values <= CG_FEW && n * k <= CG_FEW) {
+    const int rc = launch_early(combine_few_users_kernel, 1, 1024, 0, 1, s, slots, n * k, n_values, users, first);
     if (rc != KMB_OK) return rc;
-  }
-  if (n > 0) {
-    const int rc = launch_early(combine_users_kernel, (unsigned)ceil_div(n * k, 256), 256, 0, 1, s, slots, n * k,
-                                n_values, users, first);
-    if (rc != KMB_OK) return rc;
+  } else {
+    if (n_values > 0) {
+      const int rc = launch_early(combine_clear_kernel, (unsigned)ceil_div(n_values, 256), 256, 0, 1, s, n_values, users,
+                                  first);
+      if (rc != KMB_OK) return rc;
+    }
+    if (n > 0) {
+      const int rc = launch_early(combine_users_kernel, (unsigned)ceil_div(n * k, 256), 256, 0, 1, s, slots, n * k,
+                                  n_values, users, first);
+      if (rc != KMB_OK) return rc;
+    }
   }
   KMB_DISPATCH_ROWS(dtype, {
     const int vec = rows_are_vec((const T*)values, d) && rows_are_vec((const T*)grad_out, d) &&

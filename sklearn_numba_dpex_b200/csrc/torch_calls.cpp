@@ -285,7 +285,10 @@ CALL(quantize_rows, 2) {
   at::Tensor q = empty({m, pitch}, at::kChar, x), scales = empty({m}, at::kFloat, x);
   check(kmb_quantize_rows(code, ptr(x), n, d, rows, m, ptr<int8_t>(q), pitch, ptr<float>(scales), stream_of(x)),
         "kmb_quantize_rows");
-  return wrap(pitch == d ? std::move(q) : q.narrow(1, 0, d), std::move(scales));
+  // the rows without what pads them to the pitch (a view would cost as much as the launch)
+  const int64_t sizes[2] = {m, d}, strides[2] = {pitch, 1};
+  q.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef(sizes, 2), at::IntArrayRef(strides, 2));
+  return wrap(std::move(q), std::move(scales));
 }
 
 // `t` with rows at a pitch of a multiple of 16 bytes, as the kernel's loads need them: itself if it is laid
