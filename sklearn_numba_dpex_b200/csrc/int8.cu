@@ -802,9 +802,10 @@ struct I8Plan {
 // The cycles of a plan, near enough to choose by.  A CTA goes through `rounds` tiles.  A chunk of the
 // contraction takes as long as its bytes take to arrive (60 a cycle and SM) or its products (2 cycles a token);
 // a tile's stores overlap the next tile, but not the last one; partial sums in a cluster are stored, fetched and
-// added behind the last chunk.  Measured against the model (us): 500 rows x 4096 x 4096 with 64, 128, 256 tokens
-// a tile 22.3, 14.8, 17.2 (model 22.8, 14.6, 17.8); 128 x 8192 x 2048 with 32, 64, 128 12.0, 8.0, 10.6 (11.0, 8.2,
-// 10.3); 1000 x 1000 x 1000 with 32, 64, 128 7.9, 6.4, 9.4 (7.4, 6.3, 9.1).
+// added behind the last chunk.  Measured, and by this estimate at 1.85 GHz with 2.7 us for the start (us):
+// 500 x 4096 x 4096 with 64, 128, 256 tokens a tile 22.3, 14.8, 17.2 and 18.8, 14.6, 17.8; 128 x 8192 x 2048 with
+// 32, 64, 128 12.0, 8.0, 10.6 and 10.2, 8.1, 10.3; 1000 x 1000 x 1000 with 32, 64, 128 7.9, 6.4, 9.4 and 7.4, 6.4,
+// 9.1.
 static int64_t i8_cycles(const I8Plan& plan, int64_t m, int groups, int feature_tiles, int chunks, int sms) {
   // tiles to expect: half a tile is lost at the end of each group
   int64_t token_tiles = groups == 1 ? ceil_div(m, plan.bn) : m / plan.bn + groups / 2;
