@@ -1,7 +1,9 @@
 // Launches that may start before the kernel ahead of them on the stream has ended (programmatic dependent
 // launch): set-up and launch latency overlap that kernel's end.  A kernel launched so reads and writes
 // nothing in global memory before grid_dependency_wait(), which returns when everything that the kernels
-// ahead wrote is there; to the stream the order of the kernels is what it always is.
+// ahead wrote is there; to the stream the order of the kernels is what it always is.  What the kernels ahead may
+// have written is not read-only for such a kernel's whole life, so its inputs are no `const T* __restrict__`,
+// which the compiler reads through the non-coherent path.
 #pragma once
 #include "kmb_common.cuh"
 

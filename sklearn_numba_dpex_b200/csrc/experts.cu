@@ -567,7 +567,7 @@ constexpr int SL_MAX_EXPERTS = 1024;
 
 // counts[chunk][e] for every chunk
 __global__ void __launch_bounds__(SL_THREADS)
-slots_count_kernel(const int32_t* __restrict__ experts, int64_t total, int n_experts,
+slots_count_kernel(const int32_t* experts, int64_t total, int n_experts,
                    int32_t* __restrict__ counts) {
   __shared__ int32_t s_cnt[SL_MAX_EXPERTS];
   next_grid_may_start();
@@ -635,8 +635,8 @@ slots_scan_kernel(int32_t* __restrict__ counts, int chunks, int n_experts, int32
 // ONE: a single chunk, whose counts are the totals.
 template <bool ONE>
 __global__ void __launch_bounds__(SL_THREADS)
-slots_place_kernel(const int32_t* __restrict__ experts, int64_t total, int k, int n_experts,
-                   const int32_t* __restrict__ counts, const int32_t* __restrict__ totals,
+slots_place_kernel(const int32_t* experts, int64_t total, int k, int n_experts,
+                   const int32_t* counts, const int32_t* totals,
                    int32_t* __restrict__ slots, int32_t* __restrict__ rows, int32_t* __restrict__ offsets) {
   extern __shared__ int32_t s_dyn[];
   int32_t* s_base = s_dyn;                            // first place of each expert in this chunk
@@ -769,7 +769,7 @@ struct RowPiece {
   __device__ __forceinline__ static int at(int f0, int j) {
     return VEC ? f0 + threadIdx.x * 8 + j : f0 + threadIdx.x + j * blockDim.x;
   }
-  __device__ __forceinline__ void load(const T* __restrict__ row, int f0, int d) {
+  __device__ __forceinline__ void load(const T* row, int f0, int d) {
     if constexpr (VEC) {
       uint4* dst = reinterpret_cast<uint4*>(t);
 #pragma unroll
@@ -805,8 +805,8 @@ struct RowPiece {
 // faster, 54 and 64 us.)
 template <typename T, bool VEC>
 __global__ void __maxnreg__(96)      // four blocks of 160 threads on an SM
-combine_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __restrict__ slots,
-               const float* __restrict__ weights, int k, int d, T* __restrict__ out, int parts) {
+combine_kernel(const T* values, int64_t n_values, const int32_t* slots,
+               const float* weights, int k, int d, T* __restrict__ out, int parts) {
   typedef RowPiece<T, VEC> Piece;
   next_grid_may_start();
   grid_dependency_wait();
@@ -856,7 +856,7 @@ __global__ void combine_clear_kernel(int64_t n_values, int32_t* __restrict__ use
   first[r] = INT_MAX;
 }
 
-__global__ void combine_users_kernel(const int32_t* __restrict__ slots, int64_t total, int64_t n_values,
+__global__ void combine_users_kernel(const int32_t* slots, int64_t total, int64_t n_values,
                                      int32_t* __restrict__ users, int32_t* __restrict__ first) {
   next_grid_may_start();
   grid_dependency_wait();
@@ -871,7 +871,7 @@ __global__ void combine_users_kernel(const int32_t* __restrict__ slots, int64_t 
 // Both for few rows and choices, in one launch.
 constexpr int CG_FEW = 8192;
 __global__ void __launch_bounds__(1024)
-combine_few_users_kernel(const int32_t* __restrict__ slots, int total, int n_values, int32_t* __restrict__ users,
+combine_few_users_kernel(const int32_t* slots, int total, int n_values, int32_t* __restrict__ users,
                          int32_t* __restrict__ first) {
   next_grid_may_start();
   grid_dependency_wait();
@@ -893,9 +893,9 @@ combine_few_users_kernel(const int32_t* __restrict__ slots, int total, int n_val
 // of `blocks` looks at as many rows at once as it has threads.
 template <typename T, bool VEC>
 __device__ __noinline__ void combine_other_rows(int64_t block, int64_t blocks, int64_t n_values,
-                                                const int32_t* __restrict__ slots, const float* __restrict__ weights,
-                                                const T* __restrict__ grad_out, int64_t choices, int k, int d,
-                                                const int32_t* __restrict__ users, const int32_t* __restrict__ first,
+                                                const int32_t* slots, const float* weights,
+                                                const T* grad_out, int64_t choices, int k, int d,
+                                                const int32_t* users, const int32_t* first,
                                                 T* __restrict__ grad_values) {
   typedef RowPiece<T, VEC> Piece;
   __shared__ int32_t list[CG_THREADS], other[CG_THREADS];
@@ -961,9 +961,9 @@ __device__ __noinline__ void combine_other_rows(int64_t block, int64_t blocks, i
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(CG_THREADS, 8)
-combine_grad_kernel(const T* __restrict__ values, int64_t n_values, const int32_t* __restrict__ slots,
-                    const float* __restrict__ weights, const T* __restrict__ grad_out, int64_t n, int k, int d,
-                    const int32_t* __restrict__ users, const int32_t* __restrict__ first,
+combine_grad_kernel(const T* values, int64_t n_values, const int32_t* slots,
+                    const float* weights, const T* grad_out, int64_t n, int k, int d,
+                    const int32_t* users, const int32_t* first,
                     T* __restrict__ grad_values, float* __restrict__ grad_weights, int64_t token_blocks) {
   typedef RowPiece<T, VEC> Piece;
   __shared__ float red[CG_THREADS / 32][CG_K];

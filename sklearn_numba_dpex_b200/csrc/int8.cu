@@ -54,7 +54,7 @@ struct Pair<__nv_bfloat16> { typedef __nv_bfloat162 type; };
 template <typename T>
 struct QrPiece {
   alignas(16) T t[8];
-  __device__ __forceinline__ void load(const T* __restrict__ row, int f, int d, bool vec) {
+  __device__ __forceinline__ void load(const T* row, int f, int d, bool vec) {
     if (vec) {       // rows of whole 16-byte pieces; a piece of eight floats may end behind the row
       uint4* dst = reinterpret_cast<uint4*>(t);
 #pragma unroll
@@ -108,7 +108,7 @@ struct QrPiece {
 
 template <typename T, bool WARP, int VECS>
 __global__ void __launch_bounds__(QR_THREADS, sizeof(T) == 2 ? 5 : 4)
-quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, const int32_t* __restrict__ rows, int64_t m,
+quantize_rows_kernel(const T* x, int64_t n, int d, const int32_t* rows, int64_t m,
                      int8_t* __restrict__ q, int64_t q_pitch, float* __restrict__ scales, int vec) {
   next_grid_may_start();
   grid_dependency_wait();
