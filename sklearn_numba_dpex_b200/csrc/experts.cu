@@ -265,9 +265,11 @@ __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row
 
 // Choice by logits alone.  A key holds the upper bits of a logit's order and below them the expert, counted
 // down, so that all keys of a token differ: a round is one maximum, and what it found is struck out wherever it
-// lies.  The low bits that the expert takes are empty in logits of 16 bits; of two float32 logits that differ
-// in nothing else the order may be wrong, and then the token is done again with whole keys (`unsure`: about one
-// in two hundred).  65 521 x 64 bfloat16, k = 6, took 17 us with whole keys; float32 logits gain nothing
+// lies.  The low bits that the expert takes are empty in logits of 16 bits.  Of two float32 logits that differ
+// in nothing else the order may be wrong.  Equal upper bits lie side by side in the order of the keys, so it is
+// right if the chosen of equal upper bits are equal each to the next, and no expert behind them that shares the
+// last one's upper bits is greater than that one; else the token is done again with whole keys (`unsure`: about
+// one in two hundred).  65 521 x 64 bfloat16, k = 6, took 17 us with whole keys; float32 logits gain nothing
 // (16 384 x 128, k = 8: 10 us either way), but lose nothing either.
 template <typename T, int L, int V>
 __device__ __forceinline__ Chosen route_by_logit(const RouteParams& p, const T* row, const float (&x)[V], int lane) {
@@ -282,15 +284,14 @@ __device__ __forceinline__ Chosen route_by_logit(const RouteParams& p, const T* 
     bits[i] = b == 0u ? 0u : (b & ~LOW) | (LOW - (uint32_t)(e0 + i));
   }
   uint32_t mine = 0, next = 0;
-  const int rounds = exact ? p.k : p.k + 1;      // the first that is left out counts too
-  for (int j = 0; j < rounds; ++j) {
+  for (int j = 0; j < p.k; ++j) {
     uint32_t top = bits[0];
 #pragma unroll
     for (int i = 1; i < V; ++i) top = max(top, bits[i]);
     top = lanes_max<L>(top);
 #pragma unroll
     for (int i = 0; i < V; ++i) bits[i] = bits[i] == top ? 0u : bits[i];
-    if (sub == j && j < p.k) mine = top;
+    if (sub == j) mine = top;
     if (!exact && sub == j - 1) next = top;
   }
   Chosen c = {mine ? (int)(LOW - (mine & LOW)) : -1, false};
@@ -298,6 +299,17 @@ __device__ __forceinline__ Chosen route_by_logit(const RouteParams& p, const T* 
     bool close = mine != 0u && next != 0u && (mine & ~LOW) == (next & ~LOW);
     if (close)
       close = order_bits(to_float(row[LOW - (mine & LOW)])) != order_bits(to_float(row[LOW - (next & LOW)]));
+    // what was not chosen: its key is still there
+    const uint32_t last = __shfl_sync(FULL, mine, (lane & ~(L - 1)) + p.k - 1);
+    bool cut = false;
+#pragma unroll
+    for (int i = 0; i < V; ++i) cut = cut || (bits[i] != 0u && (bits[i] & ~LOW) == (last & ~LOW));
+    if (cut) {
+      const uint32_t least = order_bits(to_float(row[LOW - (last & LOW)]));
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (bits[i] != 0u && (bits[i] & ~LOW) == (last & ~LOW)) close = close || order_bits(to_float(row[e0 + i])) > least;
+    }
     c.unsure = lanes_of<L>(__ballot_sync(FULL, close), lane) != 0;
   }
   return c;

@@ -171,6 +171,36 @@ def test_route_orders_logits_that_differ_in_their_last_bits(e, base):
     _same_route(y.cuda(), min(9, e), scoring="sigmoid")
 
 
+# experts and greatest k, in every layout of the routing kernel (lanes of a token, experts of a lane)
+LAYOUTS = [(32, 8), (30, 12), (64, 8), (128, 16), (100, 20), (256, 8), (500, 8), (1000, 32)]
+
+
+@pytest.mark.parametrize("e,most", LAYOUTS)
+@pytest.mark.parametrize("base", [0.25, 1.0, -3.0])
+def test_route_finds_a_greater_logit_behind_a_tie(e, most, base):
+    """Equal logits on both sides of the last place, and among or behind them one that differs in its last bits."""
+    g = torch.Generator().manual_seed(e)
+    up, down = (float(np.nextafter(np.float32(base), np.float32(to))) for to in (9, -9))
+    for k in sorted({1, 4, 8, most}):
+        if k > most:
+            continue
+        rows = []
+        for place in sorted({0, k - 1, k, min(k + 1, e - 1), e // 2, e - 1}):
+            for value in (up, down, base * 1.00005):
+                x = torch.full((e,), base)
+                x[place] = value
+                rows.append(x)
+        some = torch.full((20, e), base)
+        some[torch.rand(20, e, generator=g) < 0.02] = up
+        some[torch.rand(20, e, generator=g) < 0.3] = down
+        some[:10][torch.rand(10, e, generator=g) < 0.5] = -9.0
+        _same_route(torch.cat([torch.stack(rows), some]).cuda(), k)
+    x = torch.full((3, e), -3.0)
+    x[:, :2] = 1.0
+    x[0, 2] = x[1, e - 1] = float(np.nextafter(np.float32(1), np.float32(2)))
+    _same_route(x.cuda(), 1)
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalize", [True, False])
 def test_route_nan_and_infinity(scoring, renormalize):
