@@ -105,11 +105,13 @@ struct Chosen {
 // Scores, keys, groups and choice of one token in arithmetic of type K.
 //
 // In 32 bits the keys carry rounding errors, and two keys closer than `margin` may be in the wrong
-// order.  The errors: the exponential 2 ulp, its argument's rounding |x - top| 2^-24 against a factor
-// exp(x - top) (at most 0.37 ulp of the largest score), the sum of the scores V + 5 additions of 2^-24
-// each, the quotient, the bias's addition.  (V + 16) 2^-24 of the largest score and key covers both
-// keys of a pair.  A token with such a pair (about one in a hundred) is done again in 64 bits, which
-// is what the definition says.  Equal logits with equal biases have equal keys and need no second look.
+// order.  The errors, in 2^-24 of the largest score and key: the exponentials in the sum of the scores 4 and its
+// V + 5 additions, which move both keys of a pair alike; for each of the two the exponential 4, its argument's
+// rounding |x - top| against a factor exp(x - top) 1, the quotient 1 and the bias's addition 1; the margin's own
+// subtraction 1.  That makes V + 24.  A token with such a pair (about one in a hundred) is done again in 64
+// bits, which is what the definition says.  Equal logits with equal biases have equal keys and need no second
+// look; so each choice is compared with the next, and the last one with all that was not chosen and is not its
+// equal.
 template <typename K, int L, int V, bool PLAIN, typename T>
 __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row, const float (&x)[V], int lane,
                                               bool by_logit, float* s_keys) {
@@ -160,7 +162,7 @@ __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row
     }
     if (narrow) {
       const uint32_t m = lanes_max<L>(__float_as_uint((float)most));
-      margin = (K)((float)(V + 16) * 0x1p-24f) * (top_score + (K)__uint_as_float(m));
+      margin = (K)((float)(V + 24) * 0x1p-24f) * (top_score + (K)__uint_as_float(m));
     }
   }
   bool unsure = false;
@@ -226,9 +228,7 @@ __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row
   Chosen c = {-1, false};
   B mine = 0, next = 0;
   int next_e = -1;
-  const bool check = !PLAIN && narrow && p.bias != nullptr;
-  const int rounds = check ? p.k + 1 : p.k;      // the first that is left out counts too
-  for (int j = 0; j < rounds; ++j) {
+  for (int j = 0; j < p.k; ++j) {
     B best = bits[0];
 #pragma unroll
     for (int i = 1; i < V; ++i) best = best > bits[i] ? best : bits[i];
@@ -244,7 +244,7 @@ __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row
     }
     const int at_w = __shfl_sync(FULL, at, (lane & ~(L - 1)) + w);
     const int e = top == 0 ? -1 : at_w + w * V;
-    if (sub == j && j < p.k) {
+    if (sub == j) {
       c.expert = e;
       mine = top;
     }
@@ -253,11 +253,20 @@ __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row
       next_e = e;
     }
   }
-  if (check) {
-    bool close = sub < p.k && c.expert >= 0 && next_e >= 0 && !(from_order_bits(mine) - from_order_bits(next) > margin);
-    // the same bias on the same logit: the same key
-    if (close && p.bias[c.expert] == p.bias[next_e] && to_float(row[c.expert]) == to_float(row[next_e])) close = false;
-    unsure = unsure || lanes_of<L>(__ballot_sync(FULL, close), lane) != 0;
+  if constexpr (!PLAIN && narrow) {
+    if (p.bias) {
+      const auto same = [&](int a, int b) { return p.bias[a] == p.bias[b] && to_float(row[a]) == to_float(row[b]); };
+      bool close = c.expert >= 0 && next_e >= 0 && !(from_order_bits(mine) - from_order_bits(next) > margin);
+      if (close && same(c.expert, next_e)) close = false;
+      // what was not chosen: its key is still there
+      const int last_lane = (lane & ~(L - 1)) + p.k - 1;
+      const B least = order_bits(from_order_bits(__shfl_sync(FULL, mine, last_lane)) - margin);
+      const int last = __shfl_sync(FULL, c.expert, last_lane);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (bits[i] != 0 && bits[i] >= least && !same(last, e0 + i)) close = true;
+      unsure = unsure || lanes_of<L>(__ballot_sync(FULL, close), lane) != 0;
+    }
   }
   c.unsure = unsure;
   return c;

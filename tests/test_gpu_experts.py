@@ -202,6 +202,35 @@ def test_route_finds_a_greater_logit_behind_a_tie(e, most, base):
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e,most", LAYOUTS)
+def test_route_finds_a_greater_key_behind_equal_ones(scoring, e, most):
+    """Few kinds of experts with equal logits and biases, whose keys differ by less than 32 bits from kind to
+    kind: the last place falls among equals while a greater key may lie behind them."""
+    for seed in range(12):
+        g = torch.Generator().manual_seed(seed)
+        kinds = torch.randn(max(2, e // 16), generator=g)
+        x = kinds[torch.randint(0, len(kinds), (e,), generator=g)]
+        bias = (0.7 - torch.from_numpy(_scores(x.double().numpy(), scoring))).float()
+        for k in sorted({1, 4, 8, most}):
+            if k <= most:
+                _same_route(x[None].repeat(3, 1).cuda(), k, scoring=scoring, bias=bias.cuda())
+
+
+@pytest.mark.parametrize("e,most", LAYOUTS)
+def test_route_equal_keys_of_a_bias_step(e, most):
+    """Two equal experts and one behind them, greater by 1.7e-8 where 32 bits see three equal keys."""
+    x = torch.full((2, e), -9.0)
+    x[0, :2], x[0, e - 1] = 0.22753906, 0.19921875
+    x[1, 1:3], x[1, 3] = 0.22753906, 0.19921875
+    bias = torch.zeros(2, e)
+    bias[0, :2], bias[0, e - 1] = -0.002, 0.005
+    bias[1, 1:3], bias[1, 3] = -0.002, 0.005
+    for dtype in (torch.float32, torch.bfloat16):
+        for i in range(2):
+            _same_route(x[i:i + 1].to(dtype).cuda(), 1, scoring="sigmoid", bias=bias[i].cuda())
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalize", [True, False])
 def test_route_nan_and_infinity(scoring, renormalize):
     x = torch.randn(6, 40, generator=torch.Generator().manual_seed(2))
