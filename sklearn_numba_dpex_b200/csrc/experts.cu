@@ -653,6 +653,10 @@ slots_scan_kernel(int32_t* __restrict__ counts, int chunks, int n_experts, int32
   if (warp == 0 && mine) totals[e] = carry;
 }
 
+constexpr size_t slots_place_smem(int n_experts) {
+  return (size_t)n_experts * (2 * sizeof(int32_t) + SL_WARPS * sizeof(uint16_t));
+}
+
 // ONE: a single chunk, whose counts are the totals.
 template <bool ONE>
 __global__ void __launch_bounds__(SL_THREADS)
@@ -1155,11 +1159,14 @@ int kmb_expert_slots(const int32_t* experts, int64_t n, int k, int n_experts, in
   cudaStream_t s = (cudaStream_t)stream;
   const int64_t total = n * k;
   const int chunks = (int)ceil_div(total, SL_CHUNK);
-  const size_t smem = (size_t)n_experts * (2 * sizeof(int32_t) + SL_WARPS * sizeof(uint16_t));
-  // the counters of 16 warps and the ordered chunk may pass the 48 KB that need no asking
+  const size_t smem = slots_place_smem(n_experts);
+  // The counters of 16 warps and the ordered chunk may pass the 48 KB that need no asking.  The limit belongs to
+  // the kernel, not to the call: every call that needs one sets the same, so that none lowers it under another's
+  // launch.
   const auto place = chunks <= 1 ? slots_place_kernel<true> : slots_place_kernel<false>;
   if (smem > 8 * 1024)
-    KMB_CHECK_CUDA(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    KMB_CHECK_CUDA(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)slots_place_smem(SL_MAX_EXPERTS)));
   if (chunks <= 1)
     return launch_early(place, 1, SL_THREADS, smem, 1, s, experts, total, k, n_experts, nullptr, nullptr, slots, rows,
                         offsets);

@@ -7,6 +7,10 @@ below 1e-17 of the largest), the exponential 4 u, the sum at most 37 additions, 
 u each: below 128 u = 2^-17, twice that with a softmax over all experts whose sum and quotient enter again.
 Results in 16 bits add half a step of their type.
 """
+import ctypes
+import functools
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -346,6 +350,39 @@ def test_expert_slots(n, k, e, kind):
     for a, b in zip(got, ref_slots(x, e)):
         assert a.dtype == torch.int32
         np.testing.assert_array_equal(a.cpu().numpy(), b)
+
+
+def test_expert_order_from_several_threads():
+    """Through the C interface, which runs without the interpreter's lock: calls that need much shared memory
+    beside calls that need little."""
+    from sklearn_numba_dpex_b200 import _cabi
+
+    n, k, counts, failed = 500, 8, (1024, 256, 1000, 210), []
+    together = threading.Barrier(len(counts))
+
+    def calls(e):
+        x = np.random.default_rng(e).integers(0, e, (n, k)).astype(np.int32)
+        xd = torch.from_numpy(x).cuda()
+        out = [torch.empty(size, dtype=torch.int32, device="cuda") for size in ((n, k), (n * k,), (e + 1,))]
+        stream = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        at = [_cabi.ptr(t) for t in (xd, *out)]
+        run = functools.partial(_cabi.lib.kmb_expert_slots, at[0], n, k, e, *at[1:], None, 0, ctypes.c_void_p(stream.cuda_stream))
+        together.wait()
+        for _ in range(20000):
+            if run() != _cabi.KMB_OK:
+                failed.append((e, _cabi.last_error()))
+                break
+        stream.synchronize()
+        if not all(np.array_equal(a.cpu().numpy(), b) for a, b in zip(out, ref_slots(x, e))):
+            failed.append((e, "another order"))
+
+    threads = [threading.Thread(target=calls, args=(e,)) for e in counts]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
 
 
 # --------------------------------------------------------------------------- weighted sums
