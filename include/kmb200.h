@@ -417,7 +417,7 @@ int kmb_route_topk_grad(int dtype, const void* logits, const int32_t* experts, c
 /* Expert order of the n * k choices: sorted by expert, token order kept within one.  slots (n, k): place of
  * each choice; rows (n * k): token in each place; offsets (n_experts + 1): first place of each expert.
  * A choice outside [0, n_experts) has slot -1, and rows behind offsets[n_experts] are -1.
- * n_experts <= 1024. */
+ * n_experts <= 1024, n * k < 2^31 - 4096. */
 int kmb_expert_slots(const int32_t* experts, int64_t n, int k, int n_experts, int32_t* slots, int32_t* rows,
                      int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream);
 size_t kmb_expert_slots_workspace_bytes(int64_t n, int k, int n_experts);
@@ -427,7 +427,8 @@ size_t kmb_expert_slots_workspace_bytes(int64_t n, int k, int n_experts);
 int kmb_combine_experts(int dtype, const void* values, int64_t n_values, const int32_t* slots,
                         const float* weights, int64_t n, int k, int d, void* out, void* stream);
 /* grad_values (n_values, d) and grad_weights (n, k) from grad_out (n, d).  Rows that several choices share
- * get the sum of their gradients in ascending order of the choices, rows that nobody chose get zeros. */
+ * get the sum of their gradients in ascending order of the choices, rows that nobody chose get zeros.
+ * n * k < 2^31 - 4096, d < 2^30. */
 int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, const int32_t* slots,
                              const float* weights, const void* grad_out, int64_t n, int k, int d,
                              void* grad_values, float* grad_weights, void* workspace, size_t workspace_bytes,

@@ -11,6 +11,7 @@
 namespace kmb {
 
 constexpr unsigned FULL = 0xffffffffu;
+constexpr int64_t MAX_CHOICES = INT32_MAX - 4096;    // n * k: places are 32-bit numbers, grids a little longer
 
 // ================================================================================== routing
 // L lanes of a warp per token (8, 16 or 32).  Lane l of them holds the V consecutive experts l * V ..
@@ -1149,7 +1150,7 @@ int kmb_expert_slots(const int32_t* experts, int64_t n, int k, int n_experts, in
   KMB_REQUIRE(n >= 0 && k >= 1, "kmb_expert_slots: bad sizes");
   KMB_REQUIRE(n_experts >= 1 && n_experts <= SL_MAX_EXPERTS,
               "kmb_expert_slots: the number of experts must be in [1, %d], got %d", SL_MAX_EXPERTS, n_experts);
-  KMB_REQUIRE(n < (1ll << 31) / k - SL_CHUNK, "kmb_expert_slots: n * k must be below 2^31");
+  KMB_REQUIRE(n <= MAX_CHOICES / k, "kmb_expert_slots: n * k must be below 2^31 - 4096");
   KMB_REQUIRE(offsets && (n == 0 || (experts && slots && rows)), "kmb_expert_slots: NULL argument");
   const size_t need = kmb_expert_slots_workspace_bytes(n, k, n_experts);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
@@ -1209,7 +1210,7 @@ int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, co
                              void* stream) {
   KMB_REQUIRE(n >= 0 && n_values >= 0 && k >= 1 && d >= 1, "kmb_combine_experts_grad: bad sizes");
   KMB_REQUIRE(d < CB_MAX_D, "kmb_combine_experts_grad: d must be below 2^30");
-  KMB_REQUIRE(n <= (1ll << 30) && n < 0x7f7f7f7fll / k, "kmb_combine_experts_grad: n * k must be below 2^31");
+  KMB_REQUIRE(n <= MAX_CHOICES / k, "kmb_combine_experts_grad: n * k must be below 2^31 - 4096");
   if (n == 0 && n_values == 0) return KMB_OK;
   KMB_REQUIRE((n_values == 0 || (values && grad_values)) && (n == 0 || (slots && weights && grad_out && grad_weights)),
               "kmb_combine_experts_grad: NULL argument");

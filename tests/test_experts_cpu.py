@@ -103,3 +103,16 @@ def test_host_tensors_are_refused():
                  lambda: common.int8_matmul(q, x[:, 0], q, x[:, 0])):
         with pytest.raises(ValueError, match="CUDA tensor"):
             call()
+
+
+def test_number_of_choices():
+    """Up to 2^31 - 4097 choices in all, however many a token has."""
+    for n, k in (((1 << 31) - 4096, 1), (1 << 29, 4), (1, (1 << 31) - 4096), (3, 715826550)):
+        _raises(lambda l: l.kmb_expert_slots(P, n, k, 8, P, P, P, P, 1 << 40, None), "below 2\\^31 - 4096")
+        _raises(lambda l: l.kmb_combine_experts_grad(0, P, 100, P, P, P, n, k, 8, P, P, P, 1 << 20, None), "below 2\\^31 - 4096")
+    from sklearn_numba_dpex_b200 import _cabi
+
+    for n, k in (((1 << 31) - 4097, 1), (1, 600000), (1, (1 << 31) - 4097)):       # the next thing they lack is a workspace
+        if _cabi.lib.kmb_expert_slots_workspace_bytes(n, k, 8):
+            _raises(lambda l: l.kmb_expert_slots(P, n, k, 8, P, P, P, None, 0, None), "workspace", _cabi.KmbError)
+        _raises(lambda l: l.kmb_combine_experts_grad(0, P, 100, P, P, P, n, k, 8, P, P, None, 0, None), "workspace", _cabi.KmbError)

@@ -352,6 +352,20 @@ def test_expert_slots(n, k, e, kind):
         np.testing.assert_array_equal(a.cpu().numpy(), b)
 
 
+@pytest.mark.parametrize("n,k", [(0, 1 << 20), (1, 600000), (3, 700001)])
+def test_expert_slots_of_many_choices_a_token(n, k):
+    from sklearn_numba_dpex_b200.common import combine_experts_grad, expert_slots
+
+    x = np.random.default_rng(k).integers(-1, 7, (n, k)).astype(np.int32)
+    slots, rows, offsets = expert_slots(torch.from_numpy(x).cuda(), 7)
+    for a, b in zip((slots, rows, offsets), ref_slots(x, 7)):
+        np.testing.assert_array_equal(a.cpu().numpy(), b)
+    values, weights, grad = torch.ones(n * k, 1, device="cuda"), torch.full((n, k), 0.5, device="cuda"), torch.full((n, 1), 4.0, device="cuda")
+    got_v, got_w = combine_experts_grad(values, slots, weights, grad)
+    assert (got_v[: int(offsets[-1])] == 2).all() and (got_v[int(offsets[-1]):] == 0).all()
+    assert torch.equal(got_w, torch.where(slots >= 0, 4.0, 0.0))
+
+
 def test_expert_order_from_several_threads():
     """Through the C interface, which runs without the interpreter's lock: calls that need much shared memory
     beside calls that need little."""
