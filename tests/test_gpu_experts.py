@@ -281,6 +281,35 @@ def test_route_gradient_is_the_formula(dtype, n, e, k, scoring, renormalize):
     assert (np.abs(explicit.double().cpu().numpy() - want) <= bound).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_gradient_of_saturated_sigmoids(dtype, renormalize):
+    """1 - s keeps its digits: relative to it the two sigmoids are off by 6 u each (exponential 4, sum, quotient),
+    their product with the gradient and the scale by 4 more; shares and what they sum to as ever."""
+    from sklearn_numba_dpex_b200.common import route_topk, route_topk_grad
+
+    t, k = TYPES[dtype], 32
+    x = torch.stack([torch.linspace(low, low + 36, k) for low in (-40.0, -10.0, 0.0, 8.0)]).to(t)
+    grad = torch.randn(4, k, generator=torch.Generator().manual_seed(3))
+    _, experts = route_topk(x.cuda(), k, scoring="sigmoid", renormalize=renormalize, scale=2.5)
+    got = route_topk_grad(x.cuda(), experts, grad.cuda(), scoring="sigmoid", renormalize=renormalize, scale=2.5)
+    x64, at = x.double().numpy(), experts.cpu().numpy().astype(np.int64)
+    assert (np.sort(at, 1) == np.arange(k)).all()
+    g = np.zeros((4, k))
+    np.put_along_axis(g, at, grad.double().numpy() * 2.5, 1)
+    rest = 1 / (1 + np.exp(x64))
+    if renormalize:
+        share = np.stack([_shares(r, "sigmoid") for r in x64])
+        want = share * (g - (share * g).sum(1, keepdims=True)) * rest
+        bound = 256 * U * 2 * np.abs(g).max() * share * rest
+    else:
+        want = g / (1 + np.exp(-x64)) * rest
+        bound = 16 * U * np.abs(want)
+    info = torch.finfo(t)
+    bound = bound * (1 + info.eps) + info.eps / 2 * np.abs(want) + info.smallest_normal * info.eps
+    assert (np.abs(got.double().cpu().numpy() - want) <= bound).all()
+
+
 @pytest.mark.parametrize("scoring,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True),
                                                  ("sigmoid", False)])
 def test_route_gradient_is_the_slope(scoring, renormalize):
