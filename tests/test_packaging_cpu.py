@@ -4,6 +4,8 @@ and the registered object is the engine class with the protocol scikit-learn's e
 calls."""
 import importlib.metadata
 import os
+import subprocess
+import sys
 import tomllib
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -51,3 +53,44 @@ def test_package_data_names_the_library_and_the_build_hook_exists():
     assert "libkmb200.so" in meta["tool"]["setuptools"]["package-data"]["sklearn_numba_dpex_b200"]
     assert os.path.exists(os.path.join(ROOT, "setup.py"))
     assert os.path.exists(os.path.join(ROOT, "sklearn_numba_dpex_b200", "build.py"))
+
+
+WITHOUT_CALLS = """
+import sys
+sys.modules["sklearn_numba_dpex_b200._torch_calls"] = None        # as if it were not built
+import sklearn_numba_dpex_b200.kmeans.drivers
+from sklearn_numba_dpex_b200.common.random import create_xoroshiro128pp_states
+from sklearn_numba_dpex_b200.common import get_random_raw, topk, topk_idx
+from sklearn_numba_dpex_b200 import common
+assert callable(topk) and callable(topk_idx) and callable(common.topk)
+assert {"topk", "route_topk", "int8_matmul"} <= set(dir(common))
+assert not hasattr(common, "no_such_helper")
+for name in ("route_topk", "int8_matmul", "experts", "int8"):
+    try:
+        getattr(common, name)
+    except ImportError as exc:
+        assert "sklearn_numba_dpex_b200.build" in str(exc), exc
+    else:
+        raise SystemExit(name + " did not miss its extension")
+print("without-ok")
+"""
+
+
+def test_engine_and_helpers_need_no_extension():
+    """A fit with k-means++ seeding, top-k and the random helpers work without the extension of the expert calls;
+    those name the command that builds it."""
+    proc = subprocess.run([sys.executable, "-c", WITHOUT_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=600)
+    assert proc.returncode == 0 and "without-ok" in proc.stdout, proc.stdout + proc.stderr
+
+
+def test_names_of_the_helpers_are_what_their_modules_hold():
+    from sklearn_numba_dpex_b200 import common
+    from sklearn_numba_dpex_b200.common import experts, int8
+
+    for module, names in ((experts, ("route_topk", "route_topk_grad", "expert_slots", "combine_experts", "combine_experts_grad")),
+                          (int8, ("quantize_rows", "int8_matmul", "check_int8_waits"))):
+        for name in names:
+            assert getattr(common, name) is getattr(module, name)
+    held = {}
+    exec("from sklearn_numba_dpex_b200.common import *", held)
+    assert set(common.__all__) <= set(held)
