@@ -4,7 +4,7 @@ this file.
     python -m sklearn_numba_dpex_b200.build [--force] [--verbose]
 
 nvcc cross-compiles without a GPU.  Objects are rebuilt only when their source or a
-header is newer; the shared library links the CUDA runtime statically, so it has no
+header is newer, the extension also when the interpreter, torch or the command changed; the shared library links the CUDA runtime statically, so it has no
 dependency on the interpreter's own CUDA libraries.
 """
 import argparse
@@ -20,6 +20,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OBJ_DIR = os.path.join(CSRC, "build")
 LIB_PATH = os.path.join(HERE, "libkmb200.so")
 CALLS_PATH = os.path.join(HERE, "_torch_calls.so")
+CALLS_STAMP = os.path.join(OBJ_DIR, "torch_calls.stamp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -93,18 +94,35 @@ def build_calls(force=False):
     from torch.utils.cpp_extension import include_paths, library_paths
 
     src = os.path.join(CSRC, "torch_calls.cpp")
-    newest = max(os.path.getmtime(src), _headers_mtime())
-    if not force and os.path.exists(CALLS_PATH) and os.path.getmtime(CALLS_PATH) >= newest:
-        return CALLS_PATH
     includes = include_paths("cuda") + [sysconfig.get_paths()["include"], INCLUDE]
     cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", CALLS_PATH]
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DKMB_TORCH_VERSION="{torch.__version__}"',
+           src, "-o", CALLS_PATH]
     cmd += [f"-I{path}" for path in includes] + [f"-L{path}" for path in library_paths("cuda")]
     cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-L{HERE}", "-l:libkmb200.so", "-Wl,-rpath,$ORIGIN"]
+    # the extension fits one interpreter and one torch: an older file for others is no newer for its time
+    made_for = "\n".join([sys.version, torch.__version__, *cmd])
+    newest = max(os.path.getmtime(src), _headers_mtime())
+    if not force and _calls_made_for() == made_for and os.path.exists(CALLS_PATH) and os.path.getmtime(CALLS_PATH) >= newest:
+        return CALLS_PATH
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    if os.path.exists(CALLS_STAMP):
+        os.remove(CALLS_STAMP)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"g++ failed on torch_calls.cpp:\n{proc.stdout}\n{proc.stderr}")
+    with open(CALLS_STAMP, "w") as fh:
+        fh.write(made_for)
     return CALLS_PATH
+
+
+def _calls_made_for():
+    """What the extension was built for and with, as build_calls noted it."""
+    try:
+        with open(CALLS_STAMP) as fh:
+            return fh.read()
+    except OSError:
+        return None
 
 
 if __name__ == "__main__":

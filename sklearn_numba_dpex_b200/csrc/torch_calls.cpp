@@ -6,6 +6,7 @@
 // turns a C++ exception into a Python one: bad arguments into ValueError, failures of the library into the
 // exception that its status stands for (_cabi.check).
 #include <stdarg.h>
+#include <string.h>
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -358,9 +359,32 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, g_me
 
 }  // namespace
 
+// The file's name does not tell what it was built for, so the module does, before it touches anything whose layout
+// hangs on it.
+static bool built_for_this_process() {
+  const char* built = PY_VERSION;
+  const char* runs = Py_GetVersion();
+  size_t minor = strchr(strchr(built, '.') + 1, '.') - built + 1;      // "3.12."
+  if (strncmp(built, runs, minor) != 0) {
+    PyErr_Format(PyExc_ImportError, "_torch_calls was built for Python %s, this is %s", built, runs);
+    return false;
+  }
+  PyObject* torch = PyImport_ImportModule("torch");
+  PyObject* version = torch ? PyObject_GetAttrString(torch, "__version__") : nullptr;
+  const char* have = version ? PyUnicode_AsUTF8(version) : nullptr;
+  const bool same = have && strcmp(have, KMB_TORCH_VERSION) == 0;
+  if (have && !same)
+    PyErr_Format(PyExc_ImportError, "_torch_calls was built for torch %s, this is %s", KMB_TORCH_VERSION, have);
+  Py_XDECREF(version);
+  Py_XDECREF(torch);
+  return same;
+}
+
 PyMODINIT_FUNC PyInit__torch_calls() {
+  if (!built_for_this_process()) return nullptr;
   PyObject* cabi = PyImport_ImportModule("sklearn_numba_dpex_b200._cabi");
   if (!cabi) return nullptr;
+  Py_XDECREF(g_kmb_error);
   g_kmb_error = PyObject_GetAttrString(cabi, "KmbError");
   Py_DECREF(cabi);
   if (!g_kmb_error) return nullptr;

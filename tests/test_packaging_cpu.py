@@ -94,3 +94,53 @@ def test_names_of_the_helpers_are_what_their_modules_hold():
     held = {}
     exec("from sklearn_numba_dpex_b200.common import *", held)
     assert set(common.__all__) <= set(held)
+
+
+def test_extension_of_another_torch_or_interpreter_is_built_anew(tmp_path, monkeypatch):
+    """By what it was built for, not by the time of its file alone: an extension that is newer than every source
+    is kept for the same torch, and built again for another one."""
+    import torch
+
+    from sklearn_numba_dpex_b200 import build
+
+    compiled = []
+
+    def compiler(cmd, **kw):
+        compiled.append(cmd)
+        (tmp_path / "_torch_calls.so").write_bytes(b"")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build, "CALLS_PATH", str(tmp_path / "_torch_calls.so"))
+    monkeypatch.setattr(build, "OBJ_DIR", str(tmp_path))
+    monkeypatch.setattr(build, "CALLS_STAMP", str(tmp_path / "torch_calls.stamp"), raising=False)
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    build.build_calls()
+    build.build_calls()
+    assert len(compiled) == 1
+    monkeypatch.setattr(torch, "__version__", "9.9.9")
+    build.build_calls()
+    build.build_calls()
+    assert len(compiled) == 2 and any("9.9.9" in word for word in compiled[1])
+    monkeypatch.setattr(build.sys, "version", "9.9")
+    build.build_calls()
+    assert len(compiled) == 3
+    (tmp_path / "_torch_calls.so").unlink()
+    build.build_calls()
+    assert len(compiled) == 4
+
+
+OTHER_TORCH = """
+import torch
+torch.__version__ = "9.9.9"
+from sklearn_numba_dpex_b200 import common
+try:
+    common.route_topk
+except ImportError as exc:
+    assert "built for torch" in str(exc) and "9.9.9" in str(exc) and "sklearn_numba_dpex_b200.build" in str(exc), exc
+    print("refused-ok")
+"""
+
+
+def test_extension_of_another_torch_is_refused():
+    proc = subprocess.run([sys.executable, "-c", OTHER_TORCH], cwd=ROOT, capture_output=True, text=True, timeout=600)
+    assert proc.returncode == 0 and "refused-ok" in proc.stdout, proc.stdout + proc.stderr
