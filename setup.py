@@ -1,6 +1,8 @@
 """Build hook: compiles the CUDA kernels into sklearn_numba_dpex_b200/libkmb200.so (nvcc,
 sm_100a) before the package files are collected, so that `pip install .` and
 `pip install -e . --no-build-isolation` both ship the library the package cannot work without.
+Without build isolation, where torch can be imported, it also builds the extension of the expert and 8-bit calls,
+which fits that torch only.
 All metadata lives in pyproject.toml."""
 import importlib.util
 import os

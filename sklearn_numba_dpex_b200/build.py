@@ -9,6 +9,7 @@ dependency on the interpreter's own CUDA libraries.
 """
 import argparse
 import concurrent.futures
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -82,7 +83,12 @@ def build(force=False, verbose=False):
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
-    build_calls(force)
+    if importlib.util.find_spec("torch") is None:
+        # an isolated build; one against some torch that pip fetches would not fit the one at run time
+        print("torch is not installed where this build runs: the expert and 8-bit calls are left out. "
+              "`pip install --no-build-isolation .` builds them with the torch that they will run with.")
+    else:
+        build_calls(force)
     return LIB_PATH
 
 

@@ -7,4 +7,5 @@ try:
                                 quantize_rows, route_topk, route_topk_grad)
 except ImportError as exc:
     raise ImportError(f"{exc}: the calls on torch tensors are not built. Run "
-                      "`python -m sklearn_numba_dpex_b200.build`; there is no fallback.") from exc
+                      "`python -m sklearn_numba_dpex_b200.build` in a checkout, or install with "
+                      "`pip install --no-build-isolation .`; there is no fallback.") from exc

@@ -144,3 +144,22 @@ except ImportError as exc:
 def test_extension_of_another_torch_is_refused():
     proc = subprocess.run([sys.executable, "-c", OTHER_TORCH], cwd=ROOT, capture_output=True, text=True, timeout=600)
     assert proc.returncode == 0 and "refused-ok" in proc.stdout, proc.stdout + proc.stderr
+
+
+def test_build_without_torch_leaves_the_extension_out(tmp_path, monkeypatch, capsys):
+    """torch is no build requirement, which pip would fetch in a version of its own: an isolated build ships the
+    library and says how to get the rest."""
+    from sklearn_numba_dpex_b200 import build
+
+    assert not any(r.startswith("torch") for r in _declared()["build-system"]["requires"])
+    (tmp_path / "lib.so").write_bytes(b"")
+    monkeypatch.setattr(build, "OBJ_DIR", str(tmp_path))
+    monkeypatch.setattr(build, "LIB_PATH", str(tmp_path / "lib.so"))
+    monkeypatch.setattr(build, "_nvcc", lambda: "nvcc")
+    monkeypatch.setattr(build, "_compile_one", lambda nvcc, src, force, verbose: (str(tmp_path / "lib.so"), ""))
+    calls = []
+    monkeypatch.setattr(build, "build_calls", calls.append)
+    assert build.build() == str(tmp_path / "lib.so") and calls == [False]
+    monkeypatch.setattr(build.importlib.util, "find_spec", lambda name: None)
+    assert build.build() == str(tmp_path / "lib.so") and calls == [False]
+    assert "--no-build-isolation" in capsys.readouterr().out
