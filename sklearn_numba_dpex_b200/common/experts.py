@@ -13,7 +13,7 @@ A layer whose experts multiply in 8 bits reads::
 All tensors live on one CUDA device; a call is enqueued on that device's current stream, waits for nothing
 and can be captured into a CUDA graph.  `route_topk` and `combine_experts` are differentiable; a backward pass that
 is to be captured calls `route_topk_grad` and `combine_experts_grad` itself, since autograd's own nodes belong to
-the stream that first used their leaves.
+the stream that first used their leaves.  Forward mode and the transforms of `torch.func` are refused with an error.
 """
 import torch
 

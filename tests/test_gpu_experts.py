@@ -731,3 +731,31 @@ def test_refusals_on_the_gpu():
     with pytest.raises(ValueError):
         combine_experts(x.double(), e, w)
     assert torch.isfinite(route_topk(x, 2)[0]).all()
+
+
+def test_transforms_are_refused():
+    """Nothing that carries a tangent, or stands for other tensors, loses it in silence."""
+    import torch.autograd.forward_ad as forward
+
+    from sklearn_numba_dpex_b200 import common
+
+    x, slots, w = torch.randn(4, 8, device="cuda"), torch.zeros(3, 2, dtype=torch.int32, device="cuda"), torch.ones(3, 2, device="cuda")
+    q, s = common.quantize_rows(x)
+    calls = [lambda t: common.route_topk(t, 2)[0], lambda t: common.route_topk(x, 2, bias=t[0])[0],
+             lambda t: common.route_topk_grad(x, slots[:1].repeat(4, 1), t[:, :2]), lambda t: common.quantize_rows(t)[1],
+             lambda t: common.combine_experts(t, slots, w), lambda t: common.combine_experts(x, slots, t[:3, :2].contiguous()),
+             lambda t: common.combine_experts_grad(x, slots, w, t[:3])[0], lambda t: common.int8_matmul(q, t[:, 0].contiguous(), q, s),
+             lambda t: common.int8_matmul(q, s, q, s, bias=t[:, 0].contiguous())]
+    for call in calls:
+        with forward.dual_level():
+            dual = forward.make_dual(x, torch.ones_like(x))
+            with pytest.raises((NotImplementedError, RuntimeError)):
+                call(dual)
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.func.jvp(call, (x,), (x,))
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.vmap(call)(x[None].repeat(3, 1, 1))
+        call(x)
+    leaf = x.clone().requires_grad_(True)
+    with forward.dual_level(), pytest.raises((NotImplementedError, RuntimeError)):
+        common.route_topk(forward.make_dual(leaf, torch.ones_like(x)), 2)
