@@ -74,7 +74,8 @@ const char* type_name(at::ScalarType t) { return c10::toString(t); }
 at::Tensor matrix(PyObject* o, const char* name) {
   const at::Tensor& t = tensor(o, name);
   if (t.dim() != 2) bad("%s must have two dimensions, got %lld", name, (long long)t.dim());
-  return t.is_contiguous() ? t : t.contiguous();
+  const at::Tensor plain = t.is_neg() ? t.resolve_neg() : t;       // a view whose memory holds the negated values
+  return plain.is_contiguous() ? plain : plain.contiguous();
 }
 at::Tensor matrix(PyObject* o, const char* name, at::ScalarType type) {
   const at::Tensor& t = tensor(o, name);
@@ -89,7 +90,7 @@ void same_device(const at::Tensor& t, const char* name, const at::Tensor& other)
 const at::Tensor& dense(PyObject* o, const char* name, at::ScalarType type, const at::Tensor& other) {
   const at::Tensor& t = tensor(o, name);
   if (t.scalar_type() != type) bad("%s must have dtype %s, got %s", name, type_name(type), type_name(t.scalar_type()));
-  if (!t.is_contiguous()) bad("%s must be contiguous", name);
+  if (!t.is_contiguous() || t.is_neg()) bad("%s must be contiguous", name);
   same_device(t, name, other);
   return t;
 }
@@ -306,7 +307,7 @@ CALL(quantize_rows, 2) {
 // out so (as quantize_rows returns it), else a copy.
 at::Tensor pitched(const at::Tensor& t, int64_t* pitch) {
   const int64_t d = t.size(-1), dims = t.dim();
-  if (t.numel() && ((uintptr_t)t.data_ptr() & 15) == 0 && (d == 1 || t.stride(-1) == 1)) {
+  if (t.numel() && !t.is_neg() && ((uintptr_t)t.data_ptr() & 15) == 0 && (d == 1 || t.stride(-1) == 1)) {
     *pitch = t.size(-2) == 1 && (dims == 2 || t.size(0) == 1) ? round16(t.stride(-2) > d ? t.stride(-2) : d) : t.stride(-2);
     if (*pitch % 16 == 0 && *pitch >= d && (dims == 2 || t.size(0) == 1 || t.stride(0) == t.size(1) * *pitch)) return t;
   }

@@ -759,3 +759,23 @@ def test_transforms_are_refused():
     leaf = x.clone().requires_grad_(True)
     with forward.dual_level(), pytest.raises((NotImplementedError, RuntimeError)):
         common.route_topk(forward.make_dual(leaf, torch.ones_like(x)), 2)
+
+
+def test_views_that_stand_for_negated_values():
+    """The imaginary part of a conjugate is a view of memory with the other sign: of one column it is contiguous too."""
+    from sklearn_numba_dpex_b200 import common
+
+    z = torch.randn(6, 1, dtype=torch.complex64, device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    q, _ = common.quantize_rows(torch.ones(6, 1, device="cuda"))
+    slots, w = torch.arange(6, dtype=torch.int32, device="cuda")[:, None], torch.ones(6, 1, device="cuda")
+    for view in (z[:1].conj().imag, z.conj().imag, torch._neg_view(z.real.contiguous())):
+        assert view.is_neg()
+        plain, n = view.resolve_neg().clone(), view.shape[0]
+        for call in (lambda t: common.route_topk(t, 1, scoring="sigmoid", renormalize=False)[0], lambda t: common.quantize_rows(t)[0],
+                     lambda t: common.combine_experts(t, slots[:n], w[:n]), lambda t: common.combine_experts(w[:n], slots[:n], t)):
+            assert torch.equal(call(view), call(plain))
+        with pytest.raises(ValueError, match="contiguous"):
+            common.int8_matmul(q[:n], view[:, 0], q, w[:, 0])
+    eights = torch.full((4, 16), 8, dtype=torch.int8, device="cuda")
+    one = torch.ones(4, device="cuda")
+    assert (common.int8_matmul(torch._neg_view(eights), one, eights, one) == -1024).all()
