@@ -6,7 +6,7 @@ A layer whose experts multiply in 8 bits reads::
 
     weights, experts = route_topk(logits, k)
     slots, rows, offsets = expert_slots(experts, n_experts)
-    q, scales = quantize_rows(x, rows=rows)
+    q, scales = quantize_rows(x.detach(), rows=rows)              # no gradient through 8 bits
     y = int8_matmul(q, scales, w, w_scales, offsets=offsets)      # w (n_experts, n, d) int8
     out = combine_experts(y, slots, weights)
 

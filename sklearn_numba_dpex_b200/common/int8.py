@@ -1,5 +1,8 @@
 """Products in 8-bit integers with a scale for each row of both operands: a linear layer's (or the
 experts') product on the integer tensor cores.  The reference has no low-precision product.
+
+Neither call has a gradient.  Where gradients are recorded, an operand that requires one is refused: pass it
+detached, or call under `torch.no_grad()`.
 """
 import ctypes
 

@@ -9,6 +9,7 @@
 #include <string.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -263,6 +264,12 @@ CALL(combine_experts_grad, 4) {
   return wrap(std::move(gv), std::move(gw));
 }
 
+// For calls that have no gradient: what asks for one would not get it.
+void no_gradient(const at::Tensor& t, const char* name, const char* call) {
+  if (t.requires_grad() && c10::GradMode::is_enabled())
+    bad("%s requires a gradient, but %s has none: detach it, or call under torch.no_grad()", name, call);
+}
+
 int64_t round16(int64_t d) { return (d + 15) / 16 * 16; }
 
 // Row pitch of 8-bit rows of our own: whole lines of 128 bytes where that costs an eighth at most.  The product
@@ -281,6 +288,7 @@ CALL(quantize_rows, 2) {
   const at::Tensor& x0 = tensor(a[0], "x");
   if (x0.dim() != 2 || x0.size(1) < 1) bad("x must have shape (n, d) with d >= 1");
   const int code = row_code(x0.scalar_type(), "x");
+  no_gradient(x0, "x", "quantize_rows");
   const at::Tensor x = matrix(a[0], "x");
   const int64_t n = x.size(0);
   const int d = width(x.size(1), "x");
@@ -337,10 +345,13 @@ CALL(int8_matmul, 7) {
   if (xs.dim() != 1 || xs.size(0) != m) bad("a_scales must have shape (%lld,)", (long long)m);
   const auto per_feature = w.sizes().slice(0, w.dim() - 1);
   if (ws.sizes() != per_feature) bad("b_scales must have a scale for each row of b");
+  no_gradient(xs, "a_scales", "int8_matmul");
+  no_gradient(ws, "b_scales", "int8_matmul");
   const float* bias = nullptr;
   if (a[4] != Py_None) {
     const at::Tensor& b = dense(a[4], "bias", at::kFloat, x);
     if (b.sizes() != per_feature) bad("bias must have the shape of b_scales");
+    no_gradient(b, "bias", "int8_matmul");
     bias = ptr<float>(b);
   }
   const int32_t* offsets = nullptr;

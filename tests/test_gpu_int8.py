@@ -271,6 +271,26 @@ def test_refusals():
     assert int8_matmul(a[:0], sa[:0], b, sb).shape == (0, 6)
 
 
+def test_operands_that_require_a_gradient_are_refused():
+    from sklearn_numba_dpex_b200.common import int8_matmul, quantize_rows
+
+    x, bias = torch.randn(4, 32, device="cuda", requires_grad=True), torch.zeros(4, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="x requires a gradient"):
+        quantize_rows(x)
+    with torch.no_grad():
+        q, s = quantize_rows(x)
+    assert torch.equal(quantize_rows(x.detach())[0], q)
+    t = s.clone().requires_grad_(True)
+    for args, kw, name in (((q, t, q, s), {}, "a_scales"), ((q, s, q, t), {}, "b_scales"), ((q, s, q, s), dict(bias=bias), "bias")):
+        with pytest.raises(ValueError, match=name + " requires a gradient"):
+            int8_matmul(*args, **kw)
+        with torch.no_grad():
+            want = int8_matmul(*args, **kw)
+        with torch.inference_mode():
+            assert torch.equal(int8_matmul(*args, **kw), want)
+    assert not int8_matmul(q, s, q, s).requires_grad
+
+
 CHILD = textwrap.dedent("""
     import os, sys, time
     import torch
