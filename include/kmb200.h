@@ -434,6 +434,9 @@ int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, co
                              void* grad_values, float* grad_weights, void* workspace, size_t workspace_bytes,
                              void* stream);
 size_t kmb_combine_experts_grad_workspace_bytes(int64_t n_values);
+/* A larger workspace for the same call, with which the gradient of rows that several choices share costs time in
+ * proportion to their users; with the one above each such row costs a walk over all n * k choices. */
+size_t kmb_combine_experts_grad_workspace_bytes_for(int64_t n_values, int64_t n, int k);
 
 /* ---- products in 8-bit integers ------------------------------------------------------- */
 /* q[i, f] = round_half_even(127 x[r, f] / max_f |x[r, f]|) and scales[i] = max_f |x[r, f]| / 127 with

@@ -97,6 +97,7 @@ _SIGNATURES = {
     "kmb_combine_experts_grad": (c_int, [c_int, _P, c_int64, _P, _P, _P, c_int64, c_int, c_int, _P, _P,
                                          _P, c_size_t, _P]),
     "kmb_combine_experts_grad_workspace_bytes": (c_size_t, [c_int64]),
+    "kmb_combine_experts_grad_workspace_bytes_for": (c_size_t, [c_int64, c_int64, c_int]),
     "kmb_quantize_rows": (c_int, [c_int, _P, c_int64, c_int, _P, c_int64, _P, c_int64, _P, _P]),
     "kmb_int8_matmul": (c_int, [c_int, _P, c_int64, _P, _P, c_int64, _P, _P, _P, c_int, _P, c_int64,
                                 c_int, c_int, _P]),

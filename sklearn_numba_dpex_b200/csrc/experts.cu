@@ -4,6 +4,8 @@
 // top-k of topk.cu and keeps its order (greatest first, lowest index among equals, NaN greatest).
 #include <limits.h>
 
+#include <type_traits>
+
 #include "early_launch.cuh"
 #include "kmb_common.cuh"
 #include "row_types.cuh"
@@ -872,125 +874,192 @@ combine_kernel(const T* values, int64_t n_values, const int32_t* slots,
 // Gradients.  Bound by HBM: the same 8192 x 8 rows of 2048 bfloat16 take 85 us (570 MB read and written, 6.7
 // TB/s), with 4 us more for the two small kernels ahead.  A block takes CG_K choices of a token, 128 threads
 // (256 threads: 111 us).  A row of values that several choices share needs the sum of their gradients, in a fixed
-// order: `users` counts the choices of each row and `first` names the lowest of them.  The blocks of the
-// tokens write the rows with one user, the last blocks of the grid all others.
-__global__ void combine_clear_kernel(int64_t n_values, int32_t* __restrict__ users, int32_t* __restrict__ first) {
+// order.  `users` counts the choices of each row; where the workspace has room for `next`, one number for each choice,
+// `head` and `next` chain them in the order in which they came, and else `head` is the lowest of them.  The
+// blocks of the tokens write the rows with one user, the last blocks of the grid all others.
+__device__ __forceinline__ void combine_clear_row(int64_t r, int32_t* users, int32_t* head, const int32_t* next) {
+  users[r] = 0;
+  head[r] = next ? -1 : INT_MAX;
+}
+// Returns the choice that came before in the chain (or -1).
+__device__ __forceinline__ int32_t combine_note_user(int32_t c, int32_t slot, int32_t* users, int32_t* head,
+                                                     const int32_t* next) {
+  atomicAdd(&users[slot], 1);
+  if (next) return atomicExch(&head[slot], c);
+  atomicMin(&head[slot], c);
+  return -1;
+}
+
+__global__ void combine_clear_kernel(int64_t n_values, int32_t* users, int32_t* head, const int32_t* next) {
   next_grid_may_start();
   grid_dependency_wait();
   const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (r >= n_values) return;
-  users[r] = 0;
-  first[r] = INT_MAX;
+  if (r < n_values) combine_clear_row(r, users, head, next);
 }
 
-__global__ void combine_users_kernel(const int32_t* slots, int64_t total, int64_t n_values,
-                                     int32_t* __restrict__ users, int32_t* __restrict__ first) {
+__global__ void combine_users_kernel(const int32_t* slots, int64_t total, int64_t n_values, int32_t* users, int32_t* head,
+                                     int32_t* next) {
   next_grid_may_start();
   grid_dependency_wait();
   const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= total) return;
   const int slot = slots[c];
   if (slot < 0 || slot >= n_values) return;
-  atomicAdd(&users[slot], 1);
-  atomicMin(&first[slot], (int32_t)c);
+  const int32_t before = combine_note_user((int32_t)c, slot, users, head, next);
+  if (next) next[c] = before;
 }
 
-// Both for few rows and choices, in one launch.
-constexpr int CG_FEW = 8192;
-__global__ void __launch_bounds__(1024)
-combine_few_users_kernel(const int32_t* slots, int total, int n_values, int32_t* __restrict__ users,
-                         int32_t* __restrict__ first) {
+// Both for few rows and choices, in one launch and in shared memory.
+constexpr int CG_FEW = 8192, CG_FEW_THREADS = 1024;
+__global__ void __launch_bounds__(CG_FEW_THREADS)
+combine_few_users_kernel(const int32_t* slots, int total, int n_values, int32_t* users, int32_t* head, int32_t* next) {
+  extern __shared__ int32_t s_few[];
+  int32_t* s_users = s_few;
+  int32_t* s_head = s_few + n_values;
   next_grid_may_start();
-  grid_dependency_wait();
-  for (int r = threadIdx.x; r < n_values; r += blockDim.x) {
-    users[r] = 0;
-    first[r] = INT_MAX;
-  }
+  for (int r = threadIdx.x; r < n_values; r += CG_FEW_THREADS) combine_clear_row(r, s_users, s_head, next);
   __syncthreads();
-  for (int c = threadIdx.x; c < total; c += blockDim.x) {
+  grid_dependency_wait();
+  for (int c = threadIdx.x; c < total; c += CG_FEW_THREADS) {
     const int slot = slots[c];
     if (slot < 0 || slot >= n_values) continue;
-    atomicAdd(&users[slot], 1);
-    atomicMin(&first[slot], c);
+    const int32_t before = combine_note_user(c, slot, s_users, s_head, next);
+    if (next) next[c] = before;
+  }
+  __syncthreads();
+  for (int r = threadIdx.x; r < n_values; r += CG_FEW_THREADS) {
+    users[r] = s_users[r];
+    head[r] = s_head[r];
   }
 }
 
-// The rows that have no user or several: zeros, or the sum over the users, which are found by walking the
-// choices from the lowest of them on, a block's width at a time, and added in ascending order.  Block `block`
-// of `blocks` looks at as many rows at once as it has threads.
+// acc += the gradients of the `found` choices in `list`, in its order.
 template <typename T, bool VEC>
-__device__ __noinline__ void combine_other_rows(int64_t block, int64_t blocks, int64_t n_values,
+__device__ __forceinline__ void combine_add_users(const int32_t* list, int found, const float* weights, const T* grad_out,
+                                                  int k, int f0, int d, float (&acc)[8]) {
+  for (int q = 0; q < found; ++q) {
+    const uint32_t c = (uint32_t)list[q];
+    const float w = weights[c];
+    RowPiece<T, VEC> g;
+    g.clear();
+    g.load(grad_out + (int64_t)(c / (uint32_t)k) * d, f0, d);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, to_float(g.t[i]), acc[i]);
+  }
+}
+
+// The rows that have no user or several: zeros, or the sum over the users in ascending order.  A row's users come
+// from its chain, which one thread follows (0.6 us a user) and the block sorts; or, without chains and for rows of
+// more than `most_chained` users, from a walk over the choices, CG_WALK of them to a thread at a time (1 us for each
+// 1024).  The walk alone costs rows times choices: 4096 rows of 64 users and 64 floats took 189 ms with it, 0.31 with
+// chains; one row of 65 536 users takes 8.4 ms.  Block `block` of `blocks` looks at `batch` rows at once.
+constexpr int CG_LIST = 2048, CG_WALK = 8;
+static_assert(CG_LIST >= CG_THREADS * CG_WALK, "the choices of one step of the walk may all be users");
+template <typename T, bool VEC>
+__device__ __noinline__ void combine_other_rows(int64_t block, int64_t blocks, int batch, int64_t n_values,
                                                 const int32_t* slots, const float* weights,
                                                 const T* grad_out, int64_t choices, int k, int d,
-                                                const int32_t* users, const int32_t* first,
-                                                T* __restrict__ grad_values) {
+                                                const int32_t* users, const int32_t* head, const int32_t* next,
+                                                int most_chained, T* __restrict__ grad_values) {
   typedef RowPiece<T, VEC> Piece;
-  __shared__ int32_t list[CG_THREADS], other[CG_THREADS];
-  __shared__ int list_n[CG_THREADS / 32], other_n[CG_THREADS / 32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int64_t base = block * blockDim.x; base < n_values; base += blocks * blockDim.x) {
+  __shared__ int32_t list[CG_LIST], other[CG_THREADS];
+  __shared__ int list_n[CG_WALK][CG_THREADS / 32], other_n[CG_THREADS / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)blockDim.x / 32;
+  const unsigned below = (1u << lane) - 1u;
+  for (int64_t base = block * batch; base < n_values; base += blocks * batch) {
     const int64_t mine = base + threadIdx.x;
-    const bool odd = mine < n_values && users[mine] != 1;
+    const bool odd = (int)threadIdx.x < batch && mine < n_values && users[mine] != 1;
+    if (!__syncthreads_or(odd)) continue;
     const unsigned odd_m = __ballot_sync(FULL, odd);
-    __syncthreads();
     if (lane == 0) other_n[warp] = __popc(odd_m);
     __syncthreads();
     int place = 0, others = 0;
-    for (int q = 0; q < (int)blockDim.x / 32; ++q) {
+    for (int q = 0; q < warps; ++q) {
       if (q < warp) place += other_n[q];
       others += other_n[q];
     }
-    if (odd) other[place + __popc(odd_m & ((1u << lane) - 1u))] = (int32_t)threadIdx.x;
+    if (odd) other[place + __popc(odd_m & below)] = (int32_t)threadIdx.x;
     __syncthreads();
     for (int o = 0; o < others; ++o) {
       const int64_t r = base + other[o];
       const int count = users[r];
+      const bool chained = next != nullptr && count <= most_chained;
+      if (chained && count > 0) {
+        int size = 1;
+        while (size < count) size *= 2;
+        if (threadIdx.x == 0)
+          for (int q = 0, c = head[r]; q < count; ++q, c = next[c]) list[q] = c;
+        for (int q = count + threadIdx.x; q < size; q += blockDim.x) list[q] = INT_MAX;
+        __syncthreads();
+        // bitonic: runs of `run` places are sorted, up and down in turn
+        for (int run = 2; run <= size; run *= 2)
+          for (int gap = run / 2; gap > 0; gap /= 2) {
+            for (int q = threadIdx.x; q < size; q += blockDim.x)
+              if (!(q & gap)) {
+                const int a = list[q], b = list[q + gap];
+                if ((a > b) == ((q & run) == 0)) {
+                  list[q] = b;
+                  list[q + gap] = a;
+                }
+              }
+            __syncthreads();
+          }
+      }
       for (int f0 = 0; f0 < d; f0 += Piece::span()) {
         const bool in = Piece::at(f0, 0) < d;
         float acc[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-        int left = count;
-        for (int64_t cb = count ? first[r] : choices; left > 0 && cb < choices; cb += blockDim.x) {
-          const int64_t c = cb + threadIdx.x;
-          const bool hit = c < choices && slots[c] == r;
-          const unsigned m = __ballot_sync(FULL, hit);
-          if (lane == 0) list_n[warp] = __popc(m);
-          __syncthreads();
-          int at = 0, found = 0;
-          for (int q = 0; q < (int)blockDim.x / 32; ++q) {
-            if (q < warp) at += list_n[q];
-            found += list_n[q];
-          }
-          if (hit) list[at + __popc(m & ((1u << lane) - 1u))] = (int32_t)(c - cb);
-          __syncthreads();
-          if (in)
-            for (int q = 0; q < found; ++q) {
-              const int64_t cc = cb + list[q];
-              const float w = weights[cc];
-              Piece g;
-              g.clear();
-              g.load(grad_out + (cc / k) * d, f0, d);
+        if (chained) {
+          if (in) combine_add_users<T, VEC>(list, count, weights, grad_out, k, f0, d, acc);
+        } else {
+          int left = count;
+          for (int64_t cb = next ? 0 : count ? head[r] : choices; left > 0 && cb < choices; cb += CG_WALK * blockDim.x) {
+            unsigned m[CG_WALK];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, to_float(g.t[i]), acc[i]);
+            for (int u = 0; u < CG_WALK; ++u) {
+              const int64_t c = cb + u * blockDim.x + threadIdx.x;
+              m[u] = __ballot_sync(FULL, c < choices && slots[c] == r);
             }
-          left -= found;
-          __syncthreads();
-        }
-        Piece o;
+            if (lane == 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o.t[i] = from_float<T>(acc[i]);
-        if (in) o.store(grad_values + r * d, f0, d);
+              for (int u = 0; u < CG_WALK; ++u) list_n[u][warp] = __popc(m[u]);
+            }
+            __syncthreads();
+            int found = 0;
+#pragma unroll
+            for (int u = 0; u < CG_WALK; ++u)
+              for (int q = 0; q < warps; ++q) {
+                if (q == warp && ((m[u] >> lane) & 1u))
+                  list[found + __popc(m[u] & below)] = (int32_t)(cb + u * blockDim.x + threadIdx.x);
+                found += list_n[u][q];
+              }
+            __syncthreads();
+            if (in) combine_add_users<T, VEC>(list, found, weights, grad_out, k, f0, d, acc);
+            left -= found;
+            __syncthreads();
+          }
+        }
+        Piece out;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out.t[i] = from_float<T>(acc[i]);
+        if (in) out.store(grad_values + r * d, f0, d);
       }
+      __syncthreads();       // the list is free again
     }
   }
 }
 
+// Nine blocks on an SM where the registers of the token's part allow it, eight else; the other rows' part
+// takes what that leaves (64 registers for both, and so eight blocks, took 94 us where nine take 92).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(CG_THREADS, 8)
+constexpr int combine_grad_blocks() { return VEC && std::is_same<T, __nv_bfloat16>::value ? 9 : 8; }
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(CG_THREADS, (combine_grad_blocks<T, VEC>()))
 combine_grad_kernel(const T* values, int64_t n_values, const int32_t* slots,
                     const float* weights, const T* grad_out, int64_t n, int k, int d,
-                    const int32_t* users, const int32_t* first,
+                    const int32_t* users, const int32_t* head, const int32_t* next, int most_chained, int batch,
                     T* __restrict__ grad_values, float* __restrict__ grad_weights, int64_t token_blocks) {
   typedef RowPiece<T, VEC> Piece;
   __shared__ float red[CG_THREADS / 32][CG_K];
@@ -998,8 +1067,8 @@ combine_grad_kernel(const T* values, int64_t n_values, const int32_t* slots,
   next_grid_may_start();
   grid_dependency_wait();
   if ((int64_t)blockIdx.x >= token_blocks) {
-    combine_other_rows<T, VEC>((int64_t)blockIdx.x - token_blocks, (int64_t)gridDim.x - token_blocks, n_values, slots,
-                               weights, grad_out, n * k, k, d, users, first, grad_values);
+    combine_other_rows<T, VEC>((int64_t)blockIdx.x - token_blocks, (int64_t)gridDim.x - token_blocks, batch, n_values,
+                               slots, weights, grad_out, n * k, k, d, users, head, next, most_chained, grad_values);
     return;
   }
   // a block takes CG_K choices of a token
@@ -1205,6 +1274,11 @@ size_t kmb_combine_experts_grad_workspace_bytes(int64_t n_values) {
   return n_values < 0 ? 0 : (size_t)n_values * 2 * sizeof(int32_t);
 }
 
+size_t kmb_combine_experts_grad_workspace_bytes_for(int64_t n_values, int64_t n, int k) {
+  if (n < 0 || k < 1 || n > MAX_CHOICES / k) return 0;
+  return n_values <= 0 ? 0 : kmb_combine_experts_grad_workspace_bytes(n_values) + (size_t)(n * k) * sizeof(int32_t);
+}
+
 int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, const int32_t* slots,
                              const float* weights, const void* grad_out, int64_t n, int k, int d,
                              void* grad_values, float* grad_weights, void* workspace, size_t workspace_bytes,
@@ -1222,31 +1296,48 @@ int kmb_combine_experts_grad(int dtype, const void* values, int64_t n_values, co
   }
   cudaStream_t s = (cudaStream_t)stream;
   int32_t* users = (int32_t*)workspace;
-  int32_t* first = users + n_values;
+  int32_t* head = users + n_values;
+  int32_t* next = n > 0 && workspace_bytes >= kmb_combine_experts_grad_workspace_bytes_for(n_values, n, k)
+                      ? head + n_values : nullptr;
   if (n_values > 0 && n_values <= CG_FEW && n * k <= CG_FEW) {
-    const int rc = launch_early(combine_few_users_kernel, 1, 1024, 0, 1, s, slots, n * k, n_values, users, first);
+    const size_t smem = (size_t)n_values * 2 * sizeof(int32_t);
+    if (smem > 48 * 1024)      // every call that needs a limit sets the same one
+      KMB_CHECK_CUDA(cudaFuncSetAttribute(combine_few_users_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          CG_FEW * 2 * (int)sizeof(int32_t)));
+    const int rc = launch_early(combine_few_users_kernel, 1, CG_FEW_THREADS, smem, 1, s, slots, n * k, n_values, users,
+                                head, next);
     if (rc != KMB_OK) return rc;
   } else {
     if (n_values > 0) {
       const int rc = launch_early(combine_clear_kernel, (unsigned)ceil_div(n_values, 256), 256, 0, 1, s, n_values, users,
-                                  first);
+                                  head, next);
       if (rc != KMB_OK) return rc;
     }
     if (n > 0) {
       const int rc = launch_early(combine_users_kernel, (unsigned)ceil_div(n * k, 256), 256, 0, 1, s, slots, n * k,
-                                  n_values, users, first);
+                                  n_values, users, head, next);
       if (rc != KMB_OK) return rc;
     }
   }
+  // a user found by its chain costs as much as 512 choices walked over
+  const int64_t chained = n * k / 512 > 32 ? n * k / 512 : 32;
+  const int most_chained = (int)(chained < CG_LIST ? chained : CG_LIST);
   KMB_DISPATCH_ROWS(dtype, {
     const int vec = rows_are_vec((const T*)values, d) && rows_are_vec((const T*)grad_out, d) &&
                     rows_are_vec((const T*)grad_values, d);
-    const int64_t fill = n_values == 0 ? 0 : (ceil_div(n_values, 64) < sm_count() ? ceil_div(n_values, 64) : sm_count());
     const unsigned threads = combine_threads(d, CG_THREADS);
+    // Blocks for the rows without a user or with several: up to four to an SM, each with as few rows at a time as that
+    // gives, but sixteen where rows have few users (1000 rows, one user each: 500 such blocks cost 0.5 us more than 63).
+    const int64_t most = (int64_t)sm_count() * 4;
+    int64_t rows = ceil_div(n_values, most);
+    if (rows < 16 && n * k <= n_values * 4) rows = 16;
+    if (rows > (int64_t)threads) rows = threads;
+    const int64_t fill = n_values == 0 ? 0 : (ceil_div(n_values, rows) < most ? ceil_div(n_values, rows) : most);
     const int64_t token_blocks = n * ceil_div(k, CG_K);
     return launch_early(vec ? combine_grad_kernel<T, true> : combine_grad_kernel<T, false>,
                         (unsigned)(token_blocks + fill), (int)threads, 0, 1, s, (const T*)values, n_values, slots,
-                        weights, (const T*)grad_out, n, k, d, users, first, (T*)grad_values, grad_weights, token_blocks);
+                        weights, (const T*)grad_out, n, k, d, users, head, next, most_chained, (int)rows,
+                        (T*)grad_values, grad_weights, token_blocks);
   });
 }
 

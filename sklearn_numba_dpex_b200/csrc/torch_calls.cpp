@@ -255,7 +255,7 @@ CALL(combine_experts_grad, 4) {
   same_device(grad, "grad_out", c.values);
   c10::cuda::CUDAGuard guard(c.values.device());
   at::Tensor gv = empty(c.values.sizes(), c.values.scalar_type(), c.values), gw = empty({c.n, c.k}, at::kFloat, c.values);
-  const size_t bytes = kmb_combine_experts_grad_workspace_bytes(c.values.size(0));
+  const size_t bytes = kmb_combine_experts_grad_workspace_bytes_for(c.values.size(0), c.n, c.k);
   at::Tensor ws = empty({(int64_t)bytes}, at::kByte, c.values);
   check(kmb_combine_experts_grad(c.code, ptr(c.values), c.values.size(0), ptr<int32_t>(c.slots), ptr<float>(c.weights),
                                  ptr(grad), c.n, c.k, c.d, ptr(gv), ptr<float>(gw), ptr(ws), bytes,

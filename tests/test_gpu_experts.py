@@ -551,6 +551,99 @@ def test_combine_many_users_of_one_row():
     assert ((got_v.double().cpu() - gv).abs() <= (n * k + 1) * U * big_v).all()
 
 
+def _shared_slots(kind, n, k, m, gen):
+    """(n, k) rows of m: every row named by some; all the choices on one; rows of 2, 31 to 33, 64 and 65, 127 to 129 and more
+    users among rows of one and none."""
+    if kind == "random":
+        return torch.randint(-1, m, (n, k), generator=gen)
+    if kind == "one":
+        return torch.full((n, k), m // 2)
+    users = torch.ones(m, dtype=torch.int64)
+    users[::5] = 0
+    for i, c in enumerate((2, 3, 31, 32, 33, 64, 65, 127, 128, 129, 500, n * k // 8)):
+        users[i * (m // 13)] = c
+    flat = torch.repeat_interleave(torch.arange(m), users)[: n * k]
+    flat = torch.cat([flat, torch.full((n * k - flat.numel(),), -1)])
+    return flat[torch.randperm(n * k, generator=gen)].view(n, k)
+
+
+def _grad_of_values(slots, weights, grad, m):
+    """In 64 bits, with the sum of the magnitudes and the number of users of each row."""
+    there = slots >= 0
+    at = slots.long()[there]
+    rows = (weights.double()[..., None] * grad.double()[:, None])[there]
+    out, big = (torch.zeros(m, grad.shape[1], dtype=torch.float64, device=rows.device) for _ in range(2))
+    return out.index_add_(0, at, rows), big.index_add_(0, at, rows.abs()), torch.bincount(at, minlength=m)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,m,d", [(50, 3, 40, 5), (1000, 8, 700, 24), (1024, 8, 8192, 16), (1025, 8, 900, 130), (5003, 7, 9001, 33),
+                                     (9000, 8, 40000, 8), (3000, 6, 30, 1100)])
+@pytest.mark.parametrize("kind", ["random", "one", "mixed"])
+def test_combine_gradient_of_shared_rows(dtype, n, k, m, d, kind):
+    """Sums over the users of a row, however they are found: one chain after the other, or by a walk over the choices.
+    The order of the sum is that of the choices: the same bits every time, with either workspace."""
+    from sklearn_numba_dpex_b200 import _cabi
+    from sklearn_numba_dpex_b200.common import combine_experts_grad
+
+    t, gen = TYPES[dtype], torch.Generator().manual_seed(n + m)
+    slots = _shared_slots(kind, n, k, m, gen).to(torch.int32).cuda()
+    values, grad = torch.randn(m, d, generator=gen).to(t).cuda(), torch.randn(n, d, generator=gen).to(t).cuda()
+    weights = torch.randn(n, k, generator=gen).cuda()
+    got, got_w = combine_experts_grad(values, slots, weights, grad)
+    want, big, users = _grad_of_values(slots, weights, grad, m)
+    info = torch.finfo(t)
+    bound = (users[:, None] + 1) * U * big + info.eps / 2 * want.abs() * (1 + 2.0 ** -9) + info.smallest_normal * info.eps
+    assert ((got.double() - want).abs() <= bound).all()
+    for _ in range(3):
+        again = combine_experts_grad(values, slots, weights, grad)
+        assert torch.equal(again[0], got) and torch.equal(again[1], got_w)
+    lib, small = _cabi.lib, torch.empty_like(got).fill_(7)
+    size = lib.kmb_combine_experts_grad_workspace_bytes(m)
+    assert size < lib.kmb_combine_experts_grad_workspace_bytes_for(m, n, k)
+    ws, small_w = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty_like(got_w)
+    code = {"fp32": _cabi.KMB_F32, "fp16": _cabi.KMB_F16, "bf16": _cabi.KMB_BF16}[dtype]
+    p = _cabi.ptr
+    _cabi.check(lib.kmb_combine_experts_grad(code, p(values), m, p(slots), p(weights), p(grad), n, k, d, p(small), p(small_w),
+                                             p(ws), size, _cabi.stream_ptr()), "kmb_combine_experts_grad")
+    assert torch.equal(small, got) and torch.equal(small_w, got_w)
+
+
+def test_combine_gradient_of_the_longest_chains():
+    """A million choices, rows of 2047, 2048 and 2049 users among rows of few and one of half a million."""
+    from sklearn_numba_dpex_b200.common import combine_experts_grad
+
+    n, k, d, gen = 1 << 17, 8, 8, torch.Generator().manual_seed(5)
+    users = torch.cat([torch.tensor([2047, 2048, 2049, 0, 1, 4095, 500000]), torch.full((100000,), 2), torch.full((3000,), 60)])
+    flat = torch.repeat_interleave(torch.arange(users.numel()), users)
+    assert flat.numel() <= n * k
+    flat = torch.cat([flat, torch.full((n * k - flat.numel(),), -1)])[torch.randperm(n * k, generator=gen)]
+    slots, m = flat.view(n, k).to(torch.int32).cuda(), users.numel()
+    weights, grad = torch.randn(n, k, generator=gen).cuda(), torch.randn(n, d, generator=gen).cuda()
+    got, _ = combine_experts_grad(torch.zeros(m, d, device="cuda"), slots, weights, grad)
+    want, big, _ = _grad_of_values(slots, weights, grad, m)
+    assert ((got.double() - want).abs() <= (users.cuda()[:, None] + 1) * U * big + 2.0 ** -24 * want.abs()).all()
+
+
+def test_combine_gradient_costs_what_its_users_cost():
+    """4096 rows of 64 users, which took 189 ms where each row meant a walk over all choices; read, their gradients
+    are 67 MB."""
+    from sklearn_numba_dpex_b200.common import combine_experts_grad
+
+    n, k, d, m = 32768, 8, 64, 4096
+    slots = torch.arange(n * k, device="cuda")[torch.randperm(n * k, device="cuda")].view(n, k).remainder(m).to(torch.int32)
+    values, weights, grad = torch.randn(m, d, device="cuda"), torch.randn(n, k, device="cuda"), torch.randn(n, d, device="cuda")
+    times = []
+    for _ in range(3):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        combine_experts_grad(values, slots, weights, grad)
+        end.record()
+        torch.cuda.synchronize()
+        times.append(start.elapsed_time(end))
+    assert min(times) < 10, times
+
+
 # --------------------------------------------------------------------------- used together
 def _layer(x, logits, w, w_scales, k, n_experts):
     from sklearn_numba_dpex_b200 import common
