@@ -381,6 +381,16 @@ def test_expert_slots(n, k, e, kind):
         np.testing.assert_array_equal(a.cpu().numpy(), b)
 
 
+@pytest.mark.parametrize("n,k,e", [(131073, 8, 33), (300007, 8, 129), (1200000, 2, 1024)])
+def test_expert_slots_of_many_chunks(n, k, e):
+    """More chunks of 4096 choices than the scan takes at a time (256): what it carries on."""
+    from sklearn_numba_dpex_b200.common import expert_slots
+
+    x = np.random.default_rng(n).integers(-1, e, (n, k)).astype(np.int32)
+    for a, b in zip(expert_slots(torch.from_numpy(x).cuda(), e), ref_slots(x, e)):
+        np.testing.assert_array_equal(a.cpu().numpy(), b)
+
+
 @pytest.mark.parametrize("n,k", [(0, 1 << 20), (1, 600000), (3, 700001)])
 def test_expert_slots_of_many_choices_a_token(n, k):
     from sklearn_numba_dpex_b200.common import combine_experts_grad, expert_slots
