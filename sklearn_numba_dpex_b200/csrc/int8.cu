@@ -257,6 +257,7 @@ struct I8Smem {
   int scan[I8_SCAN_THREADS / 32];
   float sa[BN];
   int bad;                             // SPLIT: this CTA's partial sums are not to be used
+  int far;                             // SPLIT: a scale of the tile's tokens lies far from 1
   unsigned long long full[Cfg::STAGES], empty[Cfg::STAGES];
   unsigned long long acc_full[2], acc_empty[2], drain;
   long long timeout_cycles;
@@ -434,14 +435,56 @@ __device__ __forceinline__ int load_from(const void* p, uint32_t rank) {
   return v;
 }
 
+// Barrier of the storing warps; whether any of their threads says so.
+__device__ __forceinline__ bool i8_any_of_storing_warps(bool mine) {
+  static_assert(I8_EPI_WARPS * 32 == 256, "the barrier's count");
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"((uint32_t)mine)
+      : "memory");
+  return any != 0;
+}
+// Whether a product with this scale may leave the range of 32 bits although the result does not: the other scale
+// lies within 2^60 of 1 then, or is such a one itself.  (Infinities and NaN come out the same either way.)
+__device__ __forceinline__ bool i8_far(float scale) {
+  const float a = fabsf(scale);
+  return (a > 0x1p60f && a < INFINITY) || (a < 0x1p-60f && a != 0.f);
+}
+// One result.  FAR: in 64 bits, rounded once to 32.
+template <bool FAR, typename T>
+__device__ __forceinline__ T i8_scaled(int sum, float sa, float sb, float bias) {
+  if (FAR) return from_float<T>((float)((double)sum * (double)sa * (double)sb + (double)bias));
+  return from_float<T>((float)sum * (sa * sb) + bias);
+}
+
 // Scales COLS accumulator columns (tokens) of one feature and stores them; FULL: all of them are rows.
 template <int COLS, bool FULL, typename T>
 __device__ __forceinline__ void i8_store(const uint32_t (&v)[COLS], const float* sa, float sb, float bias, T* o,
                                          int64_t stride, int rows) {
 #pragma unroll
   for (int j = 0; j < COLS; ++j) {
-    if (FULL || j < rows) *o = from_float<T>((float)(int)v[j] * (sa[j] * sb) + bias);
+    if (FULL || j < rows) *o = i8_scaled<false, T>((int)v[j], sa[j], sb, bias);
     o += stride;
+  }
+}
+// All of a warp's columns with scales far from 1, by its 32 lanes together; out of line, since inlined it made the
+// stores of every tile slower (32 groups of 512 rows, 1408 x 2048: 52.8 -> 53.9 us).
+template <typename T>
+__device__ __noinline__ void i8_store_far(uint32_t acc, int cols, const float* sa, float sb, float bias, T* o,
+                                          int64_t stride, int rows) {
+#pragma unroll 1
+  for (int c = 0; c < cols; c += 16) {
+    uint32_t v[16];
+    tmem_ld16(acc + c, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (c + j < rows) o[(c + j) * stride] = i8_scaled<true, T>((int)v[j], sa[c + j], sb, bias);
   }
 }
 
@@ -478,6 +521,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     sm->timeout_cycles = p.timeout_cycles;
     sm->abort_flag = 0;
     sm->bad = 0;
+    sm->far = 0;
     fence_barrier_init();
   }
   if (warp == 2) {
@@ -658,13 +702,18 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       const I8Tile tile = i8_tile<BN>(p, sm->first_tile, t, wide, skip);
       const uint32_t ab = nt & 1u;
       asm volatile("bar.sync 1, 256;" ::: "memory");   // everybody is done with the last tile's scales
-      for (int r = etid; r < BN; r += EPI) sm->sa[r] = r < tile.rows ? p.sa[tile.row0 + r] : 0.f;
+      bool far = false;
+      for (int r = etid; r < BN; r += EPI) {
+        const float sa = r < tile.rows ? p.sa[tile.row0 + r] : 0.f;
+        sm->sa[r] = sa;
+        far = far || i8_far(sa);
+      }
       const int feature = tile.feature0 + q * 32 + lane;
       const bool mine = feature < p.n;
       const int64_t wrow = (int64_t)tile.g * p.n + feature;
       float sb = mine ? p.sb[wrow] : 0.f;
       const float bias = (mine && p.bias) ? p.bias[wrow] : 0.f;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      far = i8_any_of_storing_warps(far);      // and the scales of the tile's tokens are there
       ok = ok && __all_sync(0xffffffffu, i8_wait(&sm->acc_full[ab], (nt >> 1) & 1u, sm));
       tc_fence_after();
       const uint32_t acc = tmem_base + ab * BN + ((uint32_t)(q * 32) << 16);
@@ -672,6 +721,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         // partial sums [token][feature] into the stages, which nobody needs any more
         int* part = reinterpret_cast<int*>(sm->a[0]);
         if (!ok && lane == 0) sm->bad = 1;
+        if (far && etid == 0) sm->far = 1;
         if (works) {
 #pragma unroll 1
           for (int c = 0; c < MINE && col0 + c < tile.rows; c += 16) {
@@ -687,14 +737,18 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         if (works) {
           T* o = out + (tile.row0 + col0) * p.n + feature;
           const int rows = mine ? tile.rows - col0 : 0;
+          if (__any_sync(0xffffffffu, far || i8_far(sb))) {
+            i8_store_far<T>(acc + col0, MINE < tile.rows - col0 ? MINE : tile.rows - col0, sm->sa + col0, sb, bias, o, p.n, rows);
+          } else {
 #pragma unroll 1
-          for (int c = 0; c < MINE && col0 + c < tile.rows; c += COLS, o += (int64_t)COLS * p.n) {
-            uint32_t v[COLS];
-            if constexpr (COLS == 32) tmem_ld32(acc + col0 + c, v);
-            else tmem_ld16(acc + col0 + c, v);
-            tmem_ld_wait();
-            if (rows - c >= COLS) i8_store<COLS, true>(v, sm->sa + col0 + c, sb, bias, o, p.n, 0);
-            else i8_store<COLS, false>(v, sm->sa + col0 + c, sb, bias, o, p.n, rows - c);
+            for (int c = 0; c < MINE && col0 + c < tile.rows; c += COLS, o += (int64_t)COLS * p.n) {
+              uint32_t v[COLS];
+              if constexpr (COLS == 32) tmem_ld32(acc + col0 + c, v);
+              else tmem_ld16(acc + col0 + c, v);
+              tmem_ld_wait();
+              if (rows - c >= COLS) i8_store<COLS, true>(v, sm->sa + col0 + c, sb, bias, o, p.n, 0);
+              else i8_store<COLS, false>(v, sm->sa + col0 + c, sb, bias, o, p.n, rows - c);
+            }
           }
         }
       }
@@ -723,6 +777,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const int64_t wrow = (int64_t)tile.g * p.n + feature;
         const float sb = bad ? __uint_as_float(0x7fffffffu) : p.sb[wrow];
         const float bias = p.bias ? p.bias[wrow] : 0.f;
+        const bool far = sm->far != 0 || i8_far(sb);
         // this warp's tokens: every 2 * splits-th of the tile, AT_ONCE of them in flight from each CTA
         constexpr int AT_ONCE = BN >= 64 ? 8 : 4;
         const int hop = splits * 2;
@@ -744,7 +799,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             const int c = c0 + u * hop;
             if (c < tile.rows)
               reinterpret_cast<T*>(p.out)[(tile.row0 + c) * p.n + feature] =
-                  from_float<T>((float)sum[u] * (sm->sa[c] * sb) + bias);
+                  far ? i8_scaled<true, T>(sum[u], sm->sa[c], sb, bias) : i8_scaled<false, T>(sum[u], sm->sa[c], sb, bias);
           }
         }
       }

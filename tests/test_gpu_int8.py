@@ -120,6 +120,40 @@ def test_product_sizes(m, n, d, out):
         _check(got, want, size)
 
 
+# a tile to a CTA, clusters that share one, pairs of CTAs, groups
+@pytest.mark.parametrize("m,n,d,g", [(3, 8, 32, None), (300, 512, 64, None), (1, 4096, 4096, None), (2, 4096, 4096, None), (40, 300, 3000, None), (4000, 2700, 136, None),
+                                     (700, 130, 48, 5)])
+@pytest.mark.parametrize("out", TYPES)
+def test_product_of_scales_far_from_one(m, n, d, g, out):
+    """Scales whose product leaves the range of 32 bits, or its full precision, where the result does not.  A result
+    beyond the type's greatest value is an infinity; one below its normal numbers is off by half a step there."""
+    from sklearn_numba_dpex_b200.common import int8_matmul
+
+    a, sa, b, sb, c = _operands(m, n, d, g=g, seed=d, bias=True)
+    gen = torch.Generator().manual_seed(m)
+    a[0] = 0                                  # a sum of zero stays the bias alone
+    sa = 10.0 ** (torch.rand(m, generator=gen, dtype=torch.float64) * 70 - 36)
+    sb = 10.0 ** (torch.rand(sb.shape, generator=gen, dtype=torch.float64) * 70 - 36)
+    sa, sb, c = sa.float(), sb.float(), torch.where(torch.rand(c.shape, generator=gen) < 0.5, torch.zeros(()), c * 1e-30)
+    sa[0] = 1e30
+    t = TYPES[out]
+    off = None if g is None else torch.tensor([i * m // g for i in range(g + 1)], dtype=torch.int32)
+    if g is None:
+        want, size = ref_product(a, sa, b, sb, c)
+    else:
+        parts = [ref_product(a[off[i]:off[i + 1]], sa[off[i]:off[i + 1]], b[i], sb[i], c[i]) for i in range(g)]
+        want, size = (torch.cat([p[j] for p in parts]) for j in (0, 1))
+    got = int8_matmul(a.cuda(), sa.cuda(), b.cuda(), sb.cuda(), bias=c.cuda(), offsets=None if g is None else off.cuda(), out_dtype=t).double().cpu()
+    info = torch.finfo(t)
+    tiny = max(info.smallest_normal * info.eps, 2.0 ** -149)
+    bound = 4 * U * size + info.eps / 2 * want.abs() * (1 + 4 * U) + tiny
+    over = want.abs() + 4 * U * size > info.max        # may round to an infinity
+    must = want.abs() - 4 * U * size > info.max * (1 + info.eps)
+    assert not torch.isnan(got).any() and not torch.isinf(got[~over]).any() and torch.isinf(got[must]).all()
+    assert ((got - want).abs() <= bound)[~over].all()
+    assert (got[0].abs() <= 1e-20).all()
+
+
 def test_product_of_the_longest_rows_does_not_overflow():
     from sklearn_numba_dpex_b200.common import int8_matmul
 
