@@ -387,6 +387,14 @@ __device__ __forceinline__ int64_t i8_row_of(const I8Params& p, int g) {
   return o < 0 ? 0 : (o > p.m ? p.m : o);
 }
 
+// Sum of two numbers of tiles.  Offsets that go up and down may name every row once for each group, more tiles than
+// 32 bits hold; the sum then stays at the greatest number there is, so that every tile lies in its group all the same.
+constexpr int I8_MAX_TILES = 1 << 30;
+__device__ __forceinline__ int i8_add_tiles(int a, int b) {
+  const unsigned sum = (unsigned)a + (unsigned)b;          // both are at most 2^30
+  return sum < (unsigned)I8_MAX_TILES ? (int)sum : I8_MAX_TILES;
+}
+
 struct I8Tile {
   int g;
   int64_t row0;     // first token row
@@ -553,24 +561,25 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const int64_t rows = i8_row_of(p, g + 1) - i8_row_of(p, g);
         cnt[j] = rows > 0 ? (int)((rows + BN - 1) / BN) * p.feature_tiles : 0;
       }
-      sum += cnt[j];
+      sum = i8_add_tiles(sum, cnt[j]);
     }
     int inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
+      if (lane >= o) inc = i8_add_tiles(inc, v);
     }
     if (scans && lane == 31) sm->scan[warp] = inc;
+    const int ahead = __shfl_up_sync(0xffffffffu, inc, 1);
     __syncthreads();
     if (scans) {
-      int base = inc - sum;
-      for (int w = 0; w < warp; ++w) base += sm->scan[w];
+      int base = lane > 0 ? ahead : 0;
+      for (int w = 0; w < warp; ++w) base = i8_add_tiles(base, sm->scan[w]);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         const int g = threadIdx.x * PER + j;
         if (g <= p.groups) sm->first_tile[g] = base;
-        base += cnt[j];
+        base = i8_add_tiles(base, cnt[j]);
       }
       if (threadIdx.x == I8_SCAN_THREADS - 1 && p.groups == I8_MAX_GROUPS) sm->first_tile[I8_MAX_GROUPS] = base;
     }
@@ -909,7 +918,7 @@ static I8Plan i8_plan(int64_t m, int groups, int n, int d) {
 template <int BN, typename T>
 int i8_run_as(const I8Plan& plan, const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, I8Params p,
               cudaStream_t s) {
-  KMB_REQUIRE(plan.tiles < (1ll << 31), "kmb_int8_matmul: too many output tiles");
+  KMB_REQUIRE(plan.tiles < I8_MAX_TILES, "kmb_int8_matmul: too many output tiles");
   const int sms = sm_count();
   CUtensorMap map_w, map_x;
   int rc = i8_make_map(&map_w, b, (int64_t)p.groups * p.n, p.d, ldb, I8_BM);

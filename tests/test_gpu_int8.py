@@ -256,6 +256,35 @@ def test_product_by_group_that_begins_late():
     assert off[0] > 0 and (got[: off[0]] == 0).all()
 
 
+@pytest.mark.parametrize("g,m,n,d", [(3, 50, 129, 64), (64, 300, 70, 144), (1024, 700, 9, 16), (20, 2500, 1100, 150)])
+def test_product_of_wrong_offsets_stays_in_its_rows(g, m, n, d):
+    """Offsets that go up and down, or lie outside the rows, give no right product, but touch nothing else: the memory
+    around the result, and the next product."""
+    from sklearn_numba_dpex_b200 import _cabi
+    from sklearn_numba_dpex_b200.common import check_int8_waits, int8_matmul
+
+    a, sa, b, sb, _ = [None if t is None else t.cuda() for t in _operands(m, n, d, g=g)]
+    good = torch.from_numpy(_group_offsets("whole", g, m, np.random.default_rng(g))).cuda()
+    want = int8_matmul(a, sa, b, sb, offsets=good, out_dtype=torch.float32)
+    lda = (d + 15) // 16 * 16
+    ap, bp = torch.zeros(m, lda, dtype=torch.int8, device="cuda"), torch.zeros(g, n, lda, dtype=torch.int8, device="cuda")
+    ap[:, :d], bp[..., :d] = a, b
+    for kind in range(4):
+        off = torch.from_numpy(np.random.default_rng(kind).integers(-m, 2 * m + 1, g + 1).astype(np.int32))
+        if kind == 0:
+            off = torch.arange(g + 1, dtype=torch.int32).remainder(2) * m           # every row once for each second group
+        elif kind == 1:
+            off = torch.arange(g, -1, -1, dtype=torch.int32)
+        off, held = off.cuda(), torch.full((m + 2, n), 7.0, device="cuda")
+        p = _cabi.ptr
+        _cabi.check(_cabi.lib.kmb_int8_matmul(_cabi.KMB_F32, p(ap), lda, p(sa), p(bp), lda, p(sb), None, p(off), g, p(held[1:]),
+                                              m, n, d, _cabi.stream_ptr()), "kmb_int8_matmul")
+        torch.cuda.synchronize()
+        assert (held[0] == 7).all() and (held[-1] == 7).all()
+        check_int8_waits()
+    assert torch.equal(int8_matmul(a, sa, b, sb, offsets=good, out_dtype=torch.float32), want)
+
+
 def test_product_whose_output_passes_32_bit_offsets():
     from sklearn_numba_dpex_b200.common import int8_matmul
 
