@@ -19,9 +19,9 @@ constexpr int64_t MAX_CHOICES = INT32_MAX - 4096;    // n * k: places are 32-bit
 // L lanes of a warp per token (8, 16 or 32).  Lane l of them holds the V consecutive experts l * V ..
 // l * V + V - 1 in registers, so that the lowest lane among equals is the lowest index.  k rounds take the
 // greatest key each: a maximum in the lane, one over the lanes, a ballot for the lowest of them.
-// Bound by instruction issue (0.69 a scheduler and cycle), not by HBM: 16 384 x 128 float32, k = 8, takes
-// 10 us (0.9 TB/s), 65 521 x 64 bfloat16, k = 6, 13 us; with a whole warp per token, whatever the number of
-// experts, 17 and 41 us.
+// Bound by the rounds, each a chain of shuffles behind the one before: neither HBM (1.0 TB/s) nor issue (0.55 to 0.65
+// a scheduler and cycle) is full.  16 384 x 128 float32, k = 8, takes 9.4 us, 65 521 x 64 bfloat16, k = 6, 13 us; with
+// a whole warp per token, whatever the number of experts, 17 and 41 us.
 constexpr int RT_WARPS = 4;
 constexpr int RT_MAX_EXPERTS = 1024;
 constexpr int RT_MAX_K = 32;       // the choices of a token live one to a lane
@@ -282,7 +282,7 @@ __device__ __forceinline__ Chosen route_token(const RouteParams& p, const T* row
 // right if the chosen of equal upper bits are equal each to the next, and no expert behind them that shares the
 // last one's upper bits is greater than that one; else the token is done again with whole keys (`unsure`: about
 // one in two hundred).  65 521 x 64 bfloat16, k = 6, took 17 us with whole keys; float32 logits gain nothing
-// (16 384 x 128, k = 8: 10 us either way), but lose nothing either.
+// (16 384 x 128, k = 8: 10 us with whole keys, 9.4 with these), but lose nothing either.
 template <typename T, int L, int V>
 __device__ __forceinline__ Chosen route_by_logit(const RouteParams& p, const T* row, const float (&x)[V], int lane) {
   constexpr bool exact = sizeof(T) == 2;
@@ -583,8 +583,8 @@ int route_grad_run(RouteGradParams p, cudaStream_t s) {
 // (match_any, which walks the distinct values, took twice as long), the warp's own counters carry the
 // rank from round to round, and the counters of the warps before it, the chunks before it and the
 // experts before it make the place.  1 048 568 choices of 256 experts take 15.6 us in three launches: 3.5
-// counting, 2.8 scanning, 10 placing, which is bound by issue (170 instructions for 32 choices), not by the
-// 12.6 MB that it moves.
+// counting, 2.8 scanning, 10 placing: 170 instructions for 32 choices at 0.55 a scheduler and cycle, in 256 blocks of
+// which some SMs get two and some one; the 12.6 MB that it moves would take 1.9.
 constexpr int SL_WARPS = 16, SL_ROUNDS = 8;
 constexpr int SL_THREADS = SL_WARPS * 32;
 constexpr int SL_CHUNK = SL_THREADS * SL_ROUNDS;
@@ -830,7 +830,7 @@ struct RowPiece {
 
 // Bound by HBM: each thread asks for the pieces of up to CB_K rows before it adds the first.  8192 tokens of
 // eight rows of 2048 bfloat16 take 50 to 55 us (302 MB, 5.5 to 6.0 TB/s), 8191 of six rows of 1031 float32,
-// which start anywhere, 46 us (5.1 TB/s).  (Copying rows ahead into shared memory with cp.async was no
+// which start anywhere and of which one in nine is not there, 46 us (214 MB, 4.6 TB/s).  (Copying rows ahead into shared memory with cp.async was no
 // faster, 54 and 64 us.)
 template <typename T, bool VEC>
 __global__ void __maxnreg__(96)      // four blocks of 160 threads on an SM
@@ -871,9 +871,9 @@ combine_kernel(const T* values, int64_t n_values, const int32_t* slots,
   }
 }
 
-// Gradients.  Bound by HBM: the same 8192 x 8 rows of 2048 bfloat16 take 85 us (570 MB read and written, 6.7
-// TB/s), with 4 us more for the two small kernels ahead.  A block takes CG_K choices of a token, 128 threads
-// (256 threads: 111 us).  A row of values that several choices share needs the sum of their gradients, in a fixed
+// Gradients.  Bound by HBM: the same 8192 x 8 rows of 2048 bfloat16 take 92.5 us with the two small kernels ahead (571 MB
+// read and written, of which 528 reach DRAM at 6.0 TB/s, the rest being found in L2).  A block takes CG_K choices of
+// a token, 128 threads (with 256 threads the large kernel alone took 111 us, with 128 85).  A row of values that several choices share needs the sum of their gradients, in a fixed
 // order.  `users` counts the choices of each row; where the workspace has room for `next`, one number for each choice,
 // `head` and `next` chain them in the order in which they came, and else `head` is the lowest of them.  The
 // blocks of the tokens write the rows with one user, the last blocks of the grid all others.
